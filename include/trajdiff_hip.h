@@ -419,6 +419,65 @@ int tdx_stem_conv_n(const float* x, const float* w, const float* bias, void* out
 int tdx_head_conv_n(const void* a, const float* w, const float* bias, float* out, int32_t B, int32_t L, int32_t C0, int32_t cout,
                     int32_t dtype, void* stream);
 
+/* ---- Sequence operators for long tracks.  No counterpart in the reference, whose attention takes 13 tokens: rotary positions with
+ * several axes (time, longitude, latitude), and attention with a window and a few first tokens that stay visible.  Tensors are
+ * (batch, token, head, channel) with element strides for the first three and contiguous channels, so q, k and v may be slices of one
+ * (B, L, 3C) row matrix. ---- */
+
+enum { TDX_ROTARY_HALVES = 0, TDX_ROTARY_PAIRS = 1 };
+/* Pair i of axis a (n = sections[a] pairs, pairs of axis 0 first) of every head at token (b, t) is turned by the angle
+ *   pos[b, t, a] * base[a]^(-i / n)      (negated when inverse != 0: the backward pass, since a rotation's transpose is its inverse),
+ * (x, y) -> (x cos - y sin, x sin + y cos).  With P = sum of the sections, pair m holds channels (m, m + P) (TDX_ROTARY_HALVES) or
+ * (2m, 2m + 1) (TDX_ROTARY_PAIRS); channels from 2P on are copied.  Angles are formed in 64 bits and reduced before they are rounded:
+ * positions are exact up to what fp32 holds.  out may be x (same strides: in place); any other overlap is not allowed. */
+typedef struct {
+  const void* x;
+  void* out;
+  const float* pos;
+  int64_t x_bs, x_ts, x_hs;          /* element strides of batch, token, head */
+  int64_t out_bs, out_ts, out_hs;
+  int64_t pos_bs, pos_ts, pos_as;    /* 0 allowed: positions shared by the batch */
+  int32_t B, T, H, D;                /* D <= 256 */
+  int32_t dtype, layout, inverse;
+  int32_t naxes;                     /* 1 .. 8 */
+  int32_t sections[8];
+  double base[8];
+} tdx_rotary_desc;
+int tdx_rotary_axes(const tdx_rotary_desc* host_desc, void* stream);
+
+/* Query row i < q_len of sequence b stands at position p = i + k_len - q_len and sees key j iff
+ *   j < k_len,  j <= p + right,  and (j >= p - left or j < sinks)
+ * (left / right < 0: no limit on that side; right = 0 is causal).  Query head h reads key head h / (Hq / Hkv).
+ *   out = softmax over the seen keys of (scale q k^T) times v,   lse = log sum exp of the same scores (natural logarithm, fp32),
+ * rows that see nothing (rows i >= q_len among them) get out = 0 and lse = -inf.  q_lens / k_lens: device int32 (B), or NULL = Tq / Tk;
+ * values are clamped to [0, Tq] / [0, Tk].  What is stored at keys that a row does not see (infinities and NaN too) does not reach it.
+ * D: a multiple of 8, at most 128; scale finite and > 0; pointers, and the byte sizes of the strides, multiples of 16; the token stride
+ * of k and v below 16 MiB; 33 token strides plus one group of head strides of q (and of dout) below 2 GiB.
+ * Softmax statistics and sums are fp32; with bf16 tensors the probabilities (and score gradients) are rounded to bf16 before the
+ * products that take them, the results once at the end.  Summation orders are fixed: results are reproducible. */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;                         /* backward: the forward's result (read) */
+  float* lse;                        /* (B, Hq, Tq); forward: may be NULL; backward: the forward's (read) */
+  int64_t q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, out_bs, out_ts, out_hs;
+  int32_t B, Tq, Tk, Hq, Hkv, D;
+  int32_t dtype;
+  int32_t left, right, sinks;
+  float scale;
+  int32_t reserved;
+  const int32_t *q_lens, *k_lens;
+  void* ws;                          /* device scratch of at least the bytes the matching *_ws_bytes() call returns (NULL if 0); */
+  int64_t ws_bytes;                  /* written before it is read, so calls that do not overlap may share it */
+  /* backward only */
+  const void* dout;                  /* gradient of out */
+  void *dq, *dk, *dv;                /* all three are overwritten (rows i >= q_len, keys j >= k_len: zero) */
+  int64_t dout_bs, dout_ts, dout_hs, dq_bs, dq_ts, dq_hs, dk_bs, dk_ts, dk_hs, dv_bs, dv_ts, dv_hs;
+} tdx_window_attn_desc;
+int64_t tdx_window_attention_ws_bytes(const tdx_window_attn_desc* host_desc);
+int tdx_window_attention(const tdx_window_attn_desc* host_desc, void* stream);
+int64_t tdx_window_attention_bwd_ws_bytes(const tdx_window_attn_desc* host_desc);
+int tdx_window_attention_bwd(const tdx_window_attn_desc* host_desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

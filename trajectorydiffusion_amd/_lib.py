@@ -42,6 +42,21 @@ class PackDesc(C.Structure):
                 ("st", _i64), ("tap_map", _i32 * 3), ("reserved", _i32)]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [("x", _vp), ("out", _vp), ("pos", _vp), ("x_bs", _i64), ("x_ts", _i64), ("x_hs", _i64), ("out_bs", _i64), ("out_ts", _i64),
+                ("out_hs", _i64), ("pos_bs", _i64), ("pos_ts", _i64), ("pos_as", _i64), ("B", _i32), ("T", _i32), ("H", _i32), ("D", _i32),
+                ("dtype", _i32), ("layout", _i32), ("inverse", _i32), ("naxes", _i32), ("sections", _i32 * 8), ("base", C.c_double * 8)]
+
+
+class WindowAttnDesc(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("q_bs", _i64), ("q_ts", _i64), ("q_hs", _i64), ("k_bs", _i64),
+                ("k_ts", _i64), ("k_hs", _i64), ("v_bs", _i64), ("v_ts", _i64), ("v_hs", _i64), ("out_bs", _i64), ("out_ts", _i64), ("out_hs", _i64),
+                ("B", _i32), ("Tq", _i32), ("Tk", _i32), ("Hq", _i32), ("Hkv", _i32), ("D", _i32), ("dtype", _i32), ("left", _i32), ("right", _i32),
+                ("sinks", _i32), ("scale", _f32), ("reserved", _i32), ("q_lens", _vp), ("k_lens", _vp), ("ws", _vp), ("ws_bytes", _i64), ("dout", _vp),
+                ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dout_bs", _i64), ("dout_ts", _i64), ("dout_hs", _i64), ("dq_bs", _i64), ("dq_ts", _i64),
+                ("dq_hs", _i64), ("dk_bs", _i64), ("dk_ts", _i64), ("dk_hs", _i64), ("dv_bs", _i64), ("dv_ts", _i64), ("dv_hs", _i64)]
+
+
 _SIGNATURES = {
     "tdx_last_error": (C.c_char_p, []),
     "tdx_version": (_i32, []),
@@ -101,6 +116,11 @@ _SIGNATURES = {
     "tdx_resample_rows": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "tdx_condmix_gather": (_i32, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp]),
     "tdx_stem_conv_n": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "tdx_rotary_axes": (_i32, [C.POINTER(RotaryDesc), _vp]),
+    "tdx_window_attention_ws_bytes": (_i64, [C.POINTER(WindowAttnDesc)]),
+    "tdx_window_attention": (_i32, [C.POINTER(WindowAttnDesc), _vp]),
+    "tdx_window_attention_bwd_ws_bytes": (_i64, [C.POINTER(WindowAttnDesc)]),
+    "tdx_window_attention_bwd": (_i32, [C.POINTER(WindowAttnDesc), _vp]),
     "tdx_head_conv_n": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
 EXPORTS = tuple(_SIGNATURES)

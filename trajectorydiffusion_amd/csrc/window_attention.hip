@@ -1,0 +1,1311 @@
+// Attention with a window and a few first tokens that stay visible (tdx_window_attention), forward and backward.
+//
+// Which key a row sees: p = i + k_len - q_len;  j < k_len,  j <= p + right,  j >= p - left or j < sinks.
+//
+// Layout of every kernel.  The Hq / Hkv query heads that read one key head are packed into the rows of a tile: row r of (batch, key
+// head) is query r / G, head r % G of the group, so the keys are loaded once for the group and a 32-row tile spans only 32 / G
+// positions of the window.  A wave owns 32 rows as the COLUMNS of its products (32x32 matrix instructions):
+//   S^T (keys x rows) = K Q^T, the accumulator of lane (n = lane & 31, h = lane >> 5) then holds, for row n, the scores of the keys
+//   8 g + 4 h + r (g, r = 0..3): softmax statistics are one number per lane (and its partner n + 32), and the probabilities are
+//   already where the second product wants its right operand, O^T (channels x rows) = V^T P^T, once its contraction index is
+//   taken in the order the scores are held in.  V^T then has to be read from LDS along the keys: with bf16 by the transposing
+//   LDS read, which hands lane i of 16 lanes column i of a 4 x 16 tile; with fp32 by plain 4-byte reads (one key per lane half).
+// K and V tiles are staged in LDS as they lie in memory (direct loads, 16 bytes a lane); the 16-byte pieces of a row are permuted
+// (swz) so that neither the row reads nor the transposed ones meet in a bank.
+#include "tdx_common.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4_t;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4_t;
+typedef __attribute__((address_space(3))) float lds_f32_t;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kFar = 1 << 30;         // a limit no position reaches (lengths stay below 2^28)
+constexpr uint32_t kOutside = 0x80000000u;
+
+struct WaArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;
+  int B, Tq, Tk, Hkv, G, D;
+  int left, right, sinks;
+  float scale;
+  const int *q_lens, *k_lens;
+  int ntiles, nsplit;                 // row (backward: or key) tiles of a (batch, key head); key (backward: row) splits
+  float* ws;
+  // backward
+  const void* dout;
+  void *dq, *dk, *dv;
+  long do_bs, do_ts, do_hs, dq_bs, dq_ts, dq_hs, dk_bs, dk_ts, dk_hs, dv_bs, dv_ts, dv_hs;
+  float *stat, *part;                 // per 32 rows {log2-sum-exp, delta}; shares of the sinks' gradients
+  int ntiles32, nparts, sink_rows;    // row tiles of 32; shares; sinks rounded up to 32 (0: no separate pass over the sinks)
+};
+
+// ---- geometry of a staged tile ------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+struct Geo {
+  static constexpr int ES = sizeof(T), PITCH = DP * ES, CH = PITCH / 16, NC = PITCH / 32, ND = DP / 32, RPI = 1024 / PITCH;
+};
+// a 32-row operand held in registers: row lane & 31, the 16-byte pieces of one lane half
+template <typename T, int DP>
+using Frags = u32x4[Geo<T, DP>::NC];
+// Permutation of the 16-byte pieces of row `row`.  Row reads (16 rows, one piece): the bank groups must differ over 16 rows.
+// Transposed reads: bf16 takes 4 rows x 64 bytes at a time (rows 4a .. 4a+3 must differ in the 64-byte block), fp32 the 128 bytes of
+// rows R and R + 4 (they must differ in the 128-byte block).
+template <typename T, int DP>
+__device__ __forceinline__ int swz(int row) {
+  constexpr int CH = Geo<T, DP>::CH;
+  if constexpr (CH == 4) return (row >> 2) & 3;
+  else if constexpr (CH == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else if constexpr (sizeof(T) == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else return (row & 3) | (((row >> 2) & 1) << 3) | (((row >> 3) & 1) << 2);
+}
+
+__device__ __forceinline__ u32x4 lds_ld16(uint32_t a) { return *reinterpret_cast<lds_u32x4_t*>(a); }
+__device__ __forceinline__ float lds_ld4(uint32_t a) { return *reinterpret_cast<lds_f32_t*>(a); }
+
+__device__ __forceinline__ u32x4 make_srd(const void* base) {
+  const uint64_t a = (uint64_t)base;
+  u32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+  r[2] = 0x7fffffffu;
+  r[3] = 0x00020000u;
+  return r;
+}
+// 64 lanes x 16 B from srd[voff] to LDS[lds_addr + 16 * lane]; lanes with voff >= 2^31 - 1 write zeros.  Issued from asm so that the
+// compiler does not order later LDS reads behind it: the kernels wait for their loads themselves (vmcnt, then a barrier).
+__device__ __forceinline__ void dma16(uint32_t lds_addr, uint32_t voff, const u32x4& srd) {
+  uint32_t keep;
+  lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "s"(lds_addr), "v"(voff), "s"(srd)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// every wave's LDS traffic is complete, then the barrier (without a release fence, which would wait for the direct loads in flight)
+__device__ __forceinline__ void wg_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Stages `ROWS` rows (row 0 at `base`, `stride` bytes apart) by NW waves; rows from `valid` on and channels from `dbytes` on are zeros.
+template <typename T, int DP, int ROWS, int NW>
+__device__ __forceinline__ void stage_rows(uint32_t lds, const char* base, uint32_t stride, int valid, int dbytes, int wave, int lane) {
+  using G = Geo<T, DP>;
+  constexpr int TOTAL = ROWS * G::PITCH / 1024;
+  const u32x4 srd = make_srd(base);
+#pragma unroll
+  for (int n = 0; n < (TOTAL + NW - 1) / NW; ++n) {
+    const int it = wave + n * NW;
+    if (TOTAL % NW == 0 || it < TOTAL) {
+      const int row = it * G::RPI + lane / G::CH;
+      const int chunk = (lane % G::CH) ^ swz<T, DP>(row);
+      const bool ok = row < valid && chunk * 16 < dbytes;
+      dma16(lds + it * 1024, ok ? (uint32_t)row * stride + chunk * 16 : kOutside, srd);
+    }
+  }
+}
+
+// ---- matrix steps ---------------------------------------------------------------------------------------------------------------
+// acc += A B over the 32 bytes of channels that a fragment pair holds (lane half h: bytes 16 h .. 16 h + 15 of the piece, both sides alike)
+__device__ __forceinline__ void mma_piece(f32x16& acc, const u32x4& a, const u32x4& b, __bf16) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_piece(f32x16& acc, const u32x4& a, const u32x4& b, float) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[s]), __uint_as_float(b[s]), acc, 0, 0, 0);
+}
+// acc (32 tile rows x 32 columns) = tile rows [row0, row0 + 32) times the fragments b
+template <typename T, int DP>
+__device__ __forceinline__ void rows_times(f32x16& acc, uint32_t tile, int row0, const Frags<T, DP>& b, int lane) {
+  using G = Geo<T, DP>;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  const int row = row0 + (lane & 31);
+  const uint32_t a0 = tile + row * G::PITCH;
+  const int c0 = (lane >> 5) ^ swz<T, DP>(row);
+#pragma unroll
+  for (int c = 0; c < G::NC; ++c) mma_piece(acc, lds_ld16(a0 + ((c0 ^ (2 * c)) << 4)), b[c], T());
+}
+// acc[dt] (channels 32 dt .. + 31 x 32 columns) += (tile rows [row0, row0 + 32))^T p, p as rows_times left it: element i of a lane is tile
+// row row0 + 8 (i / 4) + 4 h + i % 4
+template <int DP>
+__device__ __forceinline__ void cols_times(f32x16 (&acc)[DP / 32], uint32_t tile, int row0, const float (&p)[16], int lane, __bf16) {
+  using G = Geo<__bf16, DP>;
+  const int rl = 4 * (lane >> 5) + ((lane >> 2) & 3);              // the row this lane addresses inside a group of 8
+  const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);      // and the 16-byte piece inside the 64 bytes of 32 channels
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {                                     // 16 tile rows a step
+    float pe[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pe[j] = p[8 * s + j];
+    const bf16x8 b = __builtin_bit_cast(bf16x8, Elem<__bf16>::pack(pe));
+    const int ra = row0 + 16 * s + rl, rb = ra + 8;
+#pragma unroll
+    for (int dt = 0; dt < G::ND; ++dt) {
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<lds_s16x4_t*>(tile + ra * G::PITCH + (((4 * dt + piece) ^ swz<__bf16, DP>(ra)) << 4) + 8 * (lane & 1)));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<lds_s16x4_t*>(tile + rb * G::PITCH + (((4 * dt + piece) ^ swz<__bf16, DP>(rb)) << 4) + 8 * (lane & 1)));
+      const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[dt], 0, 0, 0);
+    }
+  }
+}
+template <int DP>
+__device__ __forceinline__ void cols_times(f32x16 (&acc)[DP / 32], uint32_t tile, int row0, const float (&p)[16], int lane, float) {
+  using G = Geo<float, DP>;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {                                    // two tile rows a step: one for each lane half
+    const int row = row0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+#pragma unroll
+    for (int dt = 0; dt < G::ND; ++dt) {
+      const int d = 32 * dt + (lane & 31);
+      const float a = lds_ld4(tile + row * G::PITCH + (((d >> 2) ^ swz<float, DP>(row)) << 4) + 4 * (d & 3));
+      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[dt], 0, 0, 0);
+    }
+  }
+}
+
+__device__ __forceinline__ float half_max(float v) {   // with the partner lane of the other half
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- one sequence ---------------------------------------------------------------------------------------------------------------
+struct Seq {
+  int ql, kl, shift;
+};
+__device__ __forceinline__ Seq seq_of(const WaArgs& a, int b) {
+  Seq s;
+  s.ql = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
+  s.kl = a.k_lens ? min(max(a.k_lens[b], 0), a.Tk) : a.Tk;
+  s.shift = s.kl - s.ql;
+  return s;
+}
+// Key tiles of BN keys that rows at positions [p0, p1] may see: na tiles from key 0 (the sinks, when the window begins behind them),
+// then nb tiles from key `start`.  No key lies in two tiles; the mask decides inside a tile.
+struct Tiles {
+  int na, nb, start;
+};
+__device__ __forceinline__ Tiles tiles_of(const WaArgs& a, const Seq& s, int p0, int p1, int bn) {
+  Tiles t;
+  const int hi = min(s.kl, p1 + a.right + 1);
+  const int lo = max(0, p0 - a.left);
+  const int sink = lo > 0 ? min(a.sinks, hi) : 0;
+  t.na = sink > 0 ? (sink + bn - 1) / bn : 0;
+  t.start = max(lo, t.na * bn);
+  t.nb = hi > t.start ? (hi - t.start + bn - 1) / bn : 0;
+  return t;
+}
+__device__ __forceinline__ int tile_start(const Tiles& t, int i, int bn) { return i < t.na ? i * bn : t.start + (i - t.na) * bn; }
+
+// What 32 keys from j0 are to rows at positions [p0, p1]: 0 unseen, 1 seen in part, 2 seen by all
+__device__ __forceinline__ int seen_class(const WaArgs& a, const Seq& s, int j0, int p0, int p1) {
+  if (j0 >= s.kl || j0 > p1 + a.right || (j0 + 31 < p0 - a.left && j0 >= a.sinks)) return 0;
+  return j0 + 31 < s.kl && j0 + 31 <= p0 + a.right && (j0 >= p1 - a.left || j0 + 31 < a.sinks) ? 2 : 1;
+}
+
+// ---- online softmax ----------------------------------------------------------------------------------------------------------------
+// m is the running maximum of the raw scores that the exponents are taken against.  It follows the true maximum only when that is more
+// than 8 powers of two above it: the terms stay below 2^8, nothing is lost in fp32 (nor in bf16, whose exponent is as wide), and the
+// accumulators are rescaled in the first tiles of a row only.
+template <int ND>
+__device__ __forceinline__ void softmax_step(float (&s)[16], float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
+  float t = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
+  t = half_max(t);
+  if (__ballot(t > m + slack)) {
+    const float mn = fmaxf(m, t);
+    const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= f;
+  }
+  const float off = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -off));
+    l += s[i];
+  }
+}
+// scores of keys a row does not see become -inf (element i: key j0 + 8 (i / 4) + 4 h + i % 4)
+__device__ __forceinline__ void mask_scores(float (&s)[16], const WaArgs& a, const Seq& q, int j0, int p, int lane) {
+  const int base = j0 + 4 * (lane >> 5);
+  const int hi = min(p + a.right, q.kl - 1) - base, lo = p - a.left - base, sk = a.sinks - base;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int e = 8 * (i >> 2) + (i & 3);
+    if (!(e <= hi && (e >= lo || e < sk))) s[i] = -INFINITY;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4]);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, const float (&v)[4]) {
+  *reinterpret_cast<f32x4*>(p) = (f32x4){v[0], v[1], v[2], v[3]};
+}
+template <>
+__device__ __forceinline__ void store4<__bf16>(__bf16* p, const float (&v)[4]) {
+  float e[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+  const u32x4 w = Elem<__bf16>::pack(e);
+  *reinterpret_cast<u32x2*>(p) = (u32x2){w[0], w[1]};
+}
+
+// A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN.  A row whose sum of exponentials is
+// a number but whose result is not is therefore taken again, over the keys it sees alone: one wave, its lanes split the channels.
+template <typename T>
+__device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, int g, float m, float l, int lane) {
+  const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + (long)(hk * a.G + g) * a.q_hs;
+  const T* k = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
+  const T* v = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
+  T* o = (T*)a.out + b * a.o_bs + i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
+  const int p = i + s.shift, hi = min(p + a.right, s.kl - 1), lo = max(p - a.left, 0);
+  const int d0 = lane, d1 = lane + 64;
+  const float q0 = d0 < a.D ? Elem<T>::ld(q + d0) : 0.f, q1 = d1 < a.D ? Elem<T>::ld(q + d1) : 0.f;
+  const float c = a.scale * kLog2e, off = m * c;
+  float o0 = 0.f, o1 = 0.f;
+  for (int j = 0; j <= hi; ++j) {
+    if (j < lo && j >= a.sinks) j = lo;
+    if (j > hi) break;
+    const T *kr = k + j * a.k_ts, *vr = v + j * a.v_ts;
+    float d = (d0 < a.D ? q0 * Elem<T>::ld(kr + d0) : 0.f) + (d1 < a.D ? q1 * Elem<T>::ld(kr + d1) : 0.f);
+    d = wave_sum(d);
+    const float w = __builtin_amdgcn_exp2f(fmaf(d, c, -off));
+    if (d0 < a.D) o0 = fmaf(w, Elem<T>::ld(vr + d0), o0);
+    if (d1 < a.D) o1 = fmaf(w, Elem<T>::ld(vr + d1), o1);
+  }
+  if (d0 < a.D) o[d0] = (T)(o0 / l);
+  if (d1 < a.D) o[d1] = (T)(o1 / l);
+}
+
+// blockIdx -> work item so that each XCD (workgroups go round the 8 of them) takes a contiguous run of items: neighbours read the same keys
+__device__ __forceinline__ int xcd_item(int n) {
+  const int per = n >> 3, rest = n & 7, x = blockIdx.x & 7;
+  return x * per + min(x, rest) + (blockIdx.x >> 3);
+}
+
+// Q (or dO) fragments of row `row` (a query head's row), zero beyond the channels or when !ok
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags(Frags<T, DP>& f, const T* row, bool ok, int D, int lane) {
+#pragma unroll
+  for (int c = 0; c < Geo<T, DP>::NC; ++c) {
+    const int d = (32 * c + 16 * (lane >> 5)) / (int)sizeof(T);
+    f[c] = ok && d < D ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u};
+  }
+}
+
+// Uses the fragments, so that the compiler's wait for their loads stands here and not inside a loop, where it would also wait for the
+// direct loads in flight.
+template <typename F, int N>
+__device__ __forceinline__ void arrived(F (&f)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; ++c) asm volatile("" : "+v"(f[c]));
+}
+
+// ---- forward, many rows: 4 waves x 32 rows, K and V tiles of BN keys double-buffered in LDS ------------------------------------------
+template <typename T, int DP, int BN>
+__global__ __launch_bounds__(256, 2) void window_attn_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geo<T, DP>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  constexpr uint32_t TILE = BN * G::PITCH;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = xcd_item(gridDim.x);
+  const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  const int R = a.Tq * a.G, r0 = tile * 128, rw = r0 + wave * 32;
+  const int rend = min(r0 + 128, s.ql * a.G);            // rows of the tile that see anything at all
+  const int r = rw + (lane & 31), i = r / a.G, g = r - i * a.G;
+  const bool row_ok = r < s.ql * a.G;
+  const T* kb = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
+  const T* vb = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
+  const uint32_t ks = a.k_ts * G::ES, vs = a.v_ts * G::ES;
+  const int dbytes = a.D * G::ES;
+  f32x16 o[G::ND];
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const float c = a.scale * kLog2e, slack = 8.0f / c;
+  if (r0 < rend) {
+    Frags<T, DP> qf;
+    load_frags<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
+    arrived(qf);
+    const int p = i + s.shift;
+    const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;   // positions of this wave's rows
+    const bool wave_ok = rw < rend;
+    const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, BN);
+    const int n = t.na + t.nb;
+    auto stage = [&](int it) {
+      const int j0 = tile_start(t, it, BN);
+      const uint32_t dst = lds + (it & 1) * 2 * TILE;
+      stage_rows<T, DP, BN, 4>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, wave, lane);
+      stage_rows<T, DP, BN, 4>(dst + TILE, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, wave, lane);
+    };
+    if (n > 0) stage(0);
+    for (int it = 0; it < n; ++it) {
+      wait_vm<0>();
+      wg_barrier();
+      if (it + 1 < n) stage(it + 1);
+      const int j0 = tile_start(t, it, BN);
+      const uint32_t kt = lds + (it & 1) * 2 * TILE, vt = kt + TILE;
+#pragma unroll
+      for (int sub = 0; sub < BN / 32; ++sub) {
+        const int cls = wave_ok ? seen_class(a, s, j0 + 32 * sub, wp0, wp1) : 0;
+        if (!cls) continue;
+        f32x16 acc;
+        rows_times<T, DP>(acc, kt, 32 * sub, qf, lane);
+        float sc[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+        if (cls == 1) mask_scores(sc, a, s, j0 + 32 * sub, p, lane);
+        softmax_step<G::ND>(sc, m, l, o, c, slack);
+        cols_times<DP>(o, vt, 32 * sub, sc, lane, T());
+      }
+    }
+    l = half_sum(l);
+  }
+  // rows the sequence does not have: zero, like rows that see nothing
+  const float inv = row_ok && l != 0.f ? 1.0f / l : 0.f;
+  bool bad = false;
+  if (r < R) {
+    T* orow = (T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
+    const int h4 = 4 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
+          bad |= v[x] != v[x];
+        }
+        if (32 * d + 8 * e + h4 < a.D) store4<T>(orow + 32 * d + 8 * e + h4, v);
+      }
+    if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l) : -INFINITY;
+  }
+  uint64_t again = __ballot(bad && row_ok && l == l);
+  again = (again | (again >> 32)) & 0xffffffffull;
+  while (again) {
+    const int n = __builtin_ctzll(again);
+    again &= again - 1;
+    row_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(m, n, 64), __shfl(l, n, 64), lane);
+  }
+#endif
+}
+
+// ---- forward, few rows: one 32-row tile per workgroup, its waves (and the splits) share the keys -------------------------------------
+// Single tokens over a cache are bound by the reads of K and V: every wave streams its own key tiles through a ring of two stages in LDS, so
+// a compute unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.
+template <typename T, int DP>
+struct Few {
+  using G = Geo<T, DP>;
+  static constexpr int STAGE = 2 * 32 * G::PITCH;                               // 32 keys of K and of V
+  static constexpr int NW = G::PITCH > 256 ? 2 : 4;
+  static constexpr int RING = 2 * STAGE;
+  static constexpr int OPITCH = DP + 4;                                          // floats of a row in the exchange
+  static constexpr int XCHG = NW * 32 * (OPITCH + 2) * 4;
+  static constexpr int LDS = NW * RING > XCHG ? NW * RING : XCHG;
+};
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geo<T, DP>;
+  using F = Few<T, DP>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = xcd_item(gridDim.x);
+  const int split = item % a.nsplit, bht = item / a.nsplit, tile = bht % a.ntiles, bh = bht / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  const int R = a.Tq * a.G, r0 = tile * 32, rend = min(r0 + 32, s.ql * a.G);
+  const int r = r0 + (lane & 31), i = r / a.G, g = r - i * a.G;
+  const bool row_ok = r < s.ql * a.G;
+  const T* kb = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
+  const T* vb = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
+  const uint32_t ks = a.k_ts * G::ES, vs = a.v_ts * G::ES;
+  const int dbytes = a.D * G::ES;
+  f32x16 o[G::ND];
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const float c = a.scale * kLog2e, slack = 8.0f / c;
+  if (r0 < rend) {
+    Frags<T, DP> qf;
+    load_frags<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
+    const int p = i + s.shift, p0 = r0 / a.G + s.shift, p1 = (rend - 1) / a.G + s.shift;
+    const Tiles t = tiles_of(a, s, p0, p1, 32);
+    const int n = t.na + t.nb, per = (n + a.nsplit - 1) / a.nsplit;
+    const int first = split * per + wave, last = min(n, (split + 1) * per);
+    const uint32_t ring = lds + wave * F::RING;
+    auto stage = [&](int it, int buf) {
+      const int j0 = tile_start(t, it, 32);
+      const uint32_t dst = ring + buf * F::STAGE;
+      stage_rows<T, DP, 32, 1>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, 0, lane);
+      stage_rows<T, DP, 32, 1>(dst + F::STAGE / 2, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, 0, lane);
+    };
+    arrived(qf);               // from here on only direct loads are counted
+    if (first < last) stage(first, 0);
+    int buf = 0;
+    for (int it = first; it < last; it += F::NW, buf ^= 1) {
+      if (it + F::NW < last) {
+        stage(it + F::NW, buf ^ 1);
+        wait_vm<2 * 32 * G::PITCH / 1024>();
+      } else {
+        wait_vm<0>();
+      }
+      const int j0 = tile_start(t, it, 32);
+      const uint32_t kt = ring + buf * F::STAGE, vt = kt + F::STAGE / 2;
+      const int cls = seen_class(a, s, j0, p0, p1);
+      if (cls) {
+        f32x16 acc;
+        rows_times<T, DP>(acc, kt, 0, qf, lane);
+        float sc[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+        if (cls == 1) mask_scores(sc, a, s, j0, p, lane);
+        softmax_step<G::ND>(sc, m, l, o, c, slack);
+        cols_times<DP>(o, vt, 0, sc, lane, T());
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage has been read before the ring comes round to it
+    }
+    l = half_sum(l);
+  }
+  // the waves' shares are joined in LDS, in wave order
+  __syncthreads();
+  float* xo = reinterpret_cast<float*>(smem);                                   // [NW][32][OPITCH]
+  float* xm = xo + F::NW * 32 * F::OPITCH;                                      // [NW][32] m, then l
+  float* xl = xm + F::NW * 32;
+  {
+    const int n = lane & 31, h4 = 4 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(xo + (wave * 32 + n) * F::OPITCH + 32 * d + 8 * e + h4) =
+            (f32x4){o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+    if (lane < 32) xm[wave * 32 + n] = m, xl[wave * 32 + n] = l;
+  }
+  __syncthreads();
+  constexpr int NT = F::NW * 64, D4 = DP / 4, RPP = NT / D4;                      // rows of one pass of the workgroup
+  for (int n0 = 0; n0 < 32; n0 += RPP) {
+    const int n = n0 + threadIdx.x / D4, d = 4 * (threadIdx.x % D4);
+    if (n >= 32) continue;
+    float mm = xm[n];
+#pragma unroll
+    for (int w = 1; w < F::NW; ++w) mm = fmaxf(mm, xm[w * 32 + n]);
+    float ll = 0.f;
+    f32x4 oo = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < F::NW; ++w) {
+      const float mw = xm[w * 32 + n];
+      const float f = mw == mm ? 1.f : __builtin_amdgcn_exp2f((mw - mm) * c);
+      if (xl[w * 32 + n] == 0.f) continue;                                       // a share that saw nothing
+      ll += f * xl[w * 32 + n];
+      const f32x4 ow = *reinterpret_cast<const f32x4*>(xo + (w * 32 + n) * F::OPITCH + d);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) oo[x] = fmaf(f, ow[x], oo[x]);
+    }
+    if (a.nsplit > 1) {
+      if (r0 + n < R) {
+        float* part = a.ws + ((long)bht * a.nsplit + split) * 32 * (DP + 2);
+        *reinterpret_cast<f32x4*>(part + n * DP + d) = oo;
+        if (d == 0) part[32 * DP + n] = mm, part[32 * DP + 32 + n] = ll;
+      }
+      continue;
+    }
+    const int rr = r0 + n, ii = rr / a.G, gg = rr - ii * a.G;
+    bool bad = false;
+    const bool ok = rr < s.ql * a.G;
+    if (rr < R) {
+      const float inv = ok && ll != 0.f ? 1.0f / ll : 0.f;
+      float v[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        v[x] = inv != 0.f ? oo[x] * inv : (ll != ll ? ll : 0.f);
+        bad |= v[x] != v[x];
+      }
+      if (d < a.D) store4<T>((T*)a.out + b * a.o_bs + (long)ii * a.o_ts + (long)(hk * a.G + gg) * a.o_hs + d, v);
+      if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? mm * a.scale + __logf(ll) : -INFINITY;
+    }
+    uint64_t again = __ballot(bad && ok && ll == ll);
+    while (again) {                                                              // D4 (8 .. 32) lanes hold a row
+      const int f = __builtin_ctzll(again), row_lane = f - f % D4;
+      again &= ~(((D4 == 64 ? 0ull : (1ull << D4)) - 1) << row_lane);
+      row_again<T>(a, s, b, hk, __shfl(ii, f, 64), __shfl(gg, f, 64), __shfl(mm, f, 64), __shfl(ll, f, 64), lane);
+    }
+  }
+#endif
+}
+
+// Joins the key splits of one row: 256 threads = 4 channels each x groups that take the splits in turn, then the groups in order.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int D4 = DP / 4, NG = 256 / D4;
+  __shared__ f32x4 xo[NG][D4];
+  __shared__ float xm[NG], xl[NG];
+  const int R = a.Tq * a.G;
+  const int rr = blockIdx.x % R, bh = blockIdx.x / R, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int tile = rr >> 5, n = rr & 31;
+  const int grp = threadIdx.x / D4, dv = threadIdx.x % D4;
+  const Seq s = seq_of(a, b);
+  const float c = a.scale * kLog2e;
+  const float* base = a.ws + ((long)(bh * a.ntiles + tile) * a.nsplit) * 32 * (DP + 2);
+  float mm = -INFINITY, ll = 0.f;
+  f32x4 oo = {0.f, 0.f, 0.f, 0.f};
+  for (int sp = grp; sp < a.nsplit; sp += NG) {
+    const float* part = base + (long)sp * 32 * (DP + 2);
+    const float mw = part[32 * DP + n], lw = part[32 * DP + 32 + n];
+    const f32x4 ow = *reinterpret_cast<const f32x4*>(part + n * DP + 4 * dv);
+    if (lw == 0.f) continue;
+    const float mn = fmaxf(mm, mw);
+    const float f0 = mm == mn ? 1.f : __builtin_amdgcn_exp2f((mm - mn) * c), f1 = mw == mn ? 1.f : __builtin_amdgcn_exp2f((mw - mn) * c);
+    mm = mn;
+    ll = ll * f0 + lw * f1;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) oo[x] = oo[x] * f0 + ow[x] * f1;
+  }
+  xo[grp][dv] = oo;
+  if (dv == 0) xm[grp] = mm, xl[grp] = ll;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  float M = xm[0];
+  for (int k = 1; k < NG; ++k) M = fmaxf(M, xm[k]);
+  float L = 0.f;
+  f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  const int x4 = threadIdx.x % D4;
+  for (int k = 0; k < NG; ++k) {
+    if (xl[k] == 0.f) continue;
+    const float f = xm[k] == M ? 1.f : __builtin_amdgcn_exp2f((xm[k] - M) * c);
+    L += f * xl[k];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) O[x] = fmaf(f, xo[k][x4][x], O[x]);
+  }
+  const int i = rr / a.G, g = rr - i * a.G;
+  const bool ok = i < s.ql;
+  const float inv = ok && L != 0.f ? 1.0f / L : 0.f;
+  float v[4];
+  bool bad = false;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    v[x] = inv != 0.f ? O[x] * inv : (L != L ? L : 0.f);
+    bad |= v[x] != v[x];
+  }
+  if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store4<T>((T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs + 4 * threadIdx.x, v);
+  if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L) : -INFINITY;
+  if (__ballot(bad && ok && L == L)) row_again<T>(a, s, b, hk, i, g, M, L, threadIdx.x);
+#endif
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------------------------
+// With P = exp(scale q k^T - lse), delta = sum_d dO O, dP = dO V^T, dS = P (dP - delta):
+//   dV = P^T dO,   dQ = scale dS K,   dK = scale dS^T Q.
+// Two kernels take S and dP again, each in the orientation that leaves its sums in one wave's registers, so nothing is added by atomics
+// and the order of every sum is fixed: dQ walks the keys of 128 rows (like the forward pass), dK / dV walk the rows that see 32 keys a
+// wave.  The sinks are seen by every later row: their rows beyond the window are cut into shares that run as workgroups of their own.
+
+// The gradient of one query row, over the keys it sees alone (see row_again)
+template <typename T>
+__device__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, int g, float lse2, float delta, int lane) {
+  const long hq = (long)(hk * a.G + g);
+  const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + hq * a.q_hs;
+  const T* dO = (const T*)a.dout + b * a.do_bs + i * a.do_ts + hq * a.do_hs;
+  const T* k = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
+  const T* v = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
+  T* dq = (T*)a.dq + b * a.dq_bs + i * a.dq_ts + hq * a.dq_hs;
+  const int p = i + s.shift, hi = min(p + a.right, s.kl - 1), lo = max(p - a.left, 0);
+  const int d0 = lane, d1 = lane + 64;
+  const bool on0 = d0 < a.D, on1 = d1 < a.D;
+  const float q0 = on0 ? Elem<T>::ld(q + d0) : 0.f, q1 = on1 ? Elem<T>::ld(q + d1) : 0.f;
+  const float g0 = on0 ? Elem<T>::ld(dO + d0) : 0.f, g1 = on1 ? Elem<T>::ld(dO + d1) : 0.f;
+  const float c = a.scale * kLog2e;
+  float r0 = 0.f, r1 = 0.f;
+  for (int j = 0; j <= hi; ++j) {
+    if (j < lo && j >= a.sinks) j = lo;
+    if (j > hi) break;
+    const T *kr = k + j * a.k_ts, *vr = v + j * a.v_ts;
+    const float k0 = on0 ? Elem<T>::ld(kr + d0) : 0.f, k1 = on1 ? Elem<T>::ld(kr + d1) : 0.f;
+    const float sc = wave_sum((on0 ? q0 * k0 : 0.f) + (on1 ? q1 * k1 : 0.f));
+    const float dp = wave_sum((on0 ? g0 * Elem<T>::ld(vr + d0) : 0.f) + (on1 ? g1 * Elem<T>::ld(vr + d1) : 0.f));
+    const float ds = __builtin_amdgcn_exp2f(fmaf(sc, c, -lse2)) * (dp - delta);
+    r0 = fmaf(ds, k0, r0);
+    r1 = fmaf(ds, k1, r1);
+  }
+  if (on0) dq[d0] = (T)(r0 * a.scale);
+  if (on1) dq[d1] = (T)(r1 * a.scale);
+}
+
+template <typename T, int DP, int BN, int OCC>
+__global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geo<T, DP>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  constexpr uint32_t TILE = BN * G::PITCH;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = xcd_item(gridDim.x);
+  const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  const int R = a.Tq * a.G, r0 = tile * 128, rw = r0 + wave * 32;
+  const int rend = min(r0 + 128, s.ql * a.G);
+  const int r = rw + (lane & 31), i = r / a.G, g = r - i * a.G;
+  const long hq = (long)(hk * a.G + g);
+  const bool row_ok = r < s.ql * a.G;
+  const T* kb = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
+  const T* vb = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
+  const uint32_t ks = a.k_ts * G::ES, vs = a.v_ts * G::ES;
+  const int dbytes = a.D * G::ES;
+  f32x16 dq[G::ND];
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+  Frags<T, DP> qf, df;
+  load_frags<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
+  load_frags<T, DP>(df, (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs, row_ok, a.D, lane);
+  float delta = 0.f, lse = -INFINITY;
+  {
+    const T* orow = (const T*)a.out + b * a.o_bs + (long)i * a.o_ts + hq * a.o_hs;
+#pragma unroll
+    for (int x = 0; x < G::NC; ++x) {
+      const int d = (32 * x + 16 * (lane >> 5)) / (int)sizeof(T);
+      if (row_ok && d < a.D) {
+        float ov[Elem<T>::kVec], dv[Elem<T>::kVec];
+        Elem<T>::unpack(*reinterpret_cast<const u32x4*>(orow + d), ov);
+        Elem<T>::unpack(df[x], dv);
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e) delta = fmaf(ov[e], dv[e], delta);
+      }
+    }
+    if (row_ok) lse = a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i];
+  }
+  delta = half_sum(delta);
+  // a row that sees nothing has lse = -inf: +inf makes its probabilities 0
+  const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
+  if (lse == -INFINITY) delta = 0.f;
+  {
+    float* st = a.stat + ((long)bh * a.ntiles32 + tile * 4 + wave) * 64;
+    st[lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
+  }
+  arrived(qf);
+  arrived(df);
+  const float c = a.scale * kLog2e;
+  if (r0 < rend) {
+    const int p = i + s.shift;
+    const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;
+    const bool wave_ok = rw < rend;
+    const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, BN);
+    const int n = t.na + t.nb;
+    auto stage = [&](int it) {
+      const int j0 = tile_start(t, it, BN);
+      const uint32_t dst = lds + (it & 1) * 2 * TILE;
+      stage_rows<T, DP, BN, 4>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, wave, lane);
+      stage_rows<T, DP, BN, 4>(dst + TILE, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, wave, lane);
+    };
+    if (n > 0) stage(0);
+    for (int it = 0; it < n; ++it) {
+      wait_vm<0>();
+      wg_barrier();
+      if (it + 1 < n) stage(it + 1);
+      const int j0 = tile_start(t, it, BN);
+      const uint32_t kt = lds + (it & 1) * 2 * TILE, vt = kt + TILE;
+#pragma unroll
+      for (int sub = 0; sub < BN / 32; ++sub) {
+        const int cls = wave_ok ? seen_class(a, s, j0 + 32 * sub, wp0, wp1) : 0;
+        if (!cls) continue;
+        f32x16 acc, dp;
+        rows_times<T, DP>(acc, kt, 32 * sub, qf, lane);
+        rows_times<T, DP>(dp, vt, 32 * sub, df, lane);
+        float sc[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -lse2)) * (dp[e] - delta);
+        if (cls == 1) {
+          const int base = j0 + 32 * sub + 4 * (lane >> 5);
+          const int hi = min(p + a.right, s.kl - 1) - base, lo = p - a.left - base, sk = a.sinks - base;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int x = 8 * (e >> 2) + (e & 3);
+            if (!(x <= hi && (x >= lo || x < sk))) sc[e] = 0.f;
+          }
+        }
+        cols_times<DP>(dq, kt, 32 * sub, sc, lane, T());
+      }
+    }
+  }
+  bool bad = false;
+  if (r < R) {
+    T* drow = (T*)a.dq + b * a.dq_bs + (long)i * a.dq_ts + hq * a.dq_hs;
+    const int h4 = 4 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          v[x] = row_ok ? dq[d][4 * e + x] * a.scale : 0.f;
+          bad |= v[x] != v[x];
+        }
+        if (32 * d + 8 * e + h4 < a.D) store4<T>(drow + 32 * d + 8 * e + h4, v);
+      }
+  }
+  uint64_t again = __ballot(bad && lse2 == lse2 && delta == delta);
+  again = (again | (again >> 32)) & 0xffffffffull;
+  while (again) {
+    const int n = __builtin_ctzll(again);
+    again &= again - 1;
+    dq_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(lse2, n, 64), __shfl(delta, n, 64), lane);
+  }
+#endif
+}
+
+// Stages 32 packed rows (query i, head g of the group) of q or dout from row r0: row r at (r / G) * ts + (r % G) * hs
+template <typename T, int DP, int NW>
+__device__ __forceinline__ void stage_packed(uint32_t lds, const T* base, long ts, long hs, int gsize, int r0, int rend, int dbytes, int wave, int lane) {
+  using G = Geo<T, DP>;
+  constexpr int TOTAL = 32 * G::PITCH / 1024;
+  const int i0 = r0 / gsize;
+  const u32x4 srd = make_srd(base + i0 * ts);
+  const uint32_t tsb = ts * G::ES, hsb = hs * G::ES;
+#pragma unroll
+  for (int n = 0; n < (TOTAL + NW - 1) / NW; ++n) {
+    const int it = wave + n * NW;
+    if (TOTAL % NW == 0 || it < TOTAL) {
+      const int row = it * G::RPI + lane / G::CH;
+      const int chunk = (lane % G::CH) ^ swz<T, DP>(row);
+      const int i = (r0 + row) / gsize, g = r0 + row - i * gsize;
+      const bool ok = r0 + row < rend && chunk * 16 < dbytes;
+      dma16(lds + it * 1024, ok ? (uint32_t)(i - i0) * tsb + (uint32_t)g * hsb + chunk * 16 : kOutside, srd);
+    }
+  }
+}
+// 32 rows' {log2-sum-exp, delta}: 256 bytes, by one wave
+__device__ __forceinline__ void stage_stat(uint32_t lds, const float* st, int lane) {
+  dma16(lds, lane < 16 ? lane * 16u : kOutside, make_srd(st));
+}
+
+// The gradients of one key (and value) row over the query rows that see it alone (see row_again)
+template <typename T>
+__device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, int lane) {
+  const T* k = (const T*)a.k + b * a.k_bs + j * a.k_ts + hk * a.k_hs;
+  const T* v = (const T*)a.v + b * a.v_bs + j * a.v_ts + hk * a.v_hs;
+  const int d0 = lane, d1 = lane + 64;
+  const bool on0 = d0 < a.D, on1 = d1 < a.D;
+  const float k0 = on0 ? Elem<T>::ld(k + d0) : 0.f, k1 = on1 ? Elem<T>::ld(k + d1) : 0.f;
+  const float v0 = on0 ? Elem<T>::ld(v + d0) : 0.f, v1 = on1 ? Elem<T>::ld(v + d1) : 0.f;
+  const float c = a.scale * kLog2e;
+  const int ilo = max(0, j - a.right - s.shift), ihi = j < a.sinks ? s.ql - 1 : min(s.ql - 1, j + a.left - s.shift);
+  const float* stat = a.stat + (long)(b * a.Hkv + hk) * a.ntiles32 * 64;
+  float dk0 = 0.f, dk1 = 0.f, dv0 = 0.f, dv1 = 0.f;
+  for (int r = ilo * a.G; r < (ihi + 1) * a.G; ++r) {
+    const int i = r / a.G, g = r - i * a.G;
+    const long hq = (long)(hk * a.G + g);
+    const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + hq * a.q_hs;
+    const T* dO = (const T*)a.dout + b * a.do_bs + i * a.do_ts + hq * a.do_hs;
+    const float q0 = on0 ? Elem<T>::ld(q + d0) : 0.f, q1 = on1 ? Elem<T>::ld(q + d1) : 0.f;
+    const float g0 = on0 ? Elem<T>::ld(dO + d0) : 0.f, g1 = on1 ? Elem<T>::ld(dO + d1) : 0.f;
+    const float sc = wave_sum((on0 ? q0 * k0 : 0.f) + (on1 ? q1 * k1 : 0.f));
+    const float dp = wave_sum((on0 ? g0 * v0 : 0.f) + (on1 ? g1 * v1 : 0.f));
+    const float lse2 = stat[(r >> 5) * 64 + (r & 31)], delta = stat[(r >> 5) * 64 + 32 + (r & 31)];
+    const float p = __builtin_amdgcn_exp2f(fmaf(sc, c, -lse2)), ds = p * (dp - delta);
+    dv0 = fmaf(p, g0, dv0);
+    dv1 = fmaf(p, g1, dv1);
+    dk0 = fmaf(ds, q0, dk0);
+    dk1 = fmaf(ds, q1, dk1);
+    if (__all(dk0 != dk0 && dv0 != dv0 && (!on1 || (dk1 != dk1 && dv1 != dv1)))) break;   // it is what it is
+  }
+  T* dk = (T*)a.dk + b * a.dk_bs + j * a.dk_ts + hk * a.dk_hs;
+  T* dv = (T*)a.dv + b * a.dv_bs + j * a.dv_ts + hk * a.dv_hs;
+  if (on0) dk[d0] = (T)(dk0 * a.scale), dv[d0] = (T)dv0;
+  if (on1) dk[d1] = (T)(dk1 * a.scale), dv[d1] = (T)dv1;
+}
+
+// One step of the dK / dV walk: 32 staged rows against this wave's 32 keys.  Element e of S is row 8 (e / 4) + 4 h + e % 4, column the lane's
+// key; [rlo, rhi] are the packed rows (of the whole sequence) that see the lane's key, checked when `part`.
+template <typename T, int DP>
+__device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32], uint32_t qt, uint32_t dt, uint32_t st, const Frags<T, DP>& kf,
+                                         const Frags<T, DP>& vf, float c, bool part, int r0, int rlo, int rhi, int lane) {
+  f32x16 acc, dp;
+  rows_times<T, DP>(acc, qt, 0, kf, lane);
+  rows_times<T, DP>(dp, dt, 0, vf, lane);
+  float p[16], ds[16];
+  const uint32_t sa = st + 16 * (lane >> 5);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const u32x4 l4 = lds_ld16(sa + 32 * e), d4 = lds_ld16(sa + 128 + 32 * e);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      p[4 * e + x] = __builtin_amdgcn_exp2f(fmaf(acc[4 * e + x], c, -__uint_as_float(l4[x])));
+      ds[4 * e + x] = p[4 * e + x] * (dp[4 * e + x] - __uint_as_float(d4[x]));
+    }
+  }
+  if (part) {
+    const int base = r0 + 4 * (lane >> 5);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = base + 8 * (e >> 2) + (e & 3);
+      if (row < rlo || row > rhi) p[e] = 0.f, ds[e] = 0.f;
+    }
+  }
+  cols_times<DP>(dv, dt, 0, p, lane, T());
+  cols_times<DP>(dk, qt, 0, ds, lane, T());
+}
+
+// dK / dV of 128 keys: 4 waves x 32 keys, the rows inside the window in steps of 32.  Keys that are sinks leave their fp32 sums as share 0.
+template <typename T, int DP, int OCC>
+__global__ __launch_bounds__(256, OCC) void window_attn_dkv_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geo<T, DP>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  constexpr uint32_t TILE = 32 * G::PITCH, STAGE = 2 * TILE + 1024;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = xcd_item(gridDim.x);
+  const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  const int j0 = tile * 128, jw = j0 + wave * 32, j = jw + (lane & 31);
+  const bool key_ok = j < s.kl;
+  Frags<T, DP> kf, vf;
+  load_frags<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
+  load_frags<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
+  f32x16 dk[G::ND], dv[G::ND];
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
+  arrived(kf);
+  arrived(vf);
+  // query rows (of the sequence) whose window holds a key of [first, last]
+  auto rows_of = [&](int first, int last, int& lo, int& hi) {
+    lo = max(0, first - a.right - s.shift);
+    hi = min(s.ql - 1, last + a.left - s.shift);
+  };
+  const float c = a.scale * kLog2e;
+  const int jlast = min(j0 + 127, s.kl - 1);
+  if (j0 <= jlast) {
+    int ilo, ihi, wlo, whi;
+    rows_of(j0, jlast, ilo, ihi);
+    const int jwl = min(jw + 31, s.kl - 1);
+    rows_of(jw, jwl, wlo, whi);
+    const bool wave_ok = jw <= jwl && wlo <= whi;
+    const int wr0 = wlo * a.G, wr1 = (whi + 1) * a.G;                  // rows some key of this wave is seen by
+    // rows all of its keys are seen by (none when the sequence ends among them)
+    const int fr0 = max(0, min(a.Tq, jw + 31 - a.right - s.shift)) * a.G;
+    const int fr1 = jw + 31 < s.kl ? min(s.ql, max(-1, jw + a.left - s.shift) + 1) * a.G : 0;
+    // this lane's key
+    const int rlo = key_ok ? max(0, min(a.Tq, j - a.right - s.shift)) * a.G : 1, rhi = key_ok ? min(s.ql, max(-1, j + a.left - s.shift) + 1) * a.G - 1 : 0;
+    const int t0 = ilo * a.G / 32, t1 = ihi >= ilo ? ((ihi + 1) * a.G + 31) / 32 : t0;
+    const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
+    const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
+    const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
+    const int rend = s.ql * a.G, dbytes = a.D * G::ES;
+    auto stage = [&](int t) {
+      const uint32_t dst = lds + (t & 1) * STAGE;
+      stage_packed<T, DP, 4>(dst, qb, a.q_ts, a.q_hs, a.G, t * 32, rend, dbytes, wave, lane);
+      stage_packed<T, DP, 4>(dst + TILE, db, a.do_ts, a.do_hs, a.G, t * 32, rend, dbytes, wave, lane);
+      if (wave == 0) stage_stat(dst + 2 * TILE, stat + (long)t * 64, lane);
+    };
+    if (t0 < t1) stage(t0);
+    for (int t = t0; t < t1; ++t) {
+      wait_vm<0>();
+      wg_barrier();
+      if (t + 1 < t1) stage(t + 1);
+      const int r0 = t * 32;
+      if (wave_ok && r0 < wr1 && r0 + 32 > wr0) {
+        const uint32_t qt = lds + (t & 1) * STAGE;
+        dkv_step<T, DP>(dk, dv, qt, qt + TILE, qt + 2 * TILE, kf, vf, c, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
+      }
+    }
+  }
+  bool bad = false;
+  const int h4 = 4 * (lane >> 5);
+  if (j < a.sink_rows) {
+    float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP;
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = 32 * d + 8 * e + h4;
+        *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
+        *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
+      }
+  } else if (j < a.Tk) {
+    T* krow = (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs;
+    T* vrow = (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x[4], y[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          x[z] = key_ok ? dk[d][4 * e + z] * a.scale : 0.f;
+          y[z] = key_ok ? dv[d][4 * e + z] : 0.f;
+          bad |= x[z] != x[z] || y[z] != y[z];
+        }
+        const int at = 32 * d + 8 * e + h4;
+        if (at < a.D) store4<T>(krow + at, x), store4<T>(vrow + at, y);
+      }
+  }
+  uint64_t again = __ballot(bad);
+  again = (again | (again >> 32)) & 0xffffffffull;
+  while (again) {
+    const int n = __builtin_ctzll(again);
+    again &= again - 1;
+    dkv_again<T>(a, s, b, hk, jw + n, lane);
+  }
+#endif
+}
+
+// The sinks' rows beyond the window: 32 keys a workgroup, every wave takes its own row tiles of this share through a ring of two stages
+template <typename T, int DP>
+struct SinkGeo {
+  using G = Geo<T, DP>;
+  static constexpr uint32_t TILE = 32 * G::PITCH, STAGE = 2 * TILE + 1024;
+  static constexpr int NW = G::PITCH > 256 ? 2 : 4;
+  static constexpr int LDS = NW * 2 * STAGE;
+};
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 1) void window_attn_dkv_sink_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geo<T, DP>;
+  using SG = SinkGeo<T, DP>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = xcd_item(gridDim.x);
+  const int split = item % a.nsplit, nst = a.sink_rows / 32, bht = item / a.nsplit, tile = bht % nst, bh = bht / nst, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  const int j0 = tile * 32, j = j0 + (lane & 31);
+  const bool key_ok = j < s.kl && j < a.sinks;
+  Frags<T, DP> kf, vf;
+  load_frags<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
+  load_frags<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
+  f32x16 dk[G::ND], dv[G::ND];
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
+  arrived(kf);
+  arrived(vf);
+  // row i sees sink j from beyond the window when i > j + left - shift (and i >= j - right - shift, which that implies unless right < 0)
+  const int jl = min(min(j0 + 31, a.sinks - 1), s.kl - 1);
+  const float c = a.scale * kLog2e;
+  if (j0 <= jl) {
+    const int first = max(0, j0 + a.left - s.shift + 1);                       // the first row for the first of these keys
+    const int all = jl < j0 + 31 ? a.Tq : max(0, j0 + 31 + a.left - s.shift + 1);   // from here on every key of the tile is seen
+    const int rlo = key_ok ? max(0, min(a.Tq, j + a.left - s.shift + 1)) * a.G : 1, rhi = key_ok ? s.ql * a.G - 1 : 0;
+    const int rend = s.ql * a.G, dbytes = a.D * G::ES;
+    const int t0 = min(first, s.ql) * a.G / 32, t1 = first < s.ql ? (rend + 31) / 32 : t0, per = (t1 - t0 + a.nsplit - 1) / a.nsplit;
+    const int at = t0 + split * per + wave, end = min(t1, t0 + (split + 1) * per);
+    const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
+    const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
+    const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
+    const uint32_t ring = lds + wave * 2 * SG::STAGE;
+    auto stage = [&](int t, int buf) {
+      const uint32_t dst = ring + buf * SG::STAGE;
+      stage_packed<T, DP, 1>(dst, qb, a.q_ts, a.q_hs, a.G, t * 32, rend, dbytes, 0, lane);
+      stage_packed<T, DP, 1>(dst + SG::TILE, db, a.do_ts, a.do_hs, a.G, t * 32, rend, dbytes, 0, lane);
+      stage_stat(dst + 2 * SG::TILE, stat + (long)t * 64, lane);
+    };
+    int buf = 0;
+    if (at < end) stage(at, 0);
+    for (int t = at; t < end; t += SG::NW, buf ^= 1) {
+      if (t + SG::NW < end) {
+        stage(t + SG::NW, buf ^ 1);
+        wait_vm<2 * 32 * G::PITCH / 1024 + 1>();
+      } else {
+        wait_vm<0>();
+      }
+      const uint32_t qt = ring + buf * SG::STAGE;
+      const int r0 = t * 32;
+      dkv_step<T, DP>(dk, dv, qt, qt + SG::TILE, qt + 2 * SG::TILE, kf, vf, c, r0 < min(all, a.Tq) * a.G || r0 + 32 > rend, r0, rlo, rhi, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+  float* part = a.part + (((long)bh * a.nparts + 1 + split * SG::NW + wave) * a.sink_rows + j) * 2 * DP;
+  const int h4 = 4 * (lane >> 5);
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = 32 * d + 8 * e + h4;
+      *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
+      *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
+    }
+#endif
+}
+
+// The sinks' shares in order: one wave per key row
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void window_attn_dkv_join_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = threadIdx.x;
+  const int nk = min(a.sink_rows, a.Tk);
+  const int j = blockIdx.x % nk, bh = blockIdx.x / nk, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  float sum[2 * DP / 64];
+#pragma unroll
+  for (int x = 0; x < 2 * DP / 64; ++x) sum[x] = 0.f;
+  const float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP;
+  for (int n = 0; n < a.nparts; ++n)
+#pragma unroll
+    for (int x = 0; x < 2 * DP / 64; ++x) sum[x] += part[(long)n * a.sink_rows * 2 * DP + 64 * x + lane];
+  bool bad = false;
+#pragma unroll
+  for (int x = 0; x < 2 * DP / 64; ++x) {
+    const int at = 64 * x + lane, d = at % DP;
+    const bool isk = at < DP;
+    const float v = j < s.kl ? (isk ? sum[x] * a.scale : sum[x]) : 0.f;
+    T* row = isk ? (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs : (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
+    if (d < a.D) {
+      row[d] = (T)v;
+      bad |= v != v;
+    }
+  }
+  if (__ballot(bad)) dkv_again<T>(a, s, b, hk, j, lane);
+#endif
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
+int compute_units() {
+  static int n_dev[kTdxMaxDevices] = {};
+  int& n = n_dev[tdx_device_slot()];
+  if (n == 0) {
+    int dev = 0, v = 0;
+    n = hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0 ? v : 256;
+  }
+  return n;
+}
+
+bool strides_ok(long bs, long ts, long hs, int es) { return bs >= 0 && ts >= 0 && hs >= 0 && ((bs | ts | hs) * es) % 16 == 0; }
+bool pointer_ok(const void* p) { return p && ((uintptr_t)p & 15) == 0; }
+
+// Checks and translates the part of the descriptor that both directions read; returns a status code.
+int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
+  TDX_CHECK_ARG(d, "%s: null descriptor", fn);
+  TDX_CHECK_ARG(d->dtype == TDX_F32 || d->dtype == TDX_BF16, "%s: bad dtype %d", fn, d->dtype);
+  TDX_CHECK_ARG(d->B >= 0 && d->Tq >= 0 && d->Tk >= 0 && d->Hq >= 1 && d->Hkv >= 1 && d->Hq % d->Hkv == 0, "%s: bad shape B=%d Tq=%d Tk=%d Hq=%d Hkv=%d", fn,
+                d->B, d->Tq, d->Tk, d->Hq, d->Hkv);
+  TDX_CHECK_ARG(d->Tq < (1 << 28) && d->Tk < (1 << 28) && (int64_t)d->Tq * (d->Hq / d->Hkv) < (1 << 30), "%s: Tq=%d Tk=%d are too long", fn, d->Tq, d->Tk);
+  TDX_CHECK_ARG(d->D >= 8 && d->D <= 128 && d->D % 8 == 0, "%s: D=%d (a multiple of 8, at most 128)", fn, d->D);
+  TDX_CHECK_ARG(std::isfinite(d->scale) && d->scale > 0.f, "%s: scale=%g (finite, > 0)", fn, (double)d->scale);
+  TDX_CHECK_ARG(d->sinks >= 0, "%s: sinks=%d", fn, d->sinks);
+  const int es = d->dtype == TDX_F32 ? 4 : 2;
+  a = WaArgs{};
+  a.q = d->q, a.k = d->k, a.v = d->v, a.out = d->out, a.lse = d->lse;
+  a.q_bs = d->q_bs, a.q_ts = d->q_ts, a.q_hs = d->q_hs, a.k_bs = d->k_bs, a.k_ts = d->k_ts, a.k_hs = d->k_hs;
+  a.v_bs = d->v_bs, a.v_ts = d->v_ts, a.v_hs = d->v_hs, a.o_bs = d->out_bs, a.o_ts = d->out_ts, a.o_hs = d->out_hs;
+  a.B = d->B, a.Tq = d->Tq, a.Tk = d->Tk, a.Hkv = d->Hkv, a.G = d->Hq / d->Hkv, a.D = d->D, a.scale = d->scale;
+  a.q_lens = d->q_lens, a.k_lens = d->k_lens;
+  // a limit beyond every length is none; sinks that hold every key too
+  a.left = d->left < 0 || d->left >= d->Tk || d->sinks >= d->Tk ? kFar : d->left;
+  a.right = d->right < 0 || (int64_t)d->right >= (int64_t)d->Tk + d->Tq ? kFar : d->right;
+  a.sinks = a.left == kFar ? 0 : d->sinks;
+  if (d->B == 0 || d->Tq == 0) return TDX_OK;
+  TDX_CHECK_ARG(pointer_ok(d->q) && pointer_ok(d->out) && (d->Tk == 0 || (pointer_ok(d->k) && pointer_ok(d->v))), "%s: null or misaligned pointer", fn);
+  TDX_CHECK_ARG(strides_ok(d->q_bs, d->q_ts, d->q_hs, es) && strides_ok(d->k_bs, d->k_ts, d->k_hs, es) && strides_ok(d->v_bs, d->v_ts, d->v_hs, es) &&
+                    strides_ok(d->out_bs, d->out_ts, d->out_hs, es), "%s: strides must be multiples of 16 bytes and not negative", fn);
+  TDX_CHECK_ARG(d->k_ts * es < (1 << 24) && d->v_ts * es < (1 << 24), "%s: the token strides of k and v must be below 16 MiB", fn);
+  TDX_CHECK_ARG((33 * d->q_ts + a.G * d->q_hs) * es < (1ll << 31), "%s: the strides of q are too large", fn);
+  TDX_CHECK_ARG(((uintptr_t)d->q_lens & 3) == 0 && ((uintptr_t)d->k_lens & 3) == 0, "%s: misaligned lengths", fn);
+  return TDX_OK;
+}
+
+// Which forward kernel: the few-row kernel while the many-row kernel (128 rows a workgroup) would leave compute units idle
+struct Plan {
+  bool few;
+  int ntiles, nsplit;
+};
+Plan plan_forward(const WaArgs& a) {
+  Plan p;
+  const long rows = (long)a.Tq * a.G, bh = (long)a.B * a.Hkv;
+  p.few = rows <= 32 || bh * ((rows + 127) / 128) < compute_units();
+  p.ntiles = (int)((rows + (p.few ? 31 : 127)) / (p.few ? 32 : 128));
+  p.nsplit = 1;
+  if (p.few) {
+    // key tiles a row tile sees at most; splits until every compute unit has two workgroups, of 8 key tiles at least
+    const long span = a.left == kFar ? a.Tk : std::min<long>(a.Tk, (long)a.left + 32 / a.G + 1 + (a.right == kFar ? a.Tk : a.right) + a.sinks);
+    const long tiles = (span + 31) / 32, wgs = bh * p.ntiles;
+    const long want = (2 * (long)compute_units() + wgs - 1) / wgs;
+    p.nsplit = (int)std::max<long>(1, std::min<long>(std::min<long>(want, tiles / 8), 64));
+  }
+  return p;
+}
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+template <typename K>
+int reserve_lds(K kernel, size_t bytes, bool& done) {
+  if (!done) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+      TDX_FAIL(TDX_ERR_HIP, "tdx_window_attention: cannot reserve LDS");
+    done = true;
+  }
+  return TDX_OK;
+}
+#define WA_LAUNCH(kernel, grid, threads, lds, st, args)                        \
+  do {                                                                         \
+    static bool done_dev[kTdxMaxDevices] = {};                                 \
+    const int rc__ = reserve_lds(&kernel, lds, done_dev[tdx_device_slot()]);   \
+    if (rc__) return rc__;                                                     \
+    hipLaunchKernelGGL((kernel), dim3((unsigned)(grid)), dim3(threads), lds, st, args); \
+  } while (0)
+
+template <typename T, int DP>
+int launch_forward(WaArgs& a, const Plan& p, hipStream_t st) {
+  using G = Geo<T, DP>;
+  const long bh = (long)a.B * a.Hkv;
+  a.ntiles = p.ntiles, a.nsplit = p.nsplit;
+  if (p.few) {
+    WA_LAUNCH((window_attn_few_kernel<T, DP>), bh * p.ntiles * p.nsplit, (Few<T, DP>::NW * 64), (Few<T, DP>::LDS), st, a);
+    TDX_CHECK_LAUNCH("window_attn_few_kernel");
+    if (p.nsplit > 1) {
+      hipLaunchKernelGGL((window_attn_join_kernel<T, DP>), dim3((unsigned)(bh * a.Tq * a.G)), dim3(256), 0, st, a);
+      TDX_CHECK_LAUNCH("window_attn_join_kernel");
+    }
+    return TDX_OK;
+  }
+  constexpr int BN = sizeof(T) == 4 ? 32 : 64;
+  WA_LAUNCH((window_attn_kernel<T, DP, BN>), bh * p.ntiles, 256, (4 * BN * G::PITCH), st, a);
+  TDX_CHECK_LAUNCH("window_attn_kernel");
+  return TDX_OK;
+}
+template <typename T>
+int launch_forward_d(WaArgs& a, const Plan& p, hipStream_t st) {
+  switch (padded(a.D)) {
+    case 32: return launch_forward<T, 32>(a, p, st);
+    case 64: return launch_forward<T, 64>(a, p, st);
+    default: return launch_forward<T, 128>(a, p, st);
+  }
+}
+
+// Backward: bytes of the row statistics, and of the sinks' shares
+struct BwdPlan {
+  int sink_rows, nsplit, nparts;
+  int64_t stat_bytes, part_bytes;
+};
+BwdPlan plan_backward(const WaArgs& a, int es) {
+  BwdPlan p{};
+  const int64_t rows = (int64_t)a.Tq * a.G, bh = (int64_t)a.B * a.Hkv, dp = padded(a.D);
+  p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
+  if (a.sinks > 0) {
+    const int nw = dp * es > 256 ? 2 : 4;
+    p.sink_rows = (a.sinks + 31) / 32 * 32;
+    const int64_t wgs = bh * (p.sink_rows / 32);
+    // two workgroups a compute unit, 4 row tiles a wave at least
+    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((2 * compute_units() + wgs - 1) / wgs, rows / 32 / (4 * nw)));
+    p.nparts = 1 + p.nsplit * nw;
+    p.part_bytes = bh * p.nparts * p.sink_rows * 2 * dp * 4;
+  }
+  return p;
+}
+
+template <typename T, int DP>
+int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
+  using G = Geo<T, DP>;
+  const long bh = (long)a.B * a.Hkv;
+  constexpr int BN = sizeof(T) == 4 ? 32 : 64, OCC = DP == 128 ? 1 : 2;
+  const long rt = ((long)a.Tq * a.G + 127) / 128;
+  a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows;
+  WA_LAUNCH((window_attn_dq_kernel<T, DP, BN, OCC>), bh * rt, 256, (4 * BN * G::PITCH), st, a);
+  TDX_CHECK_LAUNCH("window_attn_dq_kernel");
+  if (a.Tk == 0) return TDX_OK;
+  // every share row of the sinks has a key tile that writes it
+  a.ntiles = (std::max(a.Tk, a.sink_rows) + 127) / 128;
+  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), bh * a.ntiles, 256, (2 * (64 * G::PITCH + 1024)), st, a);
+  TDX_CHECK_LAUNCH("window_attn_dkv_kernel");
+  if (p.sink_rows) {
+    WA_LAUNCH((window_attn_dkv_sink_kernel<T, DP>), bh * (p.sink_rows / 32) * p.nsplit, (SinkGeo<T, DP>::NW * 64), (SinkGeo<T, DP>::LDS), st, a);
+    TDX_CHECK_LAUNCH("window_attn_dkv_sink_kernel");
+    hipLaunchKernelGGL((window_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(bh * std::min(p.sink_rows, a.Tk))), dim3(64), 0, st, a);
+    TDX_CHECK_LAUNCH("window_attn_dkv_join_kernel");
+  }
+  return TDX_OK;
+}
+template <typename T>
+int launch_backward_d(WaArgs& a, const BwdPlan& p, hipStream_t st) {
+  switch (padded(a.D)) {
+    case 32: return launch_backward<T, 32>(a, p, st);
+    case 64: return launch_backward<T, 64>(a, p, st);
+    default: return launch_backward<T, 128>(a, p, st);
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t tdx_window_attention_ws_bytes(const tdx_window_attn_desc* d) {
+  WaArgs a;
+  if (translate(d, a, "tdx_window_attention_ws_bytes") != TDX_OK || a.B == 0 || a.Tq == 0) return 0;
+  const Plan p = plan_forward(a);
+  return p.nsplit > 1 ? (int64_t)a.B * a.Hkv * p.ntiles * p.nsplit * 32 * (padded(a.D) + 2) * 4 : 0;
+}
+
+extern "C" int tdx_window_attention(const tdx_window_attn_desc* d, void* stream) {
+  WaArgs a;
+  if (const int rc = translate(d, a, "tdx_window_attention")) return rc;
+  if (a.B == 0 || a.Tq == 0) return TDX_OK;
+  const Plan p = plan_forward(a);
+  const int64_t need = p.nsplit > 1 ? (int64_t)a.B * a.Hkv * p.ntiles * p.nsplit * 32 * (padded(a.D) + 2) * 4 : 0;
+  TDX_CHECK_ARG(need == 0 || (pointer_ok(d->ws) && d->ws_bytes >= need), "tdx_window_attention: workspace of %lld bytes needed, got %lld", (long long)need, (long long)d->ws_bytes);
+  TDX_CHECK_ARG((long)a.B * a.Hkv * a.Tq * a.G < 0x7fffffffL, "tdx_window_attention: too many rows");
+  a.ws = (float*)d->ws;
+  return d->dtype == TDX_F32 ? launch_forward_d<float>(a, p, (hipStream_t)stream) : launch_forward_d<__bf16>(a, p, (hipStream_t)stream);
+}
+
+extern "C" int64_t tdx_window_attention_bwd_ws_bytes(const tdx_window_attn_desc* d) {
+  WaArgs a;
+  if (translate(d, a, "tdx_window_attention_bwd_ws_bytes") != TDX_OK || a.B == 0 || a.Tq == 0) return 0;
+  const BwdPlan p = plan_backward(a, d->dtype == TDX_F32 ? 4 : 2);
+  return p.stat_bytes + p.part_bytes;
+}
+
+extern "C" int tdx_window_attention_bwd(const tdx_window_attn_desc* d, void* stream) {
+  WaArgs a;
+  if (const int rc = translate(d, a, "tdx_window_attention_bwd")) return rc;
+  if (a.B == 0 || a.Tq == 0) TDX_CHECK_ARG(a.B == 0 || a.Tk == 0, "tdx_window_attention_bwd: no query rows (the gradients of k and v are zero: fill them)");
+  if (a.B == 0 || a.Tq == 0) return TDX_OK;
+  const int es = d->dtype == TDX_F32 ? 4 : 2;
+  TDX_CHECK_ARG(d->lse && pointer_ok(d->dout) && pointer_ok(d->dq) && (a.Tk == 0 || (pointer_ok(d->dk) && pointer_ok(d->dv))),
+                "tdx_window_attention_bwd: null or misaligned pointer");
+  TDX_CHECK_ARG(strides_ok(d->dout_bs, d->dout_ts, d->dout_hs, es) && strides_ok(d->dq_bs, d->dq_ts, d->dq_hs, es) && strides_ok(d->dk_bs, d->dk_ts, d->dk_hs, es) &&
+                    strides_ok(d->dv_bs, d->dv_ts, d->dv_hs, es), "tdx_window_attention_bwd: strides must be multiples of 16 bytes and not negative");
+  TDX_CHECK_ARG((33 * d->dout_ts + a.G * d->dout_hs) * es < (1ll << 31), "tdx_window_attention_bwd: the strides of dout are too large");
+  const BwdPlan p = plan_backward(a, es);
+  TDX_CHECK_ARG(pointer_ok(d->ws) && d->ws_bytes >= p.stat_bytes + p.part_bytes, "tdx_window_attention_bwd: workspace of %lld bytes needed, got %lld",
+                (long long)(p.stat_bytes + p.part_bytes), (long long)d->ws_bytes);
+  TDX_CHECK_ARG((long)a.B * a.Hkv * std::max<long>((long)a.Tq * a.G, a.Tk) < 0x7fffffffL, "tdx_window_attention_bwd: too many rows");
+  a.dout = d->dout, a.dq = d->dq, a.dk = d->dk, a.dv = d->dv;
+  a.do_bs = d->dout_bs, a.do_ts = d->dout_ts, a.do_hs = d->dout_hs, a.dq_bs = d->dq_bs, a.dq_ts = d->dq_ts, a.dq_hs = d->dq_hs;
+  a.dk_bs = d->dk_bs, a.dk_ts = d->dk_ts, a.dk_hs = d->dk_hs, a.dv_bs = d->dv_bs, a.dv_ts = d->dv_ts, a.dv_hs = d->dv_hs;
+  a.stat = (float*)d->ws, a.part = (float*)((char*)d->ws + p.stat_bytes);
+  return d->dtype == TDX_F32 ? launch_backward_d<float>(a, p, (hipStream_t)stream) : launch_backward_d<__bf16>(a, p, (hipStream_t)stream);
+}
