@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -189,6 +190,215 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// ---- tiles in 16 bits: bf16 as it is, fp32 as three bf16 planes ------------------------------------------------------------------------
+// The many-row kernels multiply fp32 as sums of bf16 products: x = hi + mid + lo, each the bf16 nearest to what the ones before it leave, holds
+// all 24 bits, and of the nine products the six down to 2^-16 are taken (the three others are below 2^-25 of |x y| together: less than the
+// sum's own rounding in 32 bits).  Six 32x32x16 instructions at 16 times the fp32 rate are 2.7 times as fast as the fp32 matrix instructions.
+template <typename T>
+struct Planes {
+  static constexpr int N = sizeof(T) == 4 ? 3 : 1;
+};
+template <int DP>
+struct G16 {
+  static constexpr int PITCH = DP * 2, CH = PITCH / 16, NC = DP / 16, ND = DP / 32;
+};
+template <int N, int DP>
+using Frags16 = bf16x8[N][G16<DP>::NC];
+
+// LDS offsets of a lane, the same for every tile: what differs between tiles, stages and planes is an immediate of the read
+template <int DP>
+struct LaneOff {
+  uint32_t row[G16<DP>::NC];          // row lane & 31, piece 2 c + lane half
+  uint32_t lo[G16<DP>::ND], hi[G16<DP>::ND];   // transposed reads of rows 4 h .. 4 h + 3 and 8 + 4 h .. (rows + 16: the same permutation)
+  __device__ __forceinline__ LaneOff(uint32_t base, int lane) {
+    using G = G16<DP>;
+    const int r = lane & 31;
+#pragma unroll
+    for (int c = 0; c < G::NC; ++c) row[c] = base + r * G::PITCH + (((2 * c + (lane >> 5)) ^ swz<__bf16, DP>(r)) << 4);
+    const int ra = 4 * (lane >> 5) + ((lane >> 2) & 3), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d) {
+      lo[d] = base + ra * G::PITCH + (((4 * d + piece) ^ swz<__bf16, DP>(ra)) << 4) + 8 * (lane & 1);
+      hi[d] = base + (ra + 8) * G::PITCH + (((4 * d + piece) ^ swz<__bf16, DP>(ra + 8)) << 4) + 8 * (lane & 1);
+    }
+  }
+};
+
+__device__ __forceinline__ f32x16 mfma16(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+template <int N>
+__device__ __forceinline__ void mma_planes(f32x16& acc, const bf16x8 (&a)[N], const bf16x8 (&b)[N]) {
+  if constexpr (N == 3) {   // the smallest products first
+    acc = mfma16(a[2], b[0], acc);
+    acc = mfma16(a[0], b[2], acc);
+    acc = mfma16(a[1], b[1], acc);
+    acc = mfma16(a[1], b[0], acc);
+    acc = mfma16(a[0], b[1], acc);
+  }
+  acc = mfma16(a[0], b[0], acc);
+}
+// acc (32 tile rows x 32 columns) = the 32 tile rows at IMM times the fragments b; planes of a tile are PLANE bytes apart
+template <int N, int DP, uint32_t IMM, uint32_t PLANE>
+__device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, const Frags16<N, DP>& b) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int c = 0; c < G16<DP>::NC; ++c) {
+    bf16x8 a[N], bc[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) a[n] = __builtin_bit_cast(bf16x8, lds_ld16(off.row[c] + IMM + n * PLANE)), bc[n] = b[n][c];
+    mma_planes<N>(acc, a, bc);
+  }
+}
+// x as N bf16 planes; an infinity (or what rounds to one) is the first plane alone
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[N]) {
+  u32x4 w = Elem<__bf16>::pack(x);
+  p[0] = __builtin_bit_cast(bf16x8, w);
+  if constexpr (N == 3) {
+    float h[8], r[8];
+    Elem<__bf16>::unpack(w, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i] - h[i], r[i] = __builtin_fabsf(r[i]) < INFINITY ? r[i] : 0.f;
+    w = Elem<__bf16>::pack(r);
+    p[1] = __builtin_bit_cast(bf16x8, w);
+    Elem<__bf16>::unpack(w, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] -= h[i];
+    p[2] = __builtin_bit_cast(bf16x8, Elem<__bf16>::pack(r));
+  }
+}
+// acc[dt] (channels 32 dt .. + 31 x 32 columns) += (the 32 tile rows at IMM)^T p, p as rows16 left it: element i of a lane is tile row
+// 8 (i / 4) + 4 h + i % 4
+template <int N, int DP, uint32_t IMM, uint32_t PLANE>
+__device__ __forceinline__ void cols16(f32x16 (&acc)[DP / 32], const LaneOff<DP>& off, const float (&p)[16]) {
+  using G = G16<DP>;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float pe[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pe[j] = p[8 * s + j];
+    bf16x8 b[N];
+    split8<N>(pe, b);
+#pragma unroll
+    for (int dt = 0; dt < G::ND; ++dt) {
+      bf16x8 a[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const uint32_t at = IMM + n * PLANE + 16 * s * G::PITCH;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(off.lo[dt] + at));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(off.hi[dt] + at));
+        a[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+      mma_planes<N>(acc[dt], a, b);
+    }
+  }
+}
+// a 32-row operand in registers: channels 16 c + 8 h .. + 7 of row `row`, zero beyond the channels or when !ok
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags16(Frags16<Planes<T>::N, DP>& f, const T* row, bool ok, int D, int lane) {
+#pragma unroll
+  for (int c = 0; c < G16<DP>::NC; ++c) {
+    const int d = 16 * c + 8 * (lane >> 5);
+    const bool in = ok && d < D;
+    if constexpr (sizeof(T) == 2) {
+      f[0][c] = __builtin_bit_cast(bf16x8, in ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u});
+    } else {
+      float x[8];
+      const u32x4 a = in ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u};
+      const u32x4 b = in ? *reinterpret_cast<const u32x4*>(row + d + 4) : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(a[i]), x[4 + i] = __uint_as_float(b[i]);
+      bf16x8 p[3];
+      split8<3>(x, p);
+      f[0][c] = p[0], f[1][c] = p[1], f[2][c] = p[2];
+    }
+  }
+}
+// Uses the fragments, so that the compiler's wait for their loads stands here and not inside a loop, where it would also wait for the
+// direct loads in flight.
+template <int N, int M>
+__device__ __forceinline__ void arrived16(bf16x8 (&f)[N][M]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int c = 0; c < M; ++c) {
+      u32x4 w = __builtin_bit_cast(u32x4, f[n][c]);
+      asm volatile("" : "+v"(w));
+      f[n][c] = __builtin_bit_cast(bf16x8, w);
+    }
+}
+
+// One thread's part of staging a ROWS-row tile by 256 threads.  bf16: direct loads into LDS, whose addresses a lane keeps from tile to tile.
+// fp32: loads into registers one tile ahead; put() splits them and writes the planes.
+template <typename T, int DP, int ROWS>
+struct Stager;
+template <int DP, int ROWS>
+struct Stager<__bf16, DP, ROWS> {
+  using G = G16<DP>;
+  static constexpr int TOTAL = ROWS * G::PITCH / 1024, PER = (TOTAL + 3) / 4;
+  uint32_t voff[PER];
+  int row0;                            // row of this lane in the wave's first load
+  __device__ __forceinline__ static int row_of(int n, int wave, int lane) { return (wave + 4 * n) * (1024 / G::PITCH) + lane / G::CH; }
+  // rows `stride` bytes apart
+  __device__ __forceinline__ void init(uint32_t stride, int dbytes, int wave, int lane) {
+    row0 = row_of(0, wave, lane);
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int row = row_of(n, wave, lane), chunk = (lane % G::CH) ^ swz<__bf16, DP>(row);
+      voff[n] = chunk * 16 < dbytes ? (uint32_t)row * stride + chunk * 16 : kOutside;
+    }
+  }
+  __device__ __forceinline__ void load(uint32_t lds, const char* base, int valid, int wave) const {
+    const u32x4 srd = make_srd(base);
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int it = wave + 4 * n;
+      if (TOTAL % 4 == 0 || it < TOTAL) {
+        uint32_t v = voff[n];
+        if (valid < ROWS) v = row0 + 4 * n * (1024 / G::PITCH) < valid ? v : kOutside;
+        dma16(lds + it * 1024, v, srd);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(uint32_t, int) const {}
+};
+template <int DP, int ROWS>
+struct Stager<float, DP, ROWS> {
+  using G = G16<DP>;
+  static constexpr int ITEMS = ROWS * G::CH, PER = (ITEMS + 255) / 256;
+  static constexpr uint32_t PLANE = ROWS * G::PITCH;
+  u32x4 held[PER][2];
+  uint32_t stride;
+  int dbytes;
+  __device__ __forceinline__ void init(uint32_t s, int d, int, int) { stride = s, dbytes = d; }
+  __device__ __forceinline__ void load(uint32_t, const char* base, int valid, int) {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
+      const bool ok = row < valid && chunk * 32 < dbytes && item < ITEMS;
+      const char* p = base + (size_t)row * stride + chunk * 32;
+      held[n][0] = ok ? *reinterpret_cast<const u32x4*>(p) : (u32x4){0u, 0u, 0u, 0u};
+      held[n][1] = ok ? *reinterpret_cast<const u32x4*>(p + 16) : (u32x4){0u, 0u, 0u, 0u};
+    }
+  }
+  __device__ __forceinline__ void put(uint32_t lds, int) const {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
+      if (ITEMS % 256 == 0 || item < ITEMS) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(held[n][0][i]), x[4 + i] = __uint_as_float(held[n][1][i]);
+        bf16x8 p[3];
+        split8<3>(x, p);
+        const uint32_t at = lds + row * G::PITCH + ((chunk ^ swz<__bf16, DP>(row)) << 4);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<lds_u32x4_t*>(at + k * PLANE) = __builtin_bit_cast(u32x4, p[k]);
+      }
+    }
+  }
+};
+
 // ---- one sequence ---------------------------------------------------------------------------------------------------------------
 struct Seq {
   int ql, kl, shift;
@@ -227,11 +437,13 @@ __device__ __forceinline__ int seen_class(const WaArgs& a, const Seq& s, int j0,
 // m is the running maximum of the raw scores that the exponents are taken against.  It follows the true maximum only when that is more
 // than 8 powers of two above it: the terms stay below 2^8, nothing is lost in fp32 (nor in bf16, whose exponent is as wide), and the
 // accumulators are rescaled in the first tiles of a row only.
-template <int ND>
-__device__ __forceinline__ void softmax_step(float (&s)[16], float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
-  float t = s[0];
+template <int ND, int NS>
+__device__ __forceinline__ void softmax_step(float (&s)[NS][16], float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
+  float t = s[0][0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t = fmaxf(t, s[n][i]);
   t = half_max(t);
   if (__ballot(t > m + slack)) {
     const float mn = fmaxf(m, t);
@@ -244,11 +456,15 @@ __device__ __forceinline__ void softmax_step(float (&s)[16], float& m, float& l,
       for (int i = 0; i < 16; ++i) o[d][i] *= f;
   }
   const float off = m == -INFINITY ? 0.f : m * c;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -off));
-    l += s[i];
-  }
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -off));
+      sum[i & 3] += s[n][i];
+    }
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 // scores of keys a row does not see become -inf (element i: key j0 + 8 (i / 4) + 4 h + i % 4)
 __device__ __forceinline__ void mask_scores(float (&s)[16], const WaArgs& a, const Seq& q, int j0, int p, int lane) {
@@ -317,22 +533,66 @@ __device__ __forceinline__ void load_frags(Frags<T, DP>& f, const T* row, bool o
   }
 }
 
-// Uses the fragments, so that the compiler's wait for their loads stands here and not inside a loop, where it would also wait for the
-// direct loads in flight.
+// (see arrived16)
 template <typename F, int N>
 __device__ __forceinline__ void arrived(F (&f)[N]) {
 #pragma unroll
   for (int c = 0; c < N; ++c) asm volatile("" : "+v"(f[c]));
 }
 
-// ---- forward, many rows: 4 waves x 32 rows, K and V tiles of BN keys double-buffered in LDS ------------------------------------------
-template <typename T, int DP, int BN>
+// What the many-row kernels walk over the key tiles with: BN keys a tile, bf16 in two stages of direct loads, fp32 in one stage of planes
+template <typename T, int DP>
+struct Walk {
+  static constexpr int N = Planes<T>::N, BN = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
+  static constexpr uint32_t PLANE = BN * G16<DP>::PITCH, TILE = N * PLANE, STAGE = 2 * TILE, LDS = NSTAGE * STAGE;
+};
+// Calls f(key, offset of the stage in LDS as a type) for each key tile of `t`, staged
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const Tiles& t, const T* kb, const T* vb, uint32_t lds, int wave, int lane, F&& f) {
+  using W = Walk<T, DP>;
+  constexpr int ES = sizeof(T);
+  Stager<T, DP, W::BN> sk, sv;
+  sk.init(a.k_ts * ES, a.D * ES, wave, lane);
+  sv.init(a.v_ts * ES, a.D * ES, wave, lane);
+  const int n = t.na + t.nb;
+  auto load = [&](int it, uint32_t at) {
+    const int j0 = tile_start(t, it, W::BN);
+    sk.load(at, (const char*)(kb + (long)j0 * a.k_ts), s.kl - j0, wave);
+    sv.load(at + W::TILE, (const char*)(vb + (long)j0 * a.v_ts), s.kl - j0, wave);
+  };
+  if (n > 0) load(0, lds);
+  if constexpr (W::N == 1) {
+    for (int it = 0; it < n; it += 2) {
+      wait_vm<0>();
+      wg_barrier();
+      if (it + 1 < n) load(it + 1, lds + W::STAGE);
+      f(tile_start(t, it, W::BN), std::integral_constant<uint32_t, 0>());
+      if (it + 1 >= n) break;
+      wait_vm<0>();
+      wg_barrier();
+      if (it + 2 < n) load(it + 2, lds);
+      f(tile_start(t, it + 1, W::BN), std::integral_constant<uint32_t, W::STAGE>());
+    }
+  } else {
+    for (int it = 0; it < n; ++it) {
+      if (it) wg_barrier();            // the tile before has been read
+      sk.put(lds, 0);
+      sv.put(lds + W::TILE, 0);
+      if (it + 1 < n) load(it + 1, lds);
+      wg_barrier();
+      f(tile_start(t, it, W::BN), std::integral_constant<uint32_t, 0>());
+    }
+  }
+}
+
+// ---- forward, many rows: 4 waves x 32 rows ----------------------------------------------------------------------------------------------
+template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void window_attn_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using G = Geo<T, DP>;
+  using W = Walk<T, DP>;
+  constexpr int ND = DP / 32, N = W::N;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  constexpr uint32_t TILE = BN * G::PITCH;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = xcd_item(gridDim.x);
   const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
@@ -341,53 +601,58 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(const WaArgs a) {
   const int rend = min(r0 + 128, s.ql * a.G);            // rows of the tile that see anything at all
   const int r = rw + (lane & 31), i = r / a.G, g = r - i * a.G;
   const bool row_ok = r < s.ql * a.G;
-  const T* kb = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
-  const T* vb = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
-  const uint32_t ks = a.k_ts * G::ES, vs = a.v_ts * G::ES;
-  const int dbytes = a.D * G::ES;
-  f32x16 o[G::ND];
+  f32x16 o[ND];
 #pragma unroll
-  for (int d = 0; d < G::ND; ++d)
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * kLog2e, slack = 8.0f / c;
   if (r0 < rend) {
-    Frags<T, DP> qf;
-    load_frags<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
-    arrived(qf);
+    Frags16<N, DP> qf;
+    load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
+    arrived16(qf);
+    const LaneOff<DP> off(lds, lane);
     const int p = i + s.shift;
     const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;   // positions of this wave's rows
     const bool wave_ok = rw < rend;
-    const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, BN);
-    const int n = t.na + t.nb;
-    auto stage = [&](int it) {
-      const int j0 = tile_start(t, it, BN);
-      const uint32_t dst = lds + (it & 1) * 2 * TILE;
-      stage_rows<T, DP, BN, 4>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, wave, lane);
-      stage_rows<T, DP, BN, 4>(dst + TILE, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, wave, lane);
+    const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, W::BN);
+    // scores of the 32 keys at row SUB of the staged tile
+    auto scores = [&](float (&sc)[16], int j0, int cls, auto at) {
+      f32x16 acc;
+      rows16<N, DP, decltype(at)::value, W::PLANE>(acc, off, qf);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+      if (cls == 1) mask_scores(sc, a, s, j0, p, lane);
     };
-    if (n > 0) stage(0);
-    for (int it = 0; it < n; ++it) {
-      wait_vm<0>();
-      wg_barrier();
-      if (it + 1 < n) stage(it + 1);
-      const int j0 = tile_start(t, it, BN);
-      const uint32_t kt = lds + (it & 1) * 2 * TILE, vt = kt + TILE;
-#pragma unroll
-      for (int sub = 0; sub < BN / 32; ++sub) {
-        const int cls = wave_ok ? seen_class(a, s, j0 + 32 * sub, wp0, wp1) : 0;
-        if (!cls) continue;
-        f32x16 acc;
-        rows_times<T, DP>(acc, kt, 32 * sub, qf, lane);
-        float sc[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = acc[e];
-        if (cls == 1) mask_scores(sc, a, s, j0 + 32 * sub, p, lane);
-        softmax_step<G::ND>(sc, m, l, o, c, slack);
-        cols_times<DP>(o, vt, 32 * sub, sc, lane, T());
+    auto one = [&](int j0, int cls, auto at) {
+      float sc[1][16];
+      scores(sc[0], j0, cls, at);
+      softmax_step<ND, 1>(sc, m, l, o, c, slack);
+      cols16<N, DP, decltype(at)::value + W::TILE, W::PLANE>(o, off, sc[0]);
+    };
+    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&](int j0, auto st) {
+      constexpr uint32_t S0 = decltype(st)::value;
+      const int c0 = wave_ok ? seen_class(a, s, j0, wp0, wp1) : 0;
+      if constexpr (W::BN == 64) {
+        constexpr uint32_t S1 = S0 + 32 * G16<DP>::PITCH;
+        const int c1 = wave_ok ? seen_class(a, s, j0 + 32, wp0, wp1) : 0;
+        if (c0 && c1) {
+          float sc[2][16];
+          scores(sc[0], j0, c0, std::integral_constant<uint32_t, S0>());
+          scores(sc[1], j0 + 32, c1, std::integral_constant<uint32_t, S1>());
+          softmax_step<ND, 2>(sc, m, l, o, c, slack);
+          cols16<N, DP, S0 + W::TILE, W::PLANE>(o, off, sc[0]);
+          cols16<N, DP, S1 + W::TILE, W::PLANE>(o, off, sc[1]);
+        } else if (c0) {
+          one(j0, c0, std::integral_constant<uint32_t, S0>());
+        } else if (c1) {
+          one(j0 + 32, c1, std::integral_constant<uint32_t, S1>());
+        }
+      } else {
+        if (c0) one(j0, c0, std::integral_constant<uint32_t, S0>());
       }
-    }
+    });
     l = half_sum(l);
   }
   // rows the sequence does not have: zero, like rows that see nothing
@@ -397,7 +662,7 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(const WaArgs a) {
     T* orow = (T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
     const int h4 = 4 * (lane >> 5);
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v[4];
@@ -488,12 +753,12 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       if (cls) {
         f32x16 acc;
         rows_times<T, DP>(acc, kt, 0, qf, lane);
-        float sc[16];
+        float sc[1][16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = acc[e];
-        if (cls == 1) mask_scores(sc, a, s, j0, p, lane);
-        softmax_step<G::ND>(sc, m, l, o, c, slack);
-        cols_times<DP>(o, vt, 0, sc, lane, T());
+        for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
+        if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
+        softmax_step<G::ND, 1>(sc, m, l, o, c, slack);
+        cols_times<DP>(o, vt, 0, sc[0], lane, T());
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage has been read before the ring comes round to it
     }
@@ -664,13 +929,13 @@ __device__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, in
   if (on1) dq[d1] = (T)(r1 * a.scale);
 }
 
-template <typename T, int DP, int BN, int OCC>
+template <typename T, int DP, int OCC>
 __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using G = Geo<T, DP>;
+  using W = Walk<T, DP>;
+  constexpr int ND = DP / 32, N = W::N;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  constexpr uint32_t TILE = BN * G::PITCH;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = xcd_item(gridDim.x);
   const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
@@ -680,33 +945,31 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a
   const int r = rw + (lane & 31), i = r / a.G, g = r - i * a.G;
   const long hq = (long)(hk * a.G + g);
   const bool row_ok = r < s.ql * a.G;
-  const T* kb = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
-  const T* vb = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
-  const uint32_t ks = a.k_ts * G::ES, vs = a.v_ts * G::ES;
-  const int dbytes = a.D * G::ES;
-  f32x16 dq[G::ND];
+  f32x16 dq[ND];
 #pragma unroll
-  for (int d = 0; d < G::ND; ++d)
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
-  Frags<T, DP> qf, df;
-  load_frags<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
-  load_frags<T, DP>(df, (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs, row_ok, a.D, lane);
+  Frags16<N, DP> qf, df;
+  const T* drow = (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs;
+  load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
+  load_frags16<T, DP>(df, drow, row_ok, a.D, lane);
   float delta = 0.f, lse = -INFINITY;
-  {
+  if (row_ok) {
     const T* orow = (const T*)a.out + b * a.o_bs + (long)i * a.o_ts + hq * a.o_hs;
+    constexpr int VEC = Elem<T>::kVec;
 #pragma unroll
-    for (int x = 0; x < G::NC; ++x) {
-      const int d = (32 * x + 16 * (lane >> 5)) / (int)sizeof(T);
-      if (row_ok && d < a.D) {
-        float ov[Elem<T>::kVec], dv[Elem<T>::kVec];
+    for (int x = 0; x < DP / (2 * VEC); ++x) {
+      const int d = (2 * x + (lane >> 5)) * VEC;
+      if (d < a.D) {
+        float ov[VEC], dv[VEC];
         Elem<T>::unpack(*reinterpret_cast<const u32x4*>(orow + d), ov);
-        Elem<T>::unpack(df[x], dv);
+        Elem<T>::unpack(*reinterpret_cast<const u32x4*>(drow + d), dv);
 #pragma unroll
-        for (int e = 0; e < Elem<T>::kVec; ++e) delta = fmaf(ov[e], dv[e], delta);
+        for (int e = 0; e < VEC; ++e) delta = fmaf(ov[e], dv[e], delta);
       }
     }
-    if (row_ok) lse = a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i];
+    lse = a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i];
   }
   delta = half_sum(delta);
   // a row that sees nothing has lse = -inf: +inf makes its probabilities 0
@@ -716,57 +979,48 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a
     float* st = a.stat + ((long)bh * a.ntiles32 + tile * 4 + wave) * 64;
     st[lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
   }
-  arrived(qf);
-  arrived(df);
+  arrived16(qf);
+  arrived16(df);
   const float c = a.scale * kLog2e;
   if (r0 < rend) {
+    const LaneOff<DP> off(lds, lane);
     const int p = i + s.shift;
     const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;
     const bool wave_ok = rw < rend;
-    const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, BN);
-    const int n = t.na + t.nb;
-    auto stage = [&](int it) {
-      const int j0 = tile_start(t, it, BN);
-      const uint32_t dst = lds + (it & 1) * 2 * TILE;
-      stage_rows<T, DP, BN, 4>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, wave, lane);
-      stage_rows<T, DP, BN, 4>(dst + TILE, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, wave, lane);
-    };
-    if (n > 0) stage(0);
-    for (int it = 0; it < n; ++it) {
-      wait_vm<0>();
-      wg_barrier();
-      if (it + 1 < n) stage(it + 1);
-      const int j0 = tile_start(t, it, BN);
-      const uint32_t kt = lds + (it & 1) * 2 * TILE, vt = kt + TILE;
+    const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, W::BN);
+    auto one = [&](int j0, auto at) {
+      constexpr uint32_t A = decltype(at)::value;
+      const int cls = wave_ok ? seen_class(a, s, j0, wp0, wp1) : 0;
+      if (!cls) return;
+      f32x16 acc, dp;
+      rows16<N, DP, A, W::PLANE>(acc, off, qf);
+      rows16<N, DP, A + W::TILE, W::PLANE>(dp, off, df);
+      float sc[16];
 #pragma unroll
-      for (int sub = 0; sub < BN / 32; ++sub) {
-        const int cls = wave_ok ? seen_class(a, s, j0 + 32 * sub, wp0, wp1) : 0;
-        if (!cls) continue;
-        f32x16 acc, dp;
-        rows_times<T, DP>(acc, kt, 32 * sub, qf, lane);
-        rows_times<T, DP>(dp, vt, 32 * sub, df, lane);
-        float sc[16];
+      for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -lse2)) * (dp[e] - delta);
+      if (cls == 1) {
+        const int base = j0 + 4 * (lane >> 5);
+        const int hi = min(p + a.right, s.kl - 1) - base, lo = p - a.left - base, sk = a.sinks - base;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -lse2)) * (dp[e] - delta);
-        if (cls == 1) {
-          const int base = j0 + 32 * sub + 4 * (lane >> 5);
-          const int hi = min(p + a.right, s.kl - 1) - base, lo = p - a.left - base, sk = a.sinks - base;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int x = 8 * (e >> 2) + (e & 3);
-            if (!(x <= hi && (x >= lo || x < sk))) sc[e] = 0.f;
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int x = 8 * (e >> 2) + (e & 3);
+          if (!(x <= hi && (x >= lo || x < sk))) sc[e] = 0.f;
         }
-        cols_times<DP>(dq, kt, 32 * sub, sc, lane, T());
       }
-    }
+      cols16<N, DP, A, W::PLANE>(dq, off, sc);
+    };
+    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&](int j0, auto st) {
+      constexpr uint32_t S0 = decltype(st)::value;
+      one(j0, std::integral_constant<uint32_t, S0>());
+      if constexpr (W::BN == 64) one(j0 + 32, std::integral_constant<uint32_t, S0 + 32 * G16<DP>::PITCH>());
+    });
   }
   bool bad = false;
   if (r < R) {
-    T* drow = (T*)a.dq + b * a.dq_bs + (long)i * a.dq_ts + hq * a.dq_hs;
+    T* qrow = (T*)a.dq + b * a.dq_bs + (long)i * a.dq_ts + hq * a.dq_hs;
     const int h4 = 4 * (lane >> 5);
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v[4];
@@ -775,7 +1029,7 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a
           v[x] = row_ok ? dq[d][4 * e + x] * a.scale : 0.f;
           bad |= v[x] != v[x];
         }
-        if (32 * d + 8 * e + h4 < a.D) store4<T>(drow + 32 * d + 8 * e + h4, v);
+        if (32 * d + 8 * e + h4 < a.D) store4<T>(qrow + 32 * d + 8 * e + h4, v);
       }
   }
   uint64_t again = __ballot(bad && lse2 == lse2 && delta == delta);
@@ -788,30 +1042,64 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a
 #endif
 }
 
-// Stages 32 packed rows (query i, head g of the group) of q or dout from row r0: row r at (r / G) * ts + (r % G) * hs
-template <typename T, int DP, int NW>
-__device__ __forceinline__ void stage_packed(uint32_t lds, const T* base, long ts, long hs, int gsize, int r0, int rend, int dbytes, int wave, int lane) {
-  using G = Geo<T, DP>;
-  constexpr int TOTAL = 32 * G::PITCH / 1024;
-  const int i0 = r0 / gsize;
-  const u32x4 srd = make_srd(base + i0 * ts);
-  const uint32_t tsb = ts * G::ES, hsb = hs * G::ES;
+// One thread's part of staging ROWS packed rows (query i, head g of the group) of q or dout: row r lies at (r / G) * ts + (r % G) * hs
+template <typename T, int DP, int ROWS>
+struct PackedStager;
+template <int DP, int ROWS>
+struct PackedStager<__bf16, DP, ROWS> {
+  using G = G16<DP>;
+  static constexpr int TOTAL = ROWS * G::PITCH / 1024;
+  __device__ __forceinline__ void load(uint32_t lds, const __bf16* base, long ts, long hs, int gs, int r0, int rend, int D, int wave, int lane) {
+    const int i0 = r0 / gs;
+    const u32x4 srd = make_srd(base + i0 * ts);
+    const uint32_t tsb = ts * 2, hsb = hs * 2;
 #pragma unroll
-  for (int n = 0; n < (TOTAL + NW - 1) / NW; ++n) {
-    const int it = wave + n * NW;
-    if (TOTAL % NW == 0 || it < TOTAL) {
-      const int row = it * G::RPI + lane / G::CH;
-      const int chunk = (lane % G::CH) ^ swz<T, DP>(row);
-      const int i = (r0 + row) / gsize, g = r0 + row - i * gsize;
-      const bool ok = r0 + row < rend && chunk * 16 < dbytes;
-      dma16(lds + it * 1024, ok ? (uint32_t)(i - i0) * tsb + (uint32_t)g * hsb + chunk * 16 : kOutside, srd);
+    for (int n = 0; n < (TOTAL + 3) / 4; ++n) {
+      const int it = wave + n * 4;
+      if (TOTAL % 4 == 0 || it < TOTAL) {
+        const int row = it * (1024 / G::PITCH) + lane / G::CH, chunk = (lane % G::CH) ^ swz<__bf16, DP>(row);
+        const int i = (r0 + row) / gs, g = r0 + row - i * gs;
+        const bool ok = r0 + row < rend && chunk * 8 < D;
+        dma16(lds + it * 1024, ok ? (uint32_t)(i - i0) * tsb + (uint32_t)g * hsb + chunk * 16 : kOutside, srd);
+      }
     }
   }
-}
-// 32 rows' {log2-sum-exp, delta}: 256 bytes, by one wave
-__device__ __forceinline__ void stage_stat(uint32_t lds, const float* st, int lane) {
-  dma16(lds, lane < 16 ? lane * 16u : kOutside, make_srd(st));
-}
+  __device__ __forceinline__ void put(uint32_t) const {}
+};
+template <int DP, int ROWS>
+struct PackedStager<float, DP, ROWS> {
+  using G = G16<DP>;
+  static constexpr int ITEMS = ROWS * G::CH, PER = (ITEMS + 255) / 256;
+  static constexpr uint32_t PLANE = ROWS * G::PITCH;
+  u32x4 held[PER][2];
+  __device__ __forceinline__ void load(uint32_t, const float* base, long ts, long hs, int gs, int r0, int rend, int D, int, int) {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
+      const int i = (r0 + row) / gs, g = r0 + row - i * gs;
+      const bool ok = r0 + row < rend && chunk * 8 < D && item < ITEMS;
+      const float* p = base + i * ts + g * hs + chunk * 8;
+      held[n][0] = ok ? *reinterpret_cast<const u32x4*>(p) : (u32x4){0u, 0u, 0u, 0u};
+      held[n][1] = ok ? *reinterpret_cast<const u32x4*>(p + 4) : (u32x4){0u, 0u, 0u, 0u};
+    }
+  }
+  __device__ __forceinline__ void put(uint32_t lds) const {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
+      if (ITEMS % 256 == 0 || item < ITEMS) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(held[n][0][i]), x[4 + i] = __uint_as_float(held[n][1][i]);
+        bf16x8 p[3];
+        split8<3>(x, p);
+        const uint32_t at = lds + row * G::PITCH + ((chunk ^ swz<__bf16, DP>(row)) << 4);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<lds_u32x4_t*>(at + k * PLANE) = __builtin_bit_cast(u32x4, p[k]);
+      }
+    }
+  }
+};
 
 // The gradients of one key (and value) row over the query rows that see it alone (see row_again)
 template <typename T>
@@ -849,19 +1137,26 @@ __device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, i
   if (on1) dk[d1] = (T)(dk1 * a.scale), dv[d1] = (T)dv1;
 }
 
-// One step of the dK / dV walk: 32 staged rows against this wave's 32 keys.  Element e of S is row 8 (e / 4) + 4 h + e % 4, column the lane's
-// key; [rlo, rhi] are the packed rows (of the whole sequence) that see the lane's key, checked when `part`.
+// What the dK / dV kernel walks over the rows with: RS rows a stage (q, dout and their {log2-sum-exp, delta}), two stages for bf16
 template <typename T, int DP>
-__device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32], uint32_t qt, uint32_t dt, uint32_t st, const Frags<T, DP>& kf,
-                                         const Frags<T, DP>& vf, float c, bool part, int r0, int rlo, int rhi, int lane) {
+struct RowWalk {
+  static constexpr int N = Planes<T>::N, RS = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
+  static constexpr uint32_t PLANE = RS * G16<DP>::PITCH, TILE = N * PLANE, STAT = 2 * TILE, STAGE = 2 * TILE + 1024, LDS = NSTAGE * STAGE;
+};
+// One step: the 32 staged rows at A (statistics at ST) against this wave's 32 keys.  Element e of S is row 8 (e / 4) + 4 h + e % 4, column the
+// lane's key; [rlo, rhi] are the packed rows (of the whole sequence) that see the lane's key, checked when `part`.
+template <typename T, int DP, uint32_t A, uint32_t ST>
+__device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32], const LaneOff<DP>& off, uint32_t stat,
+                                         const Frags16<Planes<T>::N, DP>& kf, const Frags16<Planes<T>::N, DP>& vf, float c, bool part, int r0, int rlo, int rhi,
+                                         int lane) {
+  using W = RowWalk<T, DP>;
   f32x16 acc, dp;
-  rows_times<T, DP>(acc, qt, 0, kf, lane);
-  rows_times<T, DP>(dp, dt, 0, vf, lane);
+  rows16<W::N, DP, A, W::PLANE>(acc, off, kf);
+  rows16<W::N, DP, A + W::TILE, W::PLANE>(dp, off, vf);
   float p[16], ds[16];
-  const uint32_t sa = st + 16 * (lane >> 5);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const u32x4 l4 = lds_ld16(sa + 32 * e), d4 = lds_ld16(sa + 128 + 32 * e);
+    const u32x4 l4 = lds_ld16(stat + ST + 32 * e), d4 = lds_ld16(stat + ST + 128 + 32 * e);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       p[4 * e + x] = __builtin_amdgcn_exp2f(fmaf(acc[4 * e + x], c, -__uint_as_float(l4[x])));
@@ -876,93 +1171,140 @@ __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP 
       if (row < rlo || row > rhi) p[e] = 0.f, ds[e] = 0.f;
     }
   }
-  cols_times<DP>(dv, dt, 0, p, lane, T());
-  cols_times<DP>(dk, qt, 0, ds, lane, T());
+  cols16<W::N, DP, A + W::TILE, W::PLANE>(dv, off, p);
+  cols16<W::N, DP, A, W::PLANE>(dk, off, ds);
 }
 
-// dK / dV of 128 keys: 4 waves x 32 keys, the rows inside the window in steps of 32.  Keys that are sinks leave their fp32 sums as share 0.
+// dK / dV.  Workgroups from nsink on: 128 keys, 4 waves x 32 keys, the rows inside the keys' windows.  The first nsink workgroups: the rows
+// beyond the window of 32 KB keys that are sinks, a share of them each; the waves are KB key blocks x row blocks of a stage, and every wave
+// leaves its fp32 sums.  Sinks among the 128 keys leave theirs as share 0.
 template <typename T, int DP, int OCC>
 __global__ __launch_bounds__(256, OCC) void window_attn_dkv_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using G = Geo<T, DP>;
+  using W = RowWalk<T, DP>;
+  constexpr int ND = DP / 32, N = W::N, NB = W::RS / 32, KB = 4 / NB;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  constexpr uint32_t TILE = 32 * G::PITCH, STAGE = 2 * TILE + 1024;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = xcd_item(gridDim.x);
-  const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int nst = (a.sink_rows / 32 + KB - 1) / KB;                      // sink tiles of a (batch, key head)
+  const int nsink = a.B * a.Hkv * nst * a.nsplit;
+  const bool far = (int)blockIdx.x < nsink;
+  int bh, jw, split = 0;
+  if (far) {
+    const int bht = blockIdx.x / a.nsplit;
+    split = blockIdx.x % a.nsplit;
+    bh = bht / nst;
+    jw = (bht % nst) * KB * 32 + (wave % KB) * 32;
+  } else {
+    const int n = gridDim.x - nsink, x = blockIdx.x - nsink, per = n >> 3, rest = n & 7, dev = x & 7;   // (see xcd_item)
+    const int item = dev * per + min(dev, rest) + (x >> 3);
+    bh = item / a.ntiles;
+    jw = (item % a.ntiles) * 128 + wave * 32;
+  }
+  const int hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
-  const int j0 = tile * 128, jw = j0 + wave * 32, j = jw + (lane & 31);
-  const bool key_ok = j < s.kl;
-  Frags<T, DP> kf, vf;
-  load_frags<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
-  load_frags<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
-  f32x16 dk[G::ND], dv[G::ND];
+  const int j = jw + (lane & 31);
+  const int kend = far ? min(s.kl, a.sinks) : s.kl;                       // keys of this pass
+  const bool key_ok = j < kend;
+  Frags16<N, DP> kf, vf;
+  load_frags16<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
+  load_frags16<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
+  f32x16 dk[ND], dv[ND];
 #pragma unroll
-  for (int d = 0; d < G::ND; ++d)
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
-  arrived(kf);
-  arrived(vf);
-  // query rows (of the sequence) whose window holds a key of [first, last]
-  auto rows_of = [&](int first, int last, int& lo, int& hi) {
-    lo = max(0, first - a.right - s.shift);
-    hi = min(s.ql - 1, last + a.left - s.shift);
-  };
+  arrived16(kf);
+  arrived16(vf);
   const float c = a.scale * kLog2e;
-  const int jlast = min(j0 + 127, s.kl - 1);
-  if (j0 <= jlast) {
-    int ilo, ihi, wlo, whi;
-    rows_of(j0, jlast, ilo, ihi);
-    const int jwl = min(jw + 31, s.kl - 1);
-    rows_of(jw, jwl, wlo, whi);
-    const bool wave_ok = jw <= jwl && wlo <= whi;
-    const int wr0 = wlo * a.G, wr1 = (whi + 1) * a.G;                  // rows some key of this wave is seen by
-    // rows all of its keys are seen by (none when the sequence ends among them)
-    const int fr0 = max(0, min(a.Tq, jw + 31 - a.right - s.shift)) * a.G;
-    const int fr1 = jw + 31 < s.kl ? min(s.ql, max(-1, jw + a.left - s.shift) + 1) * a.G : 0;
-    // this lane's key
-    const int rlo = key_ok ? max(0, min(a.Tq, j - a.right - s.shift)) * a.G : 1, rhi = key_ok ? min(s.ql, max(-1, j + a.left - s.shift) + 1) * a.G - 1 : 0;
-    const int t0 = ilo * a.G / 32, t1 = ihi >= ilo ? ((ihi + 1) * a.G + 31) / 32 : t0;
+  // Queries [lo(first), hi(last)] see a key of [first, last]: inside the window from first - right on up to last + left, beyond it from
+  // first + left + 1 on; clamped to [0, q_len], the end exclusive
+  auto lo = [&](int key) { return max(0, min(s.ql, far ? key + a.left - s.shift + 1 : key - a.right - s.shift)); };
+  auto hi = [&](int key) { return far ? s.ql : max(0, min(s.ql, key + a.left - s.shift + 1)); };
+  const int block_first = far ? jw - (wave % KB) * 32 : jw - wave * 32, block_last = min(block_first + (far ? KB * 32 : 128), kend) - 1;
+  const int wave_last = min(jw + 31, kend - 1);
+  if (block_first <= block_last) {
+    int t0 = lo(block_first) * a.G / W::RS, t1 = (hi(block_last) * a.G + W::RS - 1) / W::RS;
+    if (far) {
+      const int per = (max(0, t1 - t0) + a.nsplit - 1) / a.nsplit;
+      t0 += split * per;
+      t1 = min(t1, t0 + per);
+    }
+    const bool wave_ok = jw <= wave_last;
+    const int wr0 = lo(jw) * a.G, wr1 = wave_ok ? hi(wave_last) * a.G : 0;             // rows some key of this wave is seen by
+    const int fr0 = lo(jw + 31) * a.G, fr1 = jw + 31 < kend ? hi(jw) * a.G : 0;          // rows all of its keys are seen by
+    const int rlo = key_ok ? lo(j) * a.G : 1, rhi = key_ok ? hi(j) * a.G - 1 : 0;        // this lane's key
     const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
     const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
     const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
-    const int rend = s.ql * a.G, dbytes = a.D * G::ES;
-    auto stage = [&](int t) {
-      const uint32_t dst = lds + (t & 1) * STAGE;
-      stage_packed<T, DP, 4>(dst, qb, a.q_ts, a.q_hs, a.G, t * 32, rend, dbytes, wave, lane);
-      stage_packed<T, DP, 4>(dst + TILE, db, a.do_ts, a.do_hs, a.G, t * 32, rend, dbytes, wave, lane);
-      if (wave == 0) stage_stat(dst + 2 * TILE, stat + (long)t * 64, lane);
+    const int rend = s.ql * a.G;
+    const LaneOff<DP> off(lds, lane);
+    const uint32_t stat_off = lds + W::STAT + 16 * (lane >> 5);
+    PackedStager<T, DP, W::RS> sq, sd;
+    auto load = [&](int t, uint32_t at) {
+      sq.load(at, qb, a.q_ts, a.q_hs, a.G, t * W::RS, rend, a.D, wave, lane);
+      sd.load(at + W::TILE, db, a.do_ts, a.do_hs, a.G, t * W::RS, rend, a.D, wave, lane);
+      if (wave == 0) dma16(at + W::STAT, lane < W::RS / 2 ? lane * 16u : kOutside, make_srd(stat + (long)t * (2 * W::RS)));
     };
-    if (t0 < t1) stage(t0);
-    for (int t = t0; t < t1; ++t) {
-      wait_vm<0>();
-      wg_barrier();
-      if (t + 1 < t1) stage(t + 1);
-      const int r0 = t * 32;
-      if (wave_ok && r0 < wr1 && r0 + 32 > wr0) {
-        const uint32_t qt = lds + (t & 1) * STAGE;
-        dkv_step<T, DP>(dk, dv, qt, qt + TILE, qt + 2 * TILE, kf, vf, c, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
+    auto step = [&](int t, auto st) {
+      constexpr uint32_t S0 = decltype(st)::value;
+      auto sub = [&](auto k) {
+        constexpr int B32 = decltype(k)::value;
+        const int r0 = t * W::RS + 32 * B32;
+        if ((far && NB > 1 && wave / KB != B32) || r0 >= wr1 || r0 + 32 <= wr0) return;
+        dkv_step<T, DP, S0 + B32 * 32 * G16<DP>::PITCH, S0 + B32 * 256>(dk, dv, off, stat_off, kf, vf, c, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
+      };
+      sub(std::integral_constant<int, 0>());
+      if constexpr (NB == 2) sub(std::integral_constant<int, 1>());
+    };
+    if (t0 < t1) load(t0, lds);
+    if constexpr (N == 1) {
+      for (int t = t0; t < t1; t += 2) {
+        wait_vm<0>();
+        wg_barrier();
+        if (t + 1 < t1) load(t + 1, lds + W::STAGE);
+        step(t, std::integral_constant<uint32_t, 0>());
+        if (t + 1 >= t1) break;
+        wait_vm<0>();
+        wg_barrier();
+        if (t + 2 < t1) load(t + 2, lds);
+        step(t + 1, std::integral_constant<uint32_t, W::STAGE>());
+      }
+    } else {
+      for (int t = t0; t < t1; ++t) {
+        if (t > t0) wg_barrier();            // the tile before has been read
+        sq.put(lds);
+        sd.put(lds + W::TILE);
+        if (t > t0 && wave == 0) dma16(lds + W::STAT, lane < W::RS / 2 ? lane * 16u : kOutside, make_srd(stat + (long)t * (2 * W::RS)));
+        wait_vm<0>();
+        if (t + 1 < t1) {
+          sq.load(lds, qb, a.q_ts, a.q_hs, a.G, (t + 1) * W::RS, rend, a.D, wave, lane);
+          sd.load(lds + W::TILE, db, a.do_ts, a.do_hs, a.G, (t + 1) * W::RS, rend, a.D, wave, lane);
+        }
+        wg_barrier();
+        step(t, std::integral_constant<uint32_t, 0>());
       }
     }
   }
   bool bad = false;
   const int h4 = 4 * (lane >> 5);
-  if (j < a.sink_rows) {
-    float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP;
+  if (far || j < a.sinks) {
+    if (j < a.sink_rows) {
+      float* part = a.part + (((long)bh * a.nparts + (far ? 1 + split * NB + wave / KB : 0)) * a.sink_rows + j) * 2 * DP;
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d)
+      for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = 32 * d + 8 * e + h4;
-        *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
-        *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
-      }
+        for (int e = 0; e < 4; ++e) {
+          const int at = 32 * d + 8 * e + h4;
+          *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
+          *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
+        }
+    }
   } else if (j < a.Tk) {
     T* krow = (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs;
     T* vrow = (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float x[4], y[4];
@@ -986,106 +1328,35 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dkv_kernel(const WaArgs 
 #endif
 }
 
-// The sinks' rows beyond the window: 32 keys a workgroup, every wave takes its own row tiles of this share through a ring of two stages
+// The sinks' shares, in order: one workgroup a key row, its 4 waves take the shares in turn
 template <typename T, int DP>
-struct SinkGeo {
-  using G = Geo<T, DP>;
-  static constexpr uint32_t TILE = 32 * G::PITCH, STAGE = 2 * TILE + 1024;
-  static constexpr int NW = G::PITCH > 256 ? 2 : 4;
-  static constexpr int LDS = NW * 2 * STAGE;
-};
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 1) void window_attn_dkv_sink_kernel(const WaArgs a) {
+__global__ __launch_bounds__(256) void window_attn_dkv_join_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using G = Geo<T, DP>;
-  using SG = SinkGeo<T, DP>;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = xcd_item(gridDim.x);
-  const int split = item % a.nsplit, nst = a.sink_rows / 32, bht = item / a.nsplit, tile = bht % nst, bh = bht / nst, hk = bh % a.Hkv, b = bh / a.Hkv;
-  const Seq s = seq_of(a, b);
-  const int j0 = tile * 32, j = j0 + (lane & 31);
-  const bool key_ok = j < s.kl && j < a.sinks;
-  Frags<T, DP> kf, vf;
-  load_frags<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
-  load_frags<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
-  f32x16 dk[G::ND], dv[G::ND];
-#pragma unroll
-  for (int d = 0; d < G::ND; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
-  arrived(kf);
-  arrived(vf);
-  // row i sees sink j from beyond the window when i > j + left - shift (and i >= j - right - shift, which that implies unless right < 0)
-  const int jl = min(min(j0 + 31, a.sinks - 1), s.kl - 1);
-  const float c = a.scale * kLog2e;
-  if (j0 <= jl) {
-    const int first = max(0, j0 + a.left - s.shift + 1);                       // the first row for the first of these keys
-    const int all = jl < j0 + 31 ? a.Tq : max(0, j0 + 31 + a.left - s.shift + 1);   // from here on every key of the tile is seen
-    const int rlo = key_ok ? max(0, min(a.Tq, j + a.left - s.shift + 1)) * a.G : 1, rhi = key_ok ? s.ql * a.G - 1 : 0;
-    const int rend = s.ql * a.G, dbytes = a.D * G::ES;
-    const int t0 = min(first, s.ql) * a.G / 32, t1 = first < s.ql ? (rend + 31) / 32 : t0, per = (t1 - t0 + a.nsplit - 1) / a.nsplit;
-    const int at = t0 + split * per + wave, end = min(t1, t0 + (split + 1) * per);
-    const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
-    const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
-    const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
-    const uint32_t ring = lds + wave * 2 * SG::STAGE;
-    auto stage = [&](int t, int buf) {
-      const uint32_t dst = ring + buf * SG::STAGE;
-      stage_packed<T, DP, 1>(dst, qb, a.q_ts, a.q_hs, a.G, t * 32, rend, dbytes, 0, lane);
-      stage_packed<T, DP, 1>(dst + SG::TILE, db, a.do_ts, a.do_hs, a.G, t * 32, rend, dbytes, 0, lane);
-      stage_stat(dst + 2 * SG::TILE, stat + (long)t * 64, lane);
-    };
-    int buf = 0;
-    if (at < end) stage(at, 0);
-    for (int t = at; t < end; t += SG::NW, buf ^= 1) {
-      if (t + SG::NW < end) {
-        stage(t + SG::NW, buf ^ 1);
-        wait_vm<2 * 32 * G::PITCH / 1024 + 1>();
-      } else {
-        wait_vm<0>();
-      }
-      const uint32_t qt = ring + buf * SG::STAGE;
-      const int r0 = t * 32;
-      dkv_step<T, DP>(dk, dv, qt, qt + SG::TILE, qt + 2 * SG::TILE, kf, vf, c, r0 < min(all, a.Tq) * a.G || r0 + 32 > rend, r0, rlo, rhi, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-  }
-  float* part = a.part + (((long)bh * a.nparts + 1 + split * SG::NW + wave) * a.sink_rows + j) * 2 * DP;
-  const int h4 = 4 * (lane >> 5);
-#pragma unroll
-  for (int d = 0; d < G::ND; ++d)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int at = 32 * d + 8 * e + h4;
-      *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
-      *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
-    }
-#endif
-}
-
-// The sinks' shares in order: one wave per key row
-template <typename T, int DP>
-__global__ __launch_bounds__(64) void window_attn_dkv_join_kernel(const WaArgs a) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const int lane = threadIdx.x;
-  const int nk = min(a.sink_rows, a.Tk);
+  constexpr int PER = 2 * DP / 64;
+  __shared__ float share[4][2 * DP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nk = min(a.sinks, a.Tk);
   const int j = blockIdx.x % nk, bh = blockIdx.x / nk, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
-  float sum[2 * DP / 64];
+  float sum[PER];
 #pragma unroll
-  for (int x = 0; x < 2 * DP / 64; ++x) sum[x] = 0.f;
-  const float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP;
-  for (int n = 0; n < a.nparts; ++n)
+  for (int x = 0; x < PER; ++x) sum[x] = 0.f;
+  const float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP + lane;
+#pragma unroll 4
+  for (int n = wave; n < a.nparts; n += 4)
 #pragma unroll
-    for (int x = 0; x < 2 * DP / 64; ++x) sum[x] += part[(long)n * a.sink_rows * 2 * DP + 64 * x + lane];
+    for (int x = 0; x < PER; ++x) sum[x] += part[(long)n * a.sink_rows * 2 * DP + 64 * x];
+#pragma unroll
+  for (int x = 0; x < PER; ++x) share[wave][64 * x + lane] = sum[x];
+  __syncthreads();
+  if (wave) return;
   bool bad = false;
 #pragma unroll
-  for (int x = 0; x < 2 * DP / 64; ++x) {
+  for (int x = 0; x < PER; ++x) {
     const int at = 64 * x + lane, d = at % DP;
     const bool isk = at < DP;
-    const float v = j < s.kl ? (isk ? sum[x] * a.scale : sum[x]) : 0.f;
+    const float t = (share[0][at] + share[1][at]) + (share[2][at] + share[3][at]);
+    const float v = j < s.kl ? (isk ? t * a.scale : t) : 0.f;
     T* row = isk ? (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs : (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
     if (d < a.D) {
       row[d] = (T)v;
@@ -1182,7 +1453,6 @@ int reserve_lds(K kernel, size_t bytes, bool& done) {
 
 template <typename T, int DP>
 int launch_forward(WaArgs& a, const Plan& p, hipStream_t st) {
-  using G = Geo<T, DP>;
   const long bh = (long)a.B * a.Hkv;
   a.ntiles = p.ntiles, a.nsplit = p.nsplit;
   if (p.few) {
@@ -1194,8 +1464,7 @@ int launch_forward(WaArgs& a, const Plan& p, hipStream_t st) {
     }
     return TDX_OK;
   }
-  constexpr int BN = sizeof(T) == 4 ? 32 : 64;
-  WA_LAUNCH((window_attn_kernel<T, DP, BN>), bh * p.ntiles, 256, (4 * BN * G::PITCH), st, a);
+  WA_LAUNCH((window_attn_kernel<T, DP>), bh * p.ntiles, 256, (Walk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_kernel");
   return TDX_OK;
 }
@@ -1218,12 +1487,12 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
   const int64_t rows = (int64_t)a.Tq * a.G, bh = (int64_t)a.B * a.Hkv, dp = padded(a.D);
   p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
   if (a.sinks > 0) {
-    const int nw = dp * es > 256 ? 2 : 4;
+    const int nb = es == 4 ? 1 : 2, kb = 4 / nb;                        // row and key blocks of a workgroup (RowWalk)
     p.sink_rows = (a.sinks + 31) / 32 * 32;
-    const int64_t wgs = bh * (p.sink_rows / 32);
-    // two workgroups a compute unit, 4 row tiles a wave at least
-    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((2 * compute_units() + wgs - 1) / wgs, rows / 32 / (4 * nw)));
-    p.nparts = 1 + p.nsplit * nw;
+    const int64_t wgs = bh * ((p.sink_rows / 32 + kb - 1) / kb);
+    // one workgroup a compute unit, 8 stages each at least
+    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((compute_units() + wgs - 1) / wgs, rows / (nb * 32 * 8)));
+    p.nparts = 1 + p.nsplit * nb;
     p.part_bytes = bh * p.nparts * p.sink_rows * 2 * dp * 4;
   }
   return p;
@@ -1231,22 +1500,19 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
 
 template <typename T, int DP>
 int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
-  using G = Geo<T, DP>;
   const long bh = (long)a.B * a.Hkv;
-  constexpr int BN = sizeof(T) == 4 ? 32 : 64, OCC = DP == 128 ? 1 : 2;
+  constexpr int OCC = DP == 128 ? 1 : 2, KB = 4 / (RowWalk<T, DP>::RS / 32);
   const long rt = ((long)a.Tq * a.G + 127) / 128;
   a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows;
-  WA_LAUNCH((window_attn_dq_kernel<T, DP, BN, OCC>), bh * rt, 256, (4 * BN * G::PITCH), st, a);
+  WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dq_kernel");
   if (a.Tk == 0) return TDX_OK;
-  // every share row of the sinks has a key tile that writes it
-  a.ntiles = (std::max(a.Tk, a.sink_rows) + 127) / 128;
-  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), bh * a.ntiles, 256, (2 * (64 * G::PITCH + 1024)), st, a);
+  a.ntiles = (a.Tk + 127) / 128;
+  const long sink_wgs = bh * ((p.sink_rows / 32 + KB - 1) / KB) * p.nsplit;
+  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), sink_wgs + bh * a.ntiles, 256, (RowWalk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dkv_kernel");
   if (p.sink_rows) {
-    WA_LAUNCH((window_attn_dkv_sink_kernel<T, DP>), bh * (p.sink_rows / 32) * p.nsplit, (SinkGeo<T, DP>::NW * 64), (SinkGeo<T, DP>::LDS), st, a);
-    TDX_CHECK_LAUNCH("window_attn_dkv_sink_kernel");
-    hipLaunchKernelGGL((window_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(bh * std::min(p.sink_rows, a.Tk))), dim3(64), 0, st, a);
+    hipLaunchKernelGGL((window_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(bh * std::min(a.sinks, a.Tk))), dim3(256), 0, st, a);
     TDX_CHECK_LAUNCH("window_attn_dkv_join_kernel");
   }
   return TDX_OK;
