@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -32,27 +33,29 @@ _LAYOUTS = {"halves": 0, "pairs": 1}
 _CODES = {torch.float32: _lib.TDX_F32, torch.bfloat16: _lib.TDX_BF16}
 _MAX = 1 << 28     # lengths and limits the kernels count in
 
+# Filled descriptors by what they were filled from (shapes, strides, types, limits: no addresses), one set per thread: a call of a form that
+# was seen before sets its pointers and launches.  The library reads a descriptor during the call only.
+_seen = threading.local()
+_MOST_SEEN = 256
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+
+def _known(kind: str) -> dict:
+    got = _seen.__dict__.setdefault(kind, {})
+    if len(got) > _MOST_SEEN:
+        got.clear()
+    return got
 
 
-class _On:
-    """The tensors' device as the current one (the library launches on the current device), switched only when it is another."""
-    __slots__ = ("dev", "old")
-
-    def __init__(self, t: torch.Tensor):
-        self.dev = t.device.index
-
-    def __enter__(self):
-        self.old = torch.cuda.current_device()
-        if self.old != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.old != self.dev:
-            torch.cuda.set_device(self.old)
-        return False
+def _launch(fn, name: str, d, index: int) -> None:
+    """fn(descriptor, stream) on the current stream of device `index` (the library launches on the current device)."""
+    old = torch._C._cuda_getDevice()
+    if old == index:
+        rc = fn(C.byref(d), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(C.byref(d), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
@@ -69,18 +72,28 @@ def _check4(t: torch.Tensor, name: str, fn: str) -> None:
 
 
 # ---- rotary positions ---------------------------------------------------------------------------------------------------------------
-def _rotary_launch(x, pos, sections, bases, layout, inverse, out) -> None:
+def _rotary_desc(x, pos, sections, bases, layout, inverse, out) -> RotaryDesc:
     d = RotaryDesc()
-    d.x, d.out, d.pos = x.data_ptr(), out.data_ptr(), pos.data_ptr()
     d.x_bs, d.x_ts, d.x_hs = _strides(x)
     d.out_bs, d.out_ts, d.out_hs = _strides(out)
     d.pos_bs, d.pos_ts, d.pos_as = pos.stride()
+    if pos.shape[0] != x.shape[0]:
+        d.pos_bs = 0
     d.B, d.T, d.H, d.D = x.shape
     d.dtype, d.layout, d.inverse, d.naxes = _CODES[x.dtype], layout, int(inverse), len(sections)
     d.sections[:len(sections)] = sections
     d.base[:len(sections)] = bases
-    with _On(x):
-        _lib.check(_lib.lib().tdx_rotary_axes(C.byref(d), _stream(x)), "tdx_rotary_axes")
+    return d
+
+
+def _rotary_launch(x, pos, sections, bases, layout, inverse, out) -> None:
+    key = (x.shape, x.stride(), x.dtype, pos.shape, pos.stride(), sections, bases, layout, inverse, None if out.is_contiguous() else out.stride())
+    known = _known("rotary")
+    d = known.get(key)
+    if d is None:
+        d = known[key] = _rotary_desc(x, pos, sections, bases, layout, inverse, out)
+    d.x, d.out, d.pos = x.data_ptr(), out.data_ptr(), pos.data_ptr()
+    _launch(_lib.lib().tdx_rotary_axes, "tdx_rotary_axes", d, x.get_device())
 
 
 class _Rotary(torch.autograd.Function):
@@ -93,15 +106,36 @@ class _Rotary(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        if torch.is_grad_enabled():
+            raise TdxError("rotary_axes: second derivatives are not provided")
         pos, = ctx.saved_tensors
         sections, bases, layout, inverse = ctx.args
         if dout.stride(3) != 1 and dout.shape[3] != 1:
             dout = dout.contiguous()
         dx = torch.empty(dout.shape, dtype=dout.dtype, device=dout.device)
-        _rotary_launch(dout, pos, sections, bases, layout, not inverse, dx)   # a rotation's transpose is its inverse
+        if dx.numel():
+            _rotary_launch(dout, pos, sections, bases, layout, not inverse, dx)   # a rotation's transpose is its inverse
         return dx, None, None, None, None, None
+
+
+def _rotary_args(x, pos, sections, base, layout) -> Tuple:
+    """(sections, bases, layout code) of a call whose arguments go together; raises otherwise."""
+    fn = "rotary_axes"
+    _check4(x, "x", fn)
+    if layout not in _LAYOUTS:
+        raise TdxError(f"{fn}: layout {layout!r}; use 'halves' or 'pairs'")
+    sections = tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 8 or min(sections) < 0 or not 1 <= sum(sections) <= x.shape[3] // 2:
+        raise TdxError(f"{fn}: sections {sections} do not fit heads of {x.shape[3]} channels (1 to 8 axes, at most D / 2 pairs)")
+    bases = tuple(float(b) for b in base) if isinstance(base, (list, tuple)) else (float(base),) * len(sections)
+    if len(bases) != len(sections) or not all(math.isfinite(b) and b > 0 for b in bases):
+        raise TdxError(f"{fn}: base {base!r} for {len(sections)} axes (finite, > 0)")
+    if not isinstance(pos, torch.Tensor) or pos.dtype != torch.float32 or pos.device != x.device:
+        raise TdxError(f"{fn}: pos must be an fp32 tensor on {x.device}")
+    if pos.dim() not in (2, 3) or (pos.dim() == 3 and pos.shape[0] not in (1, x.shape[0])) or pos.shape[-2:] != (x.shape[1], len(sections)):
+        raise TdxError(f"{fn}: pos {tuple(pos.shape)} for x {tuple(x.shape)} and {len(sections)} axes")
+    return sections, bases, _LAYOUTS[layout]
 
 
 def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], base: Union[float, Sequence[float]] = 10000.0, layout: str = "halves",
@@ -116,64 +150,60 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     out       write here (x itself: in place); not differentiable
     Differentiable in x.  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
-    _check4(x, "x", fn)
-    if layout not in _LAYOUTS:
-        raise TdxError(f"{fn}: layout {layout!r}; use 'halves' or 'pairs'")
-    sections = tuple(int(n) for n in sections)
-    if not 1 <= len(sections) <= 8 or min(sections) < 0 or not 1 <= sum(sections) <= x.shape[3] // 2:
-        raise TdxError(f"{fn}: sections {sections} do not fit heads of {x.shape[3]} channels (1 to 8 axes, at most D / 2 pairs)")
-    bases = tuple(float(b) for b in base) if isinstance(base, (list, tuple)) else (float(base),) * len(sections)
-    if len(bases) != len(sections) or not all(math.isfinite(b) and b > 0 for b in bases):
-        raise TdxError(f"{fn}: base {base!r} for {len(sections)} axes (finite, > 0)")
-    if not isinstance(pos, torch.Tensor) or pos.dtype != torch.float32 or pos.device != x.device:
-        raise TdxError(f"{fn}: pos must be an fp32 tensor on {x.device}")
+    try:   # a form of call that was checked before?
+        key = (x.shape, x.dtype, x.device, pos.shape, pos.dtype, pos.device, tuple(sections), base if base.__class__ is float else tuple(base), layout)
+        args = _known("rotary_args").get(key)
+    except (AttributeError, TypeError):
+        key = args = None
+    if args is None:
+        args = _rotary_args(x, pos, sections, base, layout)
+        if key is not None:
+            _known("rotary_args")[key] = args
+    sections, bases, code = args
     if pos.requires_grad:
         raise TdxError(f"{fn}: positions have no gradient; detach them")
     if pos.dim() == 2:
         pos = pos.unsqueeze(0)
-    if pos.dim() != 3 or pos.shape[0] not in (1, x.shape[0]) or pos.shape[1:] != (x.shape[1], len(sections)):
-        raise TdxError(f"{fn}: pos {tuple(pos.shape)} for x {tuple(x.shape)} and {len(sections)} axes")
-    if pos.shape[0] != x.shape[0]:
-        pos = pos.expand(x.shape[0], -1, -1)
     if x.stride(3) != 1 and x.shape[3] != 1:
         if out is x:
             raise TdxError(f"{fn}: in place needs contiguous channels")
         x = x.contiguous()
-    code = _LAYOUTS[layout]
     if out is not None:
         _check4(out, "out", fn)
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
             raise TdxError(f"{fn}: out must be like x, with contiguous channels")
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise TdxError(f"{fn}: out= is not differentiable")
-        if 0 in out.stride() and any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
             raise TdxError(f"{fn}: out must not repeat its own memory")
         if x.numel():
-            _rotary_launch(x.detach(), pos, sections, bases, code, inverse, out)
+            _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
         return out
     if x.requires_grad and torch.is_grad_enabled():
+        if x.numel() == 0:
+            return x.clone()
         return _Rotary.apply(x, pos, sections, bases, code, bool(inverse))
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel():
-        _rotary_launch(x, pos, sections, bases, code, inverse, out)
+        _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
     return out
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------------------------
-def _fits(t: torch.Tensor, most_token_bytes: int) -> torch.Tensor:
-    """t itself when the kernels can take it as it lies, else a contiguous copy."""
+def _lies_well(t: torch.Tensor, most_token_bytes: int) -> bool:
+    """Whether the kernels can take t as it lies, its address aside."""
     bs, ts, hs = _strides(t)
     es = t.element_size()
-    if (t.stride(3) != 1 or t.data_ptr() % 16 or (bs * es) % 16 or (ts * es) % 16 or (hs * es) % 16 or ts * es >= most_token_bytes
-            or (33 * ts + t.shape[2] * hs) * es >= 1 << 31):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    return t.stride(3) == 1 and not ((bs | ts | hs) * es) % 16 and ts * es < most_token_bytes and (33 * ts + t.shape[2] * hs) * es < 1 << 31
 
 
-def _desc(q, k, v, out, lse, left, right, sinks, scale, q_lens, k_lens) -> WindowAttnDesc:
+def _fits(t: torch.Tensor, most_token_bytes: int) -> torch.Tensor:
+    """t itself when the kernels can take it as it lies, else a contiguous copy."""
+    return t if t.data_ptr() % 16 == 0 and _lies_well(t, most_token_bytes) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _desc(q, k, v, out, left, right, sinks, scale) -> WindowAttnDesc:
     d = WindowAttnDesc()
-    d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    d.lse = None if lse is None else lse.data_ptr()
     d.q_bs, d.q_ts, d.q_hs = _strides(q)
     d.k_bs, d.k_ts, d.k_hs = _strides(k)
     d.v_bs, d.v_ts, d.v_hs = _strides(v)
@@ -181,24 +211,47 @@ def _desc(q, k, v, out, lse, left, right, sinks, scale, q_lens, k_lens) -> Windo
     d.B, d.Tq, d.Hq, d.D = q.shape
     d.Tk, d.Hkv = k.shape[1], k.shape[2]
     d.dtype, d.left, d.right, d.sinks, d.scale = _CODES[q.dtype], left, right, sinks, scale
-    d.q_lens, d.k_lens = _lib.ptr(q_lens), _lib.ptr(k_lens)
     return d
 
 
+class _Form:
+    """What a call's shapes, strides, types and limits come to: the filled descriptors and the bytes of scratch memory."""
+    __slots__ = ("desc", "ws", "lse_shape", "bwd", "bwd_key", "bwd_ws")
+
+
+def _form(q, k, v, left, right, sinks, scale, q_lens, k_lens) -> _Form:
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), v.stride(), left, right, sinks, scale)
+    known = _known("attention")
+    f = known.get(key)
+    if f is None:
+        f = _Form()
+        out = torch.empty(q.shape, dtype=q.dtype, device="meta")
+        f.desc = _desc(q, k, v, out, left, right, sinks, scale)
+        f.lse_shape = (q.shape[0], q.shape[2], q.shape[1])
+        f.bwd = f.bwd_key = None
+        d = f.desc
+        d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), q.data_ptr()   # (checked for alignment; set again by every call)
+        with torch.cuda.device(q.device):
+            f.ws = _lib.lib().tdx_window_attention_ws_bytes(C.byref(d))
+        known[key] = f
+    return f
+
+
 def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse):
-    B, Tq, Hq, D = q.shape
-    out = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=q.device) if want_lse else None
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     if out.numel() == 0:
-        return out, lse
-    d = _desc(q, k, v, out, lse, left, right, sinks, scale, q_lens, k_lens)
-    lib = _lib.lib()
-    with _On(q):
-        n = lib.tdx_window_attention_ws_bytes(C.byref(d))
-        if n:
-            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-            d.ws, d.ws_bytes = ws.data_ptr(), n
-        _lib.check(lib.tdx_window_attention(C.byref(d), _stream(q)), "tdx_window_attention")
+        return out, torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if want_lse else None
+    f = _form(q, k, v, left, right, sinks, scale, q_lens, k_lens)
+    lse = torch.empty(f.lse_shape, dtype=torch.float32, device=dev) if want_lse else None
+    d = f.desc
+    d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    d.lse = None if lse is None else lse.data_ptr()
+    d.q_lens, d.k_lens = None if q_lens is None else q_lens.data_ptr(), None if k_lens is None else k_lens.data_ptr()
+    if f.ws:
+        ws = torch.empty(f.ws, dtype=torch.uint8, device=dev)
+        d.ws, d.ws_bytes = ws.data_ptr(), f.ws
+    _launch(_lib.lib().tdx_window_attention, "tdx_window_attention", d, q.get_device())
     return out, lse
 
 
@@ -209,30 +262,42 @@ class _WindowAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse, q_lens, k_lens)
         ctx.args = (left, right, sinks, scale)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
+        if torch.is_grad_enabled():
+            raise TdxError("window_attention: second derivatives are not provided")
+        none = (None,) * 6
+        if dout is None:
+            return (None, None, None) + none
         q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
-        left, right, sinks, scale = ctx.args
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        if dq.numel() == 0 or k.shape[1] == 0:
-            return dq.zero_(), dk.zero_(), dv.zero_(), None, None, None, None, None, None
+        dev = q.device
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        if dq.numel() == 0 or dk.numel() == 0:
+            return (dq.zero_(), dk.zero_(), dv.zero_()) + none
         dout = _fits(dout, 1 << 31)
-        d = _desc(q, k, v, out, lse, left, right, sinks, scale, q_lens, k_lens)
-        d.dout, d.dq, d.dk, d.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        d.dout_bs, d.dout_ts, d.dout_hs = _strides(dout)
-        d.dq_bs, d.dq_ts, d.dq_hs = _strides(dq)
-        d.dk_bs, d.dk_ts, d.dk_hs = _strides(dk)
-        d.dv_bs, d.dv_ts, d.dv_hs = _strides(dv)
+        f = _form(q, k, v, *ctx.args, q_lens, k_lens)
         lib = _lib.lib()
-        with _On(q):
-            n = lib.tdx_window_attention_bwd_ws_bytes(C.byref(d))
-            ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
-            d.ws, d.ws_bytes = ws.data_ptr(), n
-            _lib.check(lib.tdx_window_attention_bwd(C.byref(d), _stream(q)), "tdx_window_attention_bwd")
-        return dq, dk, dv, None, None, None, None, None, None
+        key = dout.stride()
+        if f.bwd_key != key:
+            d = f.bwd = _desc(q, k, v, out, *ctx.args)
+            d.dout_bs, d.dout_ts, d.dout_hs = _strides(dout)
+            d.dq_bs, d.dq_ts, d.dq_hs = _strides(dq)
+            d.dk_bs, d.dk_ts, d.dk_hs = _strides(dk)
+            d.dv_bs, d.dv_ts, d.dv_hs = _strides(dv)
+            d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+            with torch.cuda.device(dev):
+                f.bwd_ws = lib.tdx_window_attention_bwd_ws_bytes(C.byref(d))
+            f.bwd_key = key
+        d = f.bwd
+        ws = torch.empty(f.bwd_ws, dtype=torch.uint8, device=dev)
+        d.q, d.k, d.v, d.out, d.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
+        d.q_lens, d.k_lens = None if q_lens is None else q_lens.data_ptr(), None if k_lens is None else k_lens.data_ptr()
+        d.dout, d.dq, d.dk, d.dv, d.ws, d.ws_bytes = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), f.bwd_ws
+        _launch(lib.tdx_window_attention_bwd, "tdx_window_attention_bwd", d, q.get_device())
+        return (dq, dk, dv) + none
 
 
 def _limit(n: Optional[int], name: str) -> int:
@@ -253,6 +318,28 @@ def _lengths(t: Optional[torch.Tensor], name: str, q: torch.Tensor) -> Optional[
     return t.contiguous()
 
 
+def _attention_args(q, k, v, left, right, sinks, scale) -> Tuple:
+    """(left, right, sinks, scale, whether the tensors can be taken as they lie) of a call whose arguments go together; raises otherwise."""
+    fn = "window_attention"
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        _check4(t, n, fn)
+    B, Tq, Hq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise TdxError(f"{fn}: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype} do not go together")
+    if Hq < 1 or k.shape[2] < 1 or Hq % k.shape[2]:
+        raise TdxError(f"{fn}: {Hq} query heads over {k.shape[2]} key heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise TdxError(f"{fn}: heads of {D} channels (a multiple of 8, at most 128)")
+    left, right = _limit(left, "left"), _limit(right, "right")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise TdxError(f"{fn}: sinks={sinks!r} (a number of tokens >= 0)")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise TdxError(f"{fn}: scale={scale} (finite, > 0)")
+    as_it_lies = _lies_well(q, 1 << 31) and _lies_well(k, 1 << 24) and _lies_well(v, 1 << 24)
+    return left, right, min(sinks, _MAX), scale, as_it_lies
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Optional[int] = None, right: Optional[int] = None, sinks: int = 0,
                      q_lens: Optional[torch.Tensor] = None, k_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                      return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
@@ -267,25 +354,23 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     those behind q_len, get zeros (lse -inf) and pass no gradient; gradients of keys behind k_len are zero.  Whatever stands at keys a
     query does not see, NaN and infinities too, does not reach it.  Strided tensors are taken as they lie when their channels are
     contiguous and their strides multiples of 16 bytes, else copied.  Differentiable in q, k, v; results are reproducible."""
-    fn = "window_attention"
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        _check4(t, n, fn)
-    B, Tq, Hq, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
-        raise TdxError(f"{fn}: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype} do not go together")
-    if Hq < 1 or k.shape[2] < 1 or Hq % k.shape[2]:
-        raise TdxError(f"{fn}: {Hq} query heads over {k.shape[2]} key heads")
-    if D % 8 or not 8 <= D <= 128:
-        raise TdxError(f"{fn}: heads of {D} channels (a multiple of 8, at most 128)")
-    left, right = _limit(left, "left"), _limit(right, "right")
-    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
-        raise TdxError(f"{fn}: sinks={sinks!r} (a number of tokens >= 0)")
-    sinks = min(sinks, _MAX)
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise TdxError(f"{fn}: scale={scale} (finite, > 0)")
-    q_lens, k_lens = _lengths(q_lens, "q_lens", q), _lengths(k_lens, "k_lens", q)
-    q, k, v = _fits(q, 1 << 31), _fits(k, 1 << 24), _fits(v, 1 << 24)
+    try:   # a form of call that was checked before?
+        key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, left, right, sinks, scale,
+               left.__class__, right.__class__, sinks.__class__)
+        args = _known("attention_args").get(key)
+    except (AttributeError, TypeError, RuntimeError):
+        key = args = None
+    if args is None:
+        args = _attention_args(q, k, v, left, right, sinks, scale)
+        if key is not None:
+            _known("attention_args")[key] = args
+    left, right, sinks, scale, as_it_lies = args
+    if q_lens is not None:
+        q_lens = _lengths(q_lens, "q_lens", q)
+    if k_lens is not None:
+        k_lens = _lengths(k_lens, "k_lens", q)
+    if not as_it_lies or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _fits(q, 1 << 31), _fits(k, 1 << 24), _fits(v, 1 << 24)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _WindowAttention.apply(q, k, v, left, right, sinks, scale, q_lens, k_lens)
     else:

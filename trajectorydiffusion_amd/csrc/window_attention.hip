@@ -97,6 +97,48 @@ __device__ __forceinline__ void dma16(uint32_t lds_addr, uint32_t voff, const u3
       : "s"(lds_addr), "v"(voff), "s"(srd)
       : "memory");
 }
+// The same N times, 4096 bytes of LDS apart
+template <int N>
+__device__ __forceinline__ void dma16n(uint32_t lds_addr, const uint32_t (&voff)[N], const u32x4& srd) {
+  uint32_t keep;
+  lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
+  if constexpr (N == 4) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %2, %6, 0 offen lds\n\t"
+        "s_add_u32 m0, m0, 4096\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %3, %6, 0 offen lds\n\t"
+        "s_add_u32 m0, m0, 4096\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %4, %6, 0 offen lds\n\t"
+        "s_add_u32 m0, m0, 4096\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %5, %6, 0 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "s"(lds_addr), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(srd)
+        : "memory", "scc");
+  } else if constexpr (N == 2) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+        "s_add_u32 m0, m0, 4096\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %3, %4, 0 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "s"(lds_addr), "v"(voff[0]), "v"(voff[1]), "s"(srd)
+        : "memory", "scc");
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; ++n) dma16(lds_addr + 4096 * n, voff[n], srd);
+  }
+}
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // every wave's LDS traffic is complete, then the barrier (without a release fence, which would wait for the direct loads in flight)
@@ -236,17 +278,40 @@ __device__ __forceinline__ void mma_planes(f32x16& acc, const bf16x8 (&a)[N], co
   }
   acc = mfma16(a[0], b[0], acc);
 }
-// acc (32 tile rows x 32 columns) = the 32 tile rows at IMM times the fragments b; planes of a tile are PLANE bytes apart
-template <int N, int DP, uint32_t IMM, uint32_t PLANE>
-__device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, const Frags16<N, DP>& b) {
+// Reads run AHEAD steps in front of the matrix instructions that take them, and vector work that is ready stands between these: the order
+// is pinned, since left alone the compiler reads one fragment, waits for it and multiplies, and every step pays the read's latency.
+// (The six products of a step of fp32 planes cover it by themselves.)
+template <int N>
+__device__ __forceinline__ void pin() {
+  if constexpr (N == 1) __builtin_amdgcn_sched_barrier(0);
+}
+struct Nothing {
+  __device__ __forceinline__ void operator()(int) const {}
+};
+// acc (32 tile rows x 32 columns) = the 32 tile rows at IMM times the fragments b; planes of a tile are PLANE bytes apart.
+// between(c) is called behind the instructions of step c < NC.
+template <int N, int DP, uint32_t IMM, uint32_t PLANE, typename F = Nothing>
+__device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, const Frags16<N, DP>& b, F&& between = F()) {
+  constexpr int NC = G16<DP>::NC, AHEAD = N == 3 ? 1 : NC < 4 ? NC : 4, RING = AHEAD + 1;
+  bf16x8 a[RING][N];
+  auto read = [&](int c) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) a[c % RING][n] = __builtin_bit_cast(bf16x8, lds_ld16(off.row[c] + IMM + n * PLANE));
+  };
+#pragma unroll
+  for (int c = 0; c < AHEAD; ++c) read(c);
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
 #pragma unroll
-  for (int c = 0; c < G16<DP>::NC; ++c) {
-    bf16x8 a[N], bc[N];
+  for (int c = 0; c < NC; ++c) {
+    if (c + AHEAD < NC) read(c + AHEAD);
+    pin<N>();
+    bf16x8 bc[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) a[n] = __builtin_bit_cast(bf16x8, lds_ld16(off.row[c] + IMM + n * PLANE)), bc[n] = b[n][c];
-    mma_planes<N>(acc, a, bc);
+    for (int n = 0; n < N; ++n) bc[n] = b[n][c];
+    mma_planes<N>(acc, a[c % RING], bc);
+    between(c);
+    pin<N>();
   }
 }
 // x as N bf16 planes; an infinity (or what rounds to one) is the first plane alone
@@ -267,30 +332,43 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[N]) {
     p[2] = __builtin_bit_cast(bf16x8, Elem<__bf16>::pack(r));
   }
 }
-// acc[dt] (channels 32 dt .. + 31 x 32 columns) += (the 32 tile rows at IMM)^T p, p as rows16 left it: element i of a lane is tile row
-// 8 (i / 4) + 4 h + i % 4
-template <int N, int DP, uint32_t IMM, uint32_t PLANE>
-__device__ __forceinline__ void cols16(f32x16 (&acc)[DP / 32], const LaneOff<DP>& off, const float (&p)[16]) {
-  using G = G16<DP>;
+// the right operand of cols16: 32 rows' numbers as rows16 left them (element i of a lane is tile row 8 (i / 4) + 4 h + i % 4)
+template <int N>
+__device__ __forceinline__ void pack16(bf16x8 (&b)[2][N], const float (&p)[16]) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     float pe[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) pe[j] = p[8 * s + j];
-    bf16x8 b[N];
-    split8<N>(pe, b);
+    split8<N>(pe, b[s]);
+  }
+}
+// acc[dt] (channels 32 dt .. + 31 x 32 columns) += (the 32 tile rows at IMM)^T b.  between(k) is called behind the instructions of step
+// k < 2 ND.
+template <int N, int DP, uint32_t IMM, uint32_t PLANE, typename F = Nothing>
+__device__ __forceinline__ void cols16(f32x16 (&acc)[DP / 32], const LaneOff<DP>& off, const bf16x8 (&b)[2][N], F&& between = F()) {
+  using G = G16<DP>;
+  constexpr int STEPS = 2 * G::ND, AHEAD = N == 3 ? 1 : STEPS < 3 ? STEPS : 3, RING = AHEAD + 1;
+  bf16x8 a[RING][N];
+  auto read = [&](int k) {
+    const int s = k / G::ND, dt = k % G::ND;
 #pragma unroll
-    for (int dt = 0; dt < G::ND; ++dt) {
-      bf16x8 a[N];
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const uint32_t at = IMM + n * PLANE + 16 * s * G::PITCH;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(off.lo[dt] + at));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(off.hi[dt] + at));
-        a[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
-      mma_planes<N>(acc[dt], a, b);
+    for (int n = 0; n < N; ++n) {
+      const uint32_t at = IMM + n * PLANE + 16 * s * G::PITCH;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(off.lo[dt] + at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(off.hi[dt] + at));
+      a[k % RING][n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) read(k);
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    if (k + AHEAD < STEPS) read(k + AHEAD);
+    pin<N>();
+    mma_planes<N>(acc[k % G::ND], a[k % RING], b[k / G::ND]);
+    between(k);
+    pin<N>();
   }
 }
 // a 32-row operand in registers: channels 16 c + 8 h .. + 7 of row `row`, zero beyond the channels or when !ok
@@ -349,15 +427,15 @@ struct Stager<__bf16, DP, ROWS> {
     }
   }
   __device__ __forceinline__ void load(uint32_t lds, const char* base, int valid, int wave) const {
+    static_assert(TOTAL % 4 == 0, "whole loads for each of the 4 waves");
     const u32x4 srd = make_srd(base);
+    if (valid >= ROWS) {
+      dma16n<PER>(lds + wave * 1024, voff, srd);
+    } else {
+      uint32_t v[PER];
 #pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      const int it = wave + 4 * n;
-      if (TOTAL % 4 == 0 || it < TOTAL) {
-        uint32_t v = voff[n];
-        if (valid < ROWS) v = row0 + 4 * n * (1024 / G::PITCH) < valid ? v : kOutside;
-        dma16(lds + it * 1024, v, srd);
-      }
+      for (int n = 0; n < PER; ++n) v[n] = row0 + 4 * n * (1024 / G::PITCH) < valid ? voff[n] : kOutside;
+      dma16n<PER>(lds + wave * 1024, v, srd);
     }
   }
   __device__ __forceinline__ void put(uint32_t, int) const {}
@@ -427,24 +505,21 @@ __device__ __forceinline__ Tiles tiles_of(const WaArgs& a, const Seq& s, int p0,
 }
 __device__ __forceinline__ int tile_start(const Tiles& t, int i, int bn) { return i < t.na ? i * bn : t.start + (i - t.na) * bn; }
 
-// What 32 keys from j0 are to rows at positions [p0, p1]: 0 unseen, 1 seen in part, 2 seen by all
+// What the KEYS keys from j0 are to rows at positions [p0, p1]: 0 unseen, 1 seen in part, 2 seen by all
+template <int KEYS = 32>
 __device__ __forceinline__ int seen_class(const WaArgs& a, const Seq& s, int j0, int p0, int p1) {
-  if (j0 >= s.kl || j0 > p1 + a.right || (j0 + 31 < p0 - a.left && j0 >= a.sinks)) return 0;
-  return j0 + 31 < s.kl && j0 + 31 <= p0 + a.right && (j0 >= p1 - a.left || j0 + 31 < a.sinks) ? 2 : 1;
+  const int j1 = j0 + KEYS - 1;
+  if (j0 >= s.kl || j0 > p1 + a.right || (j1 < p0 - a.left && j0 >= a.sinks)) return 0;
+  return j1 < s.kl && j1 <= p0 + a.right && (j0 >= p1 - a.left || j1 < a.sinks) ? 2 : 1;
 }
 
 // ---- online softmax ----------------------------------------------------------------------------------------------------------------
 // m is the running maximum of the raw scores that the exponents are taken against.  It follows the true maximum only when that is more
 // than 8 powers of two above it: the terms stay below 2^8, nothing is lost in fp32 (nor in bf16, whose exponent is as wide), and the
 // accumulators are rescaled in the first tiles of a row only.
-template <int ND, int NS>
-__device__ __forceinline__ void softmax_step(float (&s)[NS][16], float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
-  float t = s[0][0];
-#pragma unroll
-  for (int n = 0; n < NS; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t = fmaxf(t, s[n][i]);
-  t = half_max(t);
+// Takes the maximum t of new scores into m (rescaling l and o); returns m c, what the exponents are taken against
+template <int ND>
+__device__ __forceinline__ float softmax_follow(float t, float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
   if (__ballot(t > m + slack)) {
     const float mn = fmaxf(m, t);
     const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
@@ -455,19 +530,29 @@ __device__ __forceinline__ void softmax_step(float (&s)[NS][16], float& m, float
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] *= f;
   }
-  const float off = m == -INFINITY ? 0.f : m * c;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  return m == -INFINITY ? 0.f : m * c;
+}
+template <int ND>
+__device__ __forceinline__ float softmax_max(const float (&s)[16], float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
+  float t = s[0];
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+  for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
+  return softmax_follow<ND>(half_max(t), m, l, o, c, slack);
+}
+// elements [A, B) of the scores become exponentials
+template <int A, int B>
+__device__ __forceinline__ void softmax_exp(float (&s)[16], float& l, float off, float c) {
+  float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -off));
-      sum[i & 3] += s[n][i];
-    }
-  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  for (int i = A; i < B; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -off));
+    sum += s[i];
+  }
+  l += sum;
 }
 // scores of keys a row does not see become -inf (element i: key j0 + 8 (i / 4) + 4 h + i % 4)
 __device__ __forceinline__ void mask_scores(float (&s)[16], const WaArgs& a, const Seq& q, int j0, int p, int lane) {
+  asm volatile("");   // (a branch, not a select over all tiles)
   const int base = j0 + 4 * (lane >> 5);
   const int hi = min(p + a.right, q.kl - 1) - base, lo = p - a.left - base, sk = a.sinks - base;
 #pragma unroll
@@ -547,8 +632,10 @@ struct Walk {
   static constexpr uint32_t PLANE = BN * G16<DP>::PITCH, TILE = N * PLANE, STAGE = 2 * TILE, LDS = NSTAGE * STAGE;
 };
 // Calls f(key, offset of the stage in LDS as a type) for each key tile of `t`, staged
-template <typename T, int DP, typename F>
-__device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const Tiles& t, const T* kb, const T* vb, uint32_t lds, int wave, int lane, F&& f) {
+// (ready() is called once the first tile's loads are on their way)
+template <typename T, int DP, typename R, typename F>
+__device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const Tiles& t, const T* kb, const T* vb, uint32_t lds, int wave, int lane, R&& ready,
+                                          F&& f) {
   using W = Walk<T, DP>;
   constexpr int ES = sizeof(T);
   Stager<T, DP, W::BN> sk, sv;
@@ -561,6 +648,7 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
     sv.load(at + W::TILE, (const char*)(vb + (long)j0 * a.v_ts), s.kl - j0, wave);
   };
   if (n > 0) load(0, lds);
+  ready();
   if constexpr (W::N == 1) {
     for (int it = 0; it < n; it += 2) {
       wait_vm<0>();
@@ -587,7 +675,7 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
 
 // ---- forward, many rows: 4 waves x 32 rows ----------------------------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void window_attn_kernel(const WaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 || DP == 128 ? 2 : 4))) void window_attn_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using W = Walk<T, DP>;
   constexpr int ND = DP / 32, N = W::N;
@@ -611,46 +699,62 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(const WaArgs a) {
   if (r0 < rend) {
     Frags16<N, DP> qf;
     load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
-    arrived16(qf);
     const LaneOff<DP> off(lds, lane);
     const int p = i + s.shift;
     const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;   // positions of this wave's rows
     const bool wave_ok = rw < rend;
     const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, W::BN);
-    // scores of the 32 keys at row SUB of the staged tile
-    auto scores = [&](float (&sc)[16], int j0, int cls, auto at) {
-      f32x16 acc;
-      rows16<N, DP, decltype(at)::value, W::PLANE>(acc, off, qf);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = acc[e];
-      if (cls == 1) mask_scores(sc, a, s, j0, p, lane);
-    };
-    auto one = [&](int j0, int cls, auto at) {
-      float sc[1][16];
-      scores(sc[0], j0, cls, at);
-      softmax_step<ND, 1>(sc, m, l, o, c, slack);
-      cols16<N, DP, decltype(at)::value + W::TILE, W::PLANE>(o, off, sc[0]);
-    };
-    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&](int j0, auto st) {
+    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&] { arrived16(qf); },
+                     [&](int j0, auto st) {
+      // a tile is taken whole: with a path of its own for a half the accumulators would be copied where the paths meet
       constexpr uint32_t S0 = decltype(st)::value;
-      const int c0 = wave_ok ? seen_class(a, s, j0, wp0, wp1) : 0;
-      if constexpr (W::BN == 64) {
+      constexpr int NS = W::BN / 32, STEPS = 2 * ND;
+      const int cls = wave_ok ? seen_class<W::BN>(a, s, j0, wp0, wp1) : 0;
+      if (!cls) return;
+      float sc[NS][16];
+      bf16x8 pb[2][N];
+      if constexpr (NS == 2) {
+        // (Taking the first half's exponentials against the maximum so far, between the second half's products, measured no faster at 128
+        // channels and costs the fourth wave at 64.)
         constexpr uint32_t S1 = S0 + 32 * G16<DP>::PITCH;
-        const int c1 = wave_ok ? seen_class(a, s, j0 + 32, wp0, wp1) : 0;
-        if (c0 && c1) {
-          float sc[2][16];
-          scores(sc[0], j0, c0, std::integral_constant<uint32_t, S0>());
-          scores(sc[1], j0 + 32, c1, std::integral_constant<uint32_t, S1>());
-          softmax_step<ND, 2>(sc, m, l, o, c, slack);
-          cols16<N, DP, S0 + W::TILE, W::PLANE>(o, off, sc[0]);
-          cols16<N, DP, S1 + W::TILE, W::PLANE>(o, off, sc[1]);
-        } else if (c0) {
-          one(j0, c0, std::integral_constant<uint32_t, S0>());
-        } else if (c1) {
-          one(j0 + 32, c1, std::integral_constant<uint32_t, S1>());
+        f32x16 acc;
+        rows16<N, DP, S0, W::PLANE>(acc, off, qf);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
+        rows16<N, DP, S1, W::PLANE>(acc, off, qf);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[1][e] = acc[e];
+        if (cls == 1) {
+          mask_scores(sc[0], a, s, j0, p, lane);
+          mask_scores(sc[1], a, s, j0 + 32, p, lane);
         }
+        float t = sc[0][0];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) t = fmaxf(t, sc[n][e]);
+        const float mc = softmax_follow<ND>(half_max(t), m, l, o, c, slack);
+        softmax_exp<0, 16>(sc[0], l, mc, c);
+        pack16<N>(pb, sc[0]);
+        // the exponentials of the second half stand between the products of the first with V
+        cols16<N, DP, S0 + W::TILE, W::PLANE>(o, off, pb, [&](int k) {
+#pragma unroll
+          for (int i = k * 16 / STEPS; i < (k + 1) * 16 / STEPS; ++i) {
+            sc[1][i] = __builtin_amdgcn_exp2f(fmaf(sc[1][i], c, -mc));
+            l += sc[1][i];
+          }
+        });
+        pack16<N>(pb, sc[1]);
+        cols16<N, DP, S1 + W::TILE, W::PLANE>(o, off, pb);
       } else {
-        if (c0) one(j0, c0, std::integral_constant<uint32_t, S0>());
+        f32x16 acc;
+        rows16<N, DP, S0, W::PLANE>(acc, off, qf);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
+        if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
+        softmax_exp<0, 16>(sc[0], l, softmax_max<ND>(sc[0], m, l, o, c, slack), c);
+        pack16<N>(pb, sc[0]);
+        cols16<N, DP, S0 + W::TILE, W::PLANE>(o, off, pb);
       }
     });
     l = half_sum(l);
@@ -753,12 +857,12 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       if (cls) {
         f32x16 acc;
         rows_times<T, DP>(acc, kt, 0, qf, lane);
-        float sc[1][16];
+        float sc[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
-        if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
-        softmax_step<G::ND, 1>(sc, m, l, o, c, slack);
-        cols_times<DP>(o, vt, 0, sc[0], lane, T());
+        for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+        if (cls == 1) mask_scores(sc, a, s, j0, p, lane);
+        softmax_exp<0, 16>(sc, l, softmax_max<G::ND>(sc, m, l, o, c, slack), c);
+        cols_times<DP>(o, vt, 0, sc, lane, T());
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage has been read before the ring comes round to it
     }
@@ -930,7 +1034,7 @@ __device__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, in
 }
 
 template <typename T, int DP, int OCC>
-__global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void window_attn_dq_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using W = Walk<T, DP>;
   constexpr int ND = DP / 32, N = W::N;
@@ -993,12 +1097,17 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a
       const int cls = wave_ok ? seen_class(a, s, j0, wp0, wp1) : 0;
       if (!cls) return;
       f32x16 acc, dp;
-      rows16<N, DP, A, W::PLANE>(acc, off, qf);
-      rows16<N, DP, A + W::TILE, W::PLANE>(dp, off, df);
       float sc[16];
+      constexpr int NC = G16<DP>::NC;
+      rows16<N, DP, A, W::PLANE>(acc, off, qf);
+      rows16<N, DP, A + W::TILE, W::PLANE>(dp, off, df, [&](int k) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -lse2)) * (dp[e] - delta);
+        for (int e = k * 16 / NC; e < (k + 1) * 16 / NC; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -lse2));
+      });
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] *= dp[e] - delta;
       if (cls == 1) {
+        asm volatile("");
         const int base = j0 + 4 * (lane >> 5);
         const int hi = min(p + a.right, s.kl - 1) - base, lo = p - a.left - base, sk = a.sinks - base;
 #pragma unroll
@@ -1007,9 +1116,11 @@ __global__ __launch_bounds__(256, OCC) void window_attn_dq_kernel(const WaArgs a
           if (!(x <= hi && (x >= lo || x < sk))) sc[e] = 0.f;
         }
       }
-      cols16<N, DP, A, W::PLANE>(dq, off, sc);
+      bf16x8 db[2][N];
+      pack16<N>(db, sc);
+      cols16<N, DP, A, W::PLANE>(dq, off, db);
     };
-    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&](int j0, auto st) {
+    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [] {}, [&](int j0, auto st) {
       constexpr uint32_t S0 = decltype(st)::value;
       one(j0, std::integral_constant<uint32_t, S0>());
       if constexpr (W::BN == 64) one(j0 + 32, std::integral_constant<uint32_t, S0 + 32 * G16<DP>::PITCH>());
@@ -1150,36 +1261,54 @@ __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP 
                                          const Frags16<Planes<T>::N, DP>& kf, const Frags16<Planes<T>::N, DP>& vf, float c, bool part, int r0, int rlo, int rhi,
                                          int lane) {
   using W = RowWalk<T, DP>;
+  constexpr int NC = G16<DP>::NC, STEPS = DP / 16;
   f32x16 acc, dp;
-  rows16<W::N, DP, A, W::PLANE>(acc, off, kf);
-  rows16<W::N, DP, A + W::TILE, W::PLANE>(dp, off, vf);
   float p[16], ds[16];
+  u32x4 l4[4], d4[4];
+  rows16<W::N, DP, A, W::PLANE>(acc, off, kf, [&](int k) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const u32x4 l4 = lds_ld16(stat + ST + 32 * e), d4 = lds_ld16(stat + ST + 128 + 32 * e);
+    for (int e = k * 4 / NC; e < (k + 1) * 4 / NC; ++e) l4[e] = lds_ld16(stat + ST + 32 * e);
+  });
+  // the exponentials stand between the products for dP, the score gradients between those for dV
+  rows16<W::N, DP, A + W::TILE, W::PLANE>(dp, off, vf, [&](int k) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      p[4 * e + x] = __builtin_amdgcn_exp2f(fmaf(acc[4 * e + x], c, -__uint_as_float(l4[x])));
-      ds[4 * e + x] = p[4 * e + x] * (dp[4 * e + x] - __uint_as_float(d4[x]));
-    }
-  }
+    for (int e = k * 16 / NC; e < (k + 1) * 16 / NC; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -__uint_as_float(l4[e >> 2][e & 3])));
+#pragma unroll
+    for (int e = k * 4 / NC; e < (k + 1) * 4 / NC; ++e) d4[e] = lds_ld16(stat + ST + 128 + 32 * e);
+  });
   if (part) {
+    asm volatile("");
     const int base = r0 + 4 * (lane >> 5);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int row = base + 8 * (e >> 2) + (e & 3);
-      if (row < rlo || row > rhi) p[e] = 0.f, ds[e] = 0.f;
+      if (row < rlo || row > rhi) p[e] = 0.f;
     }
   }
-  cols16<W::N, DP, A + W::TILE, W::PLANE>(dv, off, p);
-  cols16<W::N, DP, A, W::PLANE>(dk, off, ds);
+  bf16x8 pb[2][W::N], db[2][W::N];
+  pack16<W::N>(pb, p);
+  cols16<W::N, DP, A + W::TILE, W::PLANE>(dv, off, pb, [&](int k) {
+#pragma unroll
+    for (int e = k * 16 / STEPS; e < (k + 1) * 16 / STEPS; ++e) ds[e] = p[e] * (dp[e] - __uint_as_float(d4[e >> 2][e & 3]));
+  });
+  if (part) {   // (0 times an infinite dP)
+    asm volatile("");
+    const int base = r0 + 4 * (lane >> 5);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = base + 8 * (e >> 2) + (e & 3);
+      if (row < rlo || row > rhi) ds[e] = 0.f;
+    }
+  }
+  pack16<W::N>(db, ds);
+  cols16<W::N, DP, A, W::PLANE>(dk, off, db);
 }
 
 // dK / dV.  Workgroups from nsink on: 128 keys, 4 waves x 32 keys, the rows inside the keys' windows.  The first nsink workgroups: the rows
 // beyond the window of 32 KB keys that are sinks, a share of them each; the waves are KB key blocks x row blocks of a stage, and every wave
 // leaves its fp32 sums.  Sinks among the 128 keys leave theirs as share 0.
 template <typename T, int DP, int OCC>
-__global__ __launch_bounds__(256, OCC) void window_attn_dkv_kernel(const WaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void window_attn_dkv_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using W = RowWalk<T, DP>;
   constexpr int ND = DP / 32, N = W::N, NB = W::RS / 32, KB = 4 / NB;
@@ -1501,10 +1630,10 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
 template <typename T, int DP>
 int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
   const long bh = (long)a.B * a.Hkv;
-  constexpr int OCC = DP == 128 ? 1 : 2, KB = 4 / (RowWalk<T, DP>::RS / 32);
+  constexpr int OCC = DP == 128 ? 1 : 2, OCC_Q = sizeof(T) == 2 && DP == 64 ? 3 : sizeof(T) == 4 && DP == 128 ? 1 : 2, KB = 4 / (RowWalk<T, DP>::RS / 32);
   const long rt = ((long)a.Tq * a.G + 127) / 128;
   a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows;
-  WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
+  WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC_Q>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dq_kernel");
   if (a.Tk == 0) return TDX_OK;
   a.ntiles = (a.Tk + 127) / 128;
