@@ -180,8 +180,19 @@ __device__ __forceinline__ void rows_times(f32x16& acc, uint32_t tile, int row0,
   const int row = row0 + (lane & 31);
   const uint32_t a0 = tile + row * G::PITCH;
   const int c0 = (lane >> 5) ^ swz<T, DP>(row);
+  // reads run AHEAD pieces in front of the instructions that take them (see rows16)
+  constexpr int AHEAD = sizeof(T) == 4 ? 2 : G::NC < 4 ? G::NC : 4, RING = AHEAD + 1;
+  u32x4 p[RING];
+  auto read = [&](int c) { p[c % RING] = lds_ld16(a0 + ((c0 ^ (2 * c)) << 4)); };
 #pragma unroll
-  for (int c = 0; c < G::NC; ++c) mma_piece(acc, lds_ld16(a0 + ((c0 ^ (2 * c)) << 4)), b[c], T());
+  for (int c = 0; c < AHEAD; ++c) read(c);
+#pragma unroll
+  for (int c = 0; c < G::NC; ++c) {
+    if (c + AHEAD < G::NC) read(c + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+    mma_piece(acc, p[c % RING], b[c], T());
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 // acc[dt] (channels 32 dt .. + 31 x 32 columns) += (tile rows [row0, row0 + 32))^T p, p as rows_times left it: element i of a lane is tile
 // row row0 + 8 (i / 4) + 4 h + i % 4
@@ -211,15 +222,21 @@ __device__ __forceinline__ void cols_times(f32x16 (&acc)[DP / 32], uint32_t tile
 template <int DP>
 __device__ __forceinline__ void cols_times(f32x16 (&acc)[DP / 32], uint32_t tile, int row0, const float (&p)[16], int lane, float) {
   using G = Geo<float, DP>;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {                                    // two tile rows a step: one for each lane half
+  constexpr int STEPS = 16 * G::ND, AHEAD = 6, RING = AHEAD + 1;     // two tile rows a step, one for each lane half
+  float r[RING];
+  auto read = [&](int k) {
+    const int i = k / G::ND, d = 32 * (k % G::ND) + (lane & 31);
     const int row = row0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+    r[k % RING] = lds_ld4(tile + row * G::PITCH + (((d >> 2) ^ swz<float, DP>(row)) << 4) + 4 * (d & 3));
+  };
 #pragma unroll
-    for (int dt = 0; dt < G::ND; ++dt) {
-      const int d = 32 * dt + (lane & 31);
-      const float a = lds_ld4(tile + row * G::PITCH + (((d >> 2) ^ swz<float, DP>(row)) << 4) + 4 * (d & 3));
-      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[dt], 0, 0, 0);
-    }
+  for (int k = 0; k < AHEAD; ++k) read(k);
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    if (k + AHEAD < STEPS) read(k + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+    acc[k % G::ND] = __builtin_amdgcn_mfma_f32_32x32x2f32(r[k % RING], p[k / G::ND], acc[k % G::ND], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -675,7 +692,7 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
 
 // ---- forward, many rows: 4 waves x 32 rows ----------------------------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 || DP == 128 ? 2 : 4))) void window_attn_kernel(const WaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ? 2 : sizeof(T) == 4 ? (DP == 64 ? 3 : 4) : 4))) void window_attn_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using W = Walk<T, DP>;
   constexpr int ND = DP / 32, N = W::N;
@@ -791,22 +808,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 
 // ---- forward, few rows: one 32-row tile per workgroup, its waves (and the splits) share the keys -------------------------------------
 // Single tokens over a cache are bound by the reads of K and V: every wave streams its own key tiles through a ring of two stages in LDS, so
-// a compute unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.
-template <typename T, int DP>
+// a compute unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.  Where a row tile sees two key
+// tiles at most (short tracks) a workgroup is one wave and keeps its result in registers: more workgroups fit a compute unit, and there is
+// nothing to join.
+template <typename T, int DP, bool ONE>
 struct Few {
   using G = Geo<T, DP>;
   static constexpr int STAGE = 2 * 32 * G::PITCH;                               // 32 keys of K and of V
-  static constexpr int NW = G::PITCH > 256 ? 2 : 4;
+  static constexpr int NW = ONE ? 1 : G::PITCH > 256 ? 2 : 4;
   static constexpr int RING = 2 * STAGE;
   static constexpr int OPITCH = DP + 4;                                          // floats of a row in the exchange
-  static constexpr int XCHG = NW * 32 * (OPITCH + 2) * 4;
+  static constexpr int XCHG = ONE ? 0 : NW * 32 * (OPITCH + 2) * 4;
   static constexpr int LDS = NW * RING > XCHG ? NW * RING : XCHG;
 };
-template <typename T, int DP>
+template <typename T, int DP, bool ONE>
 __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = Geo<T, DP>;
-  using F = Few<T, DP>;
+  using F = Few<T, DP, ONE>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -841,8 +860,8 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       stage_rows<T, DP, 32, 1>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, 0, lane);
       stage_rows<T, DP, 32, 1>(dst + F::STAGE / 2, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, 0, lane);
     };
-    arrived(qf);               // from here on only direct loads are counted
     if (first < last) stage(first, 0);
+    arrived(qf);               // from here on only direct loads are counted
     int buf = 0;
     for (int it = first; it < last; it += F::NW, buf ^= 1) {
       if (it + F::NW < last) {
@@ -867,6 +886,35 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage has been read before the ring comes round to it
     }
     l = half_sum(l);
+  }
+  if constexpr (ONE) {
+    const float inv = row_ok && l != 0.f ? 1.0f / l : 0.f;
+    bool bad = false;
+    if (r < R) {
+      T* orow = (T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
+      const int h4 = 4 * (lane >> 5);
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
+            bad |= v[x] != v[x];
+          }
+          if (32 * d + 8 * e + h4 < a.D) store4<T>(orow + 32 * d + 8 * e + h4, v);
+        }
+      if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l) : -INFINITY;
+    }
+    uint64_t again = __ballot(bad && row_ok && l == l);
+    again = (again | (again >> 32)) & 0xffffffffull;
+    while (again) {
+      const int n = __builtin_ctzll(again);
+      again &= again - 1;
+      row_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(m, n, 64), __shfl(l, n, 64), lane);
+    }
+    return;
   }
   // the waves' shares are joined in LDS, in wave order
   __syncthreads();
@@ -948,20 +996,31 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
   const int grp = threadIdx.x / D4, dv = threadIdx.x % D4;
   const Seq s = seq_of(a, b);
   const float c = a.scale * kLog2e;
-  const float* base = a.ws + ((long)(bh * a.ntiles + tile) * a.nsplit) * 32 * (DP + 2);
+  constexpr long PART = 32 * (DP + 2);
+  const float* base = a.ws + ((long)(bh * a.ntiles + tile) * a.nsplit) * PART;
+  // every load of the row is on its way before the first is used: at most 64 splits, 64 / NG of them to a group
+  constexpr int PER = 64 / NG;
+  f32x4 ow[PER];
+  float mw[PER], lw[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int sp = grp + k * NG;
+    const float* part = base + min(sp, a.nsplit - 1) * PART;
+    mw[k] = part[32 * DP + n];
+    lw[k] = sp < a.nsplit ? part[32 * DP + 32 + n] : 0.f;
+    ow[k] = *reinterpret_cast<const f32x4*>(part + n * DP + 4 * dv);
+  }
   float mm = -INFINITY, ll = 0.f;
   f32x4 oo = {0.f, 0.f, 0.f, 0.f};
-  for (int sp = grp; sp < a.nsplit; sp += NG) {
-    const float* part = base + (long)sp * 32 * (DP + 2);
-    const float mw = part[32 * DP + n], lw = part[32 * DP + 32 + n];
-    const f32x4 ow = *reinterpret_cast<const f32x4*>(part + n * DP + 4 * dv);
-    if (lw == 0.f) continue;
-    const float mn = fmaxf(mm, mw);
-    const float f0 = mm == mn ? 1.f : __builtin_amdgcn_exp2f((mm - mn) * c), f1 = mw == mn ? 1.f : __builtin_amdgcn_exp2f((mw - mn) * c);
-    mm = mn;
-    ll = ll * f0 + lw * f1;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) oo[x] = oo[x] * f0 + ow[x] * f1;
+  for (int k = 0; k < PER; ++k) mm = lw[k] == 0.f ? mm : fmaxf(mm, mw[k]);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (lw[k] == 0.f) continue;                                                  // a share that saw nothing
+    const float f = mw[k] == mm ? 1.f : __builtin_amdgcn_exp2f((mw[k] - mm) * c);
+    ll = fmaf(f, lw[k], ll);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) oo[x] = fmaf(f, ow[k][x], oo[x]);
   }
   xo[grp][dv] = oo;
   if (dv == 0) xm[grp] = mm, xl[grp] = ll;
@@ -1543,11 +1602,12 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
 
 // Which forward kernel: the few-row kernel while the many-row kernel (128 rows a workgroup) would leave compute units idle
 struct Plan {
-  bool few;
+  bool few, one;
   int ntiles, nsplit;
 };
+constexpr int kMostSplits = 64;       // (the join kernel holds a row's shares in registers)
 Plan plan_forward(const WaArgs& a) {
-  Plan p;
+  Plan p{};
   const long rows = (long)a.Tq * a.G, bh = (long)a.B * a.Hkv;
   p.few = rows <= 32 || bh * ((rows + 127) / 128) < compute_units();
   p.ntiles = (int)((rows + (p.few ? 31 : 127)) / (p.few ? 32 : 128));
@@ -1557,7 +1617,8 @@ Plan plan_forward(const WaArgs& a) {
     const long span = a.left == kFar ? a.Tk : std::min<long>(a.Tk, (long)a.left + 32 / a.G + 1 + (a.right == kFar ? a.Tk : a.right) + a.sinks);
     const long tiles = (span + 31) / 32, wgs = bh * p.ntiles;
     const long want = (2 * (long)compute_units() + wgs - 1) / wgs;
-    p.nsplit = (int)std::max<long>(1, std::min<long>(std::min<long>(want, tiles / 8), 64));
+    p.nsplit = (int)std::max<long>(1, std::min<long>(std::min<long>(want, tiles / 8), kMostSplits));
+    p.one = tiles <= 2;
   }
   return p;
 }
@@ -1585,7 +1646,8 @@ int launch_forward(WaArgs& a, const Plan& p, hipStream_t st) {
   const long bh = (long)a.B * a.Hkv;
   a.ntiles = p.ntiles, a.nsplit = p.nsplit;
   if (p.few) {
-    WA_LAUNCH((window_attn_few_kernel<T, DP>), bh * p.ntiles * p.nsplit, (Few<T, DP>::NW * 64), (Few<T, DP>::LDS), st, a);
+    if (p.one) WA_LAUNCH((window_attn_few_kernel<T, DP, true>), bh * p.ntiles, 64, (Few<T, DP, true>::LDS), st, a);
+    else WA_LAUNCH((window_attn_few_kernel<T, DP, false>), bh * p.ntiles * p.nsplit, (Few<T, DP, false>::NW * 64), (Few<T, DP, false>::LDS), st, a);
     TDX_CHECK_LAUNCH("window_attn_few_kernel");
     if (p.nsplit > 1) {
       hipLaunchKernelGGL((window_attn_join_kernel<T, DP>), dim3((unsigned)(bh * a.Tq * a.G)), dim3(256), 0, st, a);
@@ -1630,7 +1692,7 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
 template <typename T, int DP>
 int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
   const long bh = (long)a.B * a.Hkv;
-  constexpr int OCC = DP == 128 ? 1 : 2, OCC_Q = sizeof(T) == 2 && DP == 64 ? 3 : sizeof(T) == 4 && DP == 128 ? 1 : 2, KB = 4 / (RowWalk<T, DP>::RS / 32);
+  constexpr int OCC = DP == 128 ? 1 : 2, OCC_Q = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : (DP == 128 ? 2 : DP == 64 ? 3 : 4), KB = 4 / (RowWalk<T, DP>::RS / 32);
   const long rt = ((long)a.Tq * a.G + 127) / 128;
   a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows;
   WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC_Q>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
