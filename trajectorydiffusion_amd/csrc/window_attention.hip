@@ -619,10 +619,20 @@ __device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, i
   if (d1 < a.D) o[d1] = (T)(o1 / l);
 }
 
-// blockIdx -> work item so that each XCD (workgroups go round the 8 of them) takes a contiguous run of items: neighbours read the same keys
-__device__ __forceinline__ int xcd_item(int n) {
-  const int per = n >> 3, rest = n & 7, x = blockIdx.x & 7;
-  return x * per + min(x, rest) + (blockIdx.x >> 3);
+// Work item `block` of n = nbh x per -> (batch and key head, item of it), so that the items of one head, which read the same keys, run on one
+// XCD (workgroups go round the 8 of them).  Heads go round the XCDs when their number allows it, since sequences differ in length (padded
+// tracks: each XCD gets heads of every sequence); else each XCD takes a contiguous run of items.
+struct Item {
+  int bh, at;
+};
+__device__ __forceinline__ Item xcd_item(int block, int nbh, int per) {
+  const int x = block & 7, y = block >> 3;
+  if (nbh % 8 == 0) {
+    const int g = y / per;
+    return {g * 8 + x, y - g * per};
+  }
+  const int n = nbh * per, run = n >> 3, rest = n & 7, item = x * run + min(x, rest) + y, bh = item / per;
+  return {bh, item - bh * per};
 }
 
 // Q (or dO) fragments of row `row` (a query head's row), zero beyond the channels or when !ok
@@ -699,8 +709,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = xcd_item(gridDim.x);
-  const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, a.ntiles);
+  const int tile = item.at, bh = item.bh, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
   const int R = a.Tq * a.G, r0 = tile * 128, rw = r0 + wave * 32;
   const int rend = min(r0 + 128, s.ql * a.G);            // rows of the tile that see anything at all
@@ -829,8 +839,8 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = xcd_item(gridDim.x);
-  const int split = item % a.nsplit, bht = item / a.nsplit, tile = bht % a.ntiles, bh = bht / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, a.ntiles * a.nsplit);
+  const int split = item.at % a.nsplit, tile = item.at / a.nsplit, bh = item.bh, bht = bh * a.ntiles + tile, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
   const int R = a.Tq * a.G, r0 = tile * 32, rend = min(r0 + 32, s.ql * a.G);
   const int r = r0 + (lane & 31), i = r / a.G, g = r - i * a.G;
@@ -1100,8 +1110,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = xcd_item(gridDim.x);
-  const int tile = item % a.ntiles, bh = item / a.ntiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, a.ntiles);
+  const int tile = item.at, bh = item.bh, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
   const int R = a.Tq * a.G, r0 = tile * 128, rw = r0 + wave * 32;
   const int rend = min(r0 + 128, s.ql * a.G);
@@ -1213,10 +1223,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
 }
 
 // One thread's part of staging ROWS packed rows (query i, head g of the group) of q or dout: row r lies at (r / G) * ts + (r % G) * hs
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int NW>
 struct PackedStager;
-template <int DP, int ROWS>
-struct PackedStager<__bf16, DP, ROWS> {
+template <int DP, int ROWS, int NW>
+struct PackedStager<__bf16, DP, ROWS, NW> {
   using G = G16<DP>;
   static constexpr int TOTAL = ROWS * G::PITCH / 1024;
   __device__ __forceinline__ void load(uint32_t lds, const __bf16* base, long ts, long hs, int gs, int r0, int rend, int D, int wave, int lane) {
@@ -1224,9 +1234,9 @@ struct PackedStager<__bf16, DP, ROWS> {
     const u32x4 srd = make_srd(base + i0 * ts);
     const uint32_t tsb = ts * 2, hsb = hs * 2;
 #pragma unroll
-    for (int n = 0; n < (TOTAL + 3) / 4; ++n) {
-      const int it = wave + n * 4;
-      if (TOTAL % 4 == 0 || it < TOTAL) {
+    for (int n = 0; n < (TOTAL + NW - 1) / NW; ++n) {
+      const int it = wave + n * NW;
+      if (TOTAL % NW == 0 || it < TOTAL) {
         const int row = it * (1024 / G::PITCH) + lane / G::CH, chunk = (lane % G::CH) ^ swz<__bf16, DP>(row);
         const int i = (r0 + row) / gs, g = r0 + row - i * gs;
         const bool ok = r0 + row < rend && chunk * 8 < D;
@@ -1236,16 +1246,16 @@ struct PackedStager<__bf16, DP, ROWS> {
   }
   __device__ __forceinline__ void put(uint32_t) const {}
 };
-template <int DP, int ROWS>
-struct PackedStager<float, DP, ROWS> {
+template <int DP, int ROWS, int NW>
+struct PackedStager<float, DP, ROWS, NW> {
   using G = G16<DP>;
-  static constexpr int ITEMS = ROWS * G::CH, PER = (ITEMS + 255) / 256;
+  static constexpr int ITEMS = ROWS * G::CH, NT = NW * 64, PER = (ITEMS + NT - 1) / NT;
   static constexpr uint32_t PLANE = ROWS * G::PITCH;
   u32x4 held[PER][2];
   __device__ __forceinline__ void load(uint32_t, const float* base, long ts, long hs, int gs, int r0, int rend, int D, int, int) {
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
-      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
+      const int item = threadIdx.x + NT * n, row = item / G::CH, chunk = item % G::CH;
       const int i = (r0 + row) / gs, g = r0 + row - i * gs;
       const bool ok = r0 + row < rend && chunk * 8 < D && item < ITEMS;
       const float* p = base + i * ts + g * hs + chunk * 8;
@@ -1256,8 +1266,8 @@ struct PackedStager<float, DP, ROWS> {
   __device__ __forceinline__ void put(uint32_t lds) const {
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
-      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
-      if (ITEMS % 256 == 0 || item < ITEMS) {
+      const int item = threadIdx.x + NT * n, row = item / G::CH, chunk = item % G::CH;
+      if (ITEMS % NT == 0 || item < ITEMS) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(held[n][0][i]), x[4 + i] = __uint_as_float(held[n][1][i]);
@@ -1273,7 +1283,7 @@ struct PackedStager<float, DP, ROWS> {
 
 // The gradients of one key (and value) row over the query rows that see it alone (see row_again)
 template <typename T>
-__device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, int lane) {
+__device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, int lane, bool want_dk, bool want_dv) {
   const T* k = (const T*)a.k + b * a.k_bs + j * a.k_ts + hk * a.k_hs;
   const T* v = (const T*)a.v + b * a.v_bs + j * a.v_ts + hk * a.v_hs;
   const int d0 = lane, d1 = lane + 64;
@@ -1303,215 +1313,277 @@ __device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, i
   }
   T* dk = (T*)a.dk + b * a.dk_bs + j * a.dk_ts + hk * a.dk_hs;
   T* dv = (T*)a.dv + b * a.dv_bs + j * a.dv_ts + hk * a.dv_hs;
-  if (on0) dk[d0] = (T)(dk0 * a.scale), dv[d0] = (T)dv0;
-  if (on1) dk[d1] = (T)(dk1 * a.scale), dv[d1] = (T)dv1;
+  if (on0 && want_dk) dk[d0] = (T)(dk0 * a.scale);
+  if (on1 && want_dk) dk[d1] = (T)(dk1 * a.scale);
+  if (on0 && want_dv) dv[d0] = (T)dv0;
+  if (on1 && want_dv) dv[d1] = (T)dv1;
 }
 
 // What the dK / dV kernel walks over the rows with: RS rows a stage (q, dout and their {log2-sum-exp, delta}), two stages for bf16
 template <typename T, int DP>
 struct RowWalk {
   static constexpr int N = Planes<T>::N, RS = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
-  static constexpr uint32_t PLANE = RS * G16<DP>::PITCH, TILE = N * PLANE, STAT = 2 * TILE, STAGE = 2 * TILE + 1024, LDS = NSTAGE * STAGE;
+  static constexpr uint32_t PLANE = RS * G16<DP>::PITCH, TILE = N * PLANE, STAT = 2 * TILE, STAGE = 2 * TILE + 1024;
+  // At 128 channels two waves share 32 keys, one for dV and one for dK: each has one accumulator, so two waves fit a SIMD where one with both
+  // had it alone, for a quarter more matrix instructions (both take S).  bf16, causal prompts of the benchmark's training case: 241 -> see
+  // the launch.  fp32 then holds its V planes in LDS, 24 KB a wave.
+  static constexpr bool TWO = DP == 128, VLDS = TWO && N == 3;
+  static constexpr int NW = TWO ? 8 : 4;
+  static constexpr uint32_t VF = NSTAGE * STAGE, LDS = VF + (VLDS ? 4 * N * G16<DP>::NC * 1024 : 0);
 };
+// Fragments a lane parks in LDS: piece (n, c) at base + (c N + n) 1024 + 16 lane
+template <int N, int DP>
+__device__ __forceinline__ void park(uint32_t base, const Frags16<N, DP>& f, int lane) {
+#pragma unroll
+  for (int c = 0; c < G16<DP>::NC; ++c)
+#pragma unroll
+    for (int n = 0; n < N; ++n) *reinterpret_cast<lds_u32x4_t*>(base + (c * N + n) * 1024 + 16 * lane) = __builtin_bit_cast(u32x4, f[n][c]);
+}
+// rows16 whose right fragments are parked at `at` (the lane's address)
+template <int N, int DP, uint32_t IMM, uint32_t PLANE, typename F = Nothing>
+__device__ __forceinline__ void rows16_parked(f32x16& acc, const LaneOff<DP>& off, uint32_t at, F&& between = F()) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int c = 0; c < G16<DP>::NC; ++c) {
+    bf16x8 a[N], b[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) a[n] = __builtin_bit_cast(bf16x8, lds_ld16(off.row[c] + IMM + n * PLANE)), b[n] = __builtin_bit_cast(bf16x8, lds_ld16(at + (c * N + n) * 1024));
+    mma_planes<N>(acc, a, b);
+    between(c);
+  }
+}
+enum { kBoth = 0, kOnlyDv = 1, kOnlyDk = 2 };
 // One step: the 32 staged rows at A (statistics at ST) against this wave's 32 keys.  Element e of S is row 8 (e / 4) + 4 h + e % 4, column the
 // lane's key; [rlo, rhi] are the packed rows (of the whole sequence) that see the lane's key, checked when `part`.
-template <typename T, int DP, uint32_t A, uint32_t ST>
+template <typename T, int DP, uint32_t A, uint32_t ST, int ROLE>
 __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32], const LaneOff<DP>& off, uint32_t stat,
-                                         const Frags16<Planes<T>::N, DP>& kf, const Frags16<Planes<T>::N, DP>& vf, float c, bool part, int r0, int rlo, int rhi,
-                                         int lane) {
+                                         const Frags16<Planes<T>::N, DP>& kf, const Frags16<Planes<T>::N, DP>& vf, uint32_t vat, float c, bool part, int r0,
+                                         int rlo, int rhi, int lane) {
   using W = RowWalk<T, DP>;
   constexpr int NC = G16<DP>::NC, STEPS = DP / 16;
   f32x16 acc, dp;
   float p[16], ds[16];
   u32x4 l4[4], d4[4];
+  auto hide = [&](float (&x)[16]) {
+    asm volatile("");
+    const int base = r0 + 4 * (lane >> 5);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = base + 8 * (e >> 2) + (e & 3);
+      if (row < rlo || row > rhi) x[e] = 0.f;
+    }
+  };
   rows16<W::N, DP, A, W::PLANE>(acc, off, kf, [&](int k) {
 #pragma unroll
     for (int e = k * 4 / NC; e < (k + 1) * 4 / NC; ++e) l4[e] = lds_ld16(stat + ST + 32 * e);
   });
   // the exponentials stand between the products for dP, the score gradients between those for dV
-  rows16<W::N, DP, A + W::TILE, W::PLANE>(dp, off, vf, [&](int k) {
+  auto exps = [&](int k) {
 #pragma unroll
     for (int e = k * 16 / NC; e < (k + 1) * 16 / NC; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -__uint_as_float(l4[e >> 2][e & 3])));
+    if constexpr (ROLE != kOnlyDv)
 #pragma unroll
-    for (int e = k * 4 / NC; e < (k + 1) * 4 / NC; ++e) d4[e] = lds_ld16(stat + ST + 128 + 32 * e);
-  });
-  if (part) {
-    asm volatile("");
-    const int base = r0 + 4 * (lane >> 5);
+      for (int e = k * 4 / NC; e < (k + 1) * 4 / NC; ++e) d4[e] = lds_ld16(stat + ST + 128 + 32 * e);
+  };
+  if constexpr (ROLE == kOnlyDv) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int row = base + 8 * (e >> 2) + (e & 3);
-      if (row < rlo || row > rhi) p[e] = 0.f;
-    }
+    for (int k = 0; k < NC; ++k) exps(k);
+  } else if constexpr (W::VLDS) {
+    rows16_parked<W::N, DP, A + W::TILE, W::PLANE>(dp, off, vat, exps);
+  } else {
+    rows16<W::N, DP, A + W::TILE, W::PLANE>(dp, off, vf, exps);
   }
-  bf16x8 pb[2][W::N], db[2][W::N];
-  pack16<W::N>(pb, p);
-  cols16<W::N, DP, A + W::TILE, W::PLANE>(dv, off, pb, [&](int k) {
+  auto grads = [&](int e) { ds[e] = p[e] * (dp[e] - __uint_as_float(d4[e >> 2][e & 3])); };
+  bf16x8 pb[2][W::N];
+  if constexpr (ROLE != kOnlyDk) {
+    if (part) hide(p);
+    pack16<W::N>(pb, p);
+    cols16<W::N, DP, A + W::TILE, W::PLANE>(dv, off, pb, [&](int k) {
+      if constexpr (ROLE == kBoth)
 #pragma unroll
-    for (int e = k * 16 / STEPS; e < (k + 1) * 16 / STEPS; ++e) ds[e] = p[e] * (dp[e] - __uint_as_float(d4[e >> 2][e & 3]));
-  });
-  if (part) {   // (0 times an infinite dP)
-    asm volatile("");
-    const int base = r0 + 4 * (lane >> 5);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int row = base + 8 * (e >> 2) + (e & 3);
-      if (row < rlo || row > rhi) ds[e] = 0.f;
-    }
+        for (int e = k * 16 / STEPS; e < (k + 1) * 16 / STEPS; ++e) grads(e);
+    });
   }
-  pack16<W::N>(db, ds);
-  cols16<W::N, DP, A, W::PLANE>(dk, off, db);
+  if constexpr (ROLE != kOnlyDv) {
+    if constexpr (ROLE == kOnlyDk)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) grads(e);
+    if (part) hide(ds);   // (an unseen row's dP may be infinite: 0 times it is not 0)
+    pack16<W::N>(pb, ds);
+    cols16<W::N, DP, A, W::PLANE>(dk, off, pb);
+  }
 }
 
-// dK / dV.  Workgroups from nsink on: 128 keys, 4 waves x 32 keys, the rows inside the keys' windows.  The first nsink workgroups: the rows
-// beyond the window of 32 KB keys that are sinks, a share of them each; the waves are KB key blocks x row blocks of a stage, and every wave
-// leaves its fp32 sums.  Sinks among the 128 keys leave theirs as share 0.
+// dK / dV.  Workgroups from nsink on: 128 keys, 32 keys a wave (or pair of waves), the rows inside the keys' windows.  The first nsink
+// workgroups: the rows beyond the window of 32 KB keys that are sinks, a share of them each; the waves are KB key blocks x row blocks of a
+// stage, and every wave leaves its fp32 sums.  Sinks among the 128 keys leave theirs as share 0.
 template <typename T, int DP, int OCC>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void window_attn_dkv_kernel(const WaArgs a) {
+__global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void window_attn_dkv_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using W = RowWalk<T, DP>;
   constexpr int ND = DP / 32, N = W::N, NB = W::RS / 32, KB = 4 / NB;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = wave & 3;   // (waves kw and kw + 4: the same keys)
   const int nst = (a.sink_rows / 32 + KB - 1) / KB;                      // sink tiles of a (batch, key head)
   const int nsink = a.B * a.Hkv * nst * a.nsplit;
   const bool far = (int)blockIdx.x < nsink;
   int bh, jw, split = 0;
   if (far) {
-    const int bht = blockIdx.x / a.nsplit;
-    split = blockIdx.x % a.nsplit;
-    bh = bht / nst;
-    jw = (bht % nst) * KB * 32 + (wave % KB) * 32;
+    const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, nst * a.nsplit);
+    split = item.at % a.nsplit;
+    bh = item.bh;
+    jw = (item.at / a.nsplit) * KB * 32 + (kw % KB) * 32;
   } else {
-    const int n = gridDim.x - nsink, x = blockIdx.x - nsink, per = n >> 3, rest = n & 7, dev = x & 7;   // (see xcd_item)
-    const int item = dev * per + min(dev, rest) + (x >> 3);
-    bh = item / a.ntiles;
-    jw = (item % a.ntiles) * 128 + wave * 32;
+    const Item item = xcd_item(blockIdx.x - nsink, a.B * a.Hkv, a.ntiles);
+    bh = item.bh;
+    jw = item.at * 128 + kw * 32;
   }
   const int hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
   const int j = jw + (lane & 31);
   const int kend = far ? min(s.kl, a.sinks) : s.kl;                       // keys of this pass
   const bool key_ok = j < kend;
-  Frags16<N, DP> kf, vf;
-  load_frags16<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
-  load_frags16<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
-  f32x16 dk[ND], dv[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
-  arrived16(kf);
-  arrived16(vf);
-  const float c = a.scale * kLog2e;
+  const int h4 = 4 * (lane >> 5);
   // Queries [lo(first), hi(last)] see a key of [first, last]: inside the window from first - right on up to last + left, beyond it from
   // first + left + 1 on; clamped to [0, q_len], the end exclusive
   auto lo = [&](int key) { return max(0, min(s.ql, far ? key + a.left - s.shift + 1 : key - a.right - s.shift)); };
   auto hi = [&](int key) { return far ? s.ql : max(0, min(s.ql, key + a.left - s.shift + 1)); };
-  const int block_first = far ? jw - (wave % KB) * 32 : jw - wave * 32, block_last = min(block_first + (far ? KB * 32 : 128), kend) - 1;
+  const int block_first = far ? jw - (kw % KB) * 32 : jw - kw * 32, block_last = min(block_first + (far ? KB * 32 : 128), kend) - 1;
   const int wave_last = min(jw + 31, kend - 1);
-  if (block_first <= block_last) {
-    int t0 = lo(block_first) * a.G / W::RS, t1 = (hi(block_last) * a.G + W::RS - 1) / W::RS;
-    if (far) {
-      const int per = (max(0, t1 - t0) + a.nsplit - 1) / a.nsplit;
-      t0 += split * per;
-      t1 = min(t1, t0 + per);
-    }
-    const bool wave_ok = jw <= wave_last;
-    const int wr0 = lo(jw) * a.G, wr1 = wave_ok ? hi(wave_last) * a.G : 0;             // rows some key of this wave is seen by
-    const int fr0 = lo(jw + 31) * a.G, fr1 = jw + 31 < kend ? hi(jw) * a.G : 0;          // rows all of its keys are seen by
-    const int rlo = key_ok ? lo(j) * a.G : 1, rhi = key_ok ? hi(j) * a.G - 1 : 0;        // this lane's key
-    const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
-    const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
-    const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
-    const int rend = s.ql * a.G;
-    const LaneOff<DP> off(lds, lane);
-    const uint32_t stat_off = lds + W::STAT + 16 * (lane >> 5);
-    PackedStager<T, DP, W::RS> sq, sd;
-    auto load = [&](int t, uint32_t at) {
-      sq.load(at, qb, a.q_ts, a.q_hs, a.G, t * W::RS, rend, a.D, wave, lane);
-      sd.load(at + W::TILE, db, a.do_ts, a.do_hs, a.G, t * W::RS, rend, a.D, wave, lane);
-      if (wave == 0) dma16(at + W::STAT, lane < W::RS / 2 ? lane * 16u : kOutside, make_srd(stat + (long)t * (2 * W::RS)));
-    };
-    auto step = [&](int t, auto st) {
-      constexpr uint32_t S0 = decltype(st)::value;
-      auto sub = [&](auto k) {
-        constexpr int B32 = decltype(k)::value;
-        const int r0 = t * W::RS + 32 * B32;
-        if ((far && NB > 1 && wave / KB != B32) || r0 >= wr1 || r0 + 32 <= wr0) return;
-        dkv_step<T, DP, S0 + B32 * 32 * G16<DP>::PITCH, S0 + B32 * 256>(dk, dv, off, stat_off, kf, vf, c, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
+
+  auto work = [&](auto role) {
+    constexpr int ROLE = decltype(role)::value;
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
+    if (block_first <= block_last) {
+      int t0 = lo(block_first) * a.G / W::RS, t1 = (hi(block_last) * a.G + W::RS - 1) / W::RS;
+      if (far) {
+        const int per = (max(0, t1 - t0) + a.nsplit - 1) / a.nsplit;
+        t0 += split * per;
+        t1 = min(t1, t0 + per);
+      }
+      const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
+      const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
+      const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
+      const int rend = s.ql * a.G;
+      PackedStager<T, DP, W::RS, W::NW> sq, sd;
+      auto load = [&](int t, uint32_t at) {
+        sq.load(at, qb, a.q_ts, a.q_hs, a.G, t * W::RS, rend, a.D, wave, lane);
+        sd.load(at + W::TILE, db, a.do_ts, a.do_hs, a.G, t * W::RS, rend, a.D, wave, lane);
       };
-      sub(std::integral_constant<int, 0>());
-      if constexpr (NB == 2) sub(std::integral_constant<int, 1>());
-    };
-    if (t0 < t1) load(t0, lds);
-    if constexpr (N == 1) {
-      for (int t = t0; t < t1; t += 2) {
-        wait_vm<0>();
-        wg_barrier();
-        if (t + 1 < t1) load(t + 1, lds + W::STAGE);
-        step(t, std::integral_constant<uint32_t, 0>());
-        if (t + 1 >= t1) break;
-        wait_vm<0>();
-        wg_barrier();
-        if (t + 2 < t1) load(t + 2, lds);
-        step(t + 1, std::integral_constant<uint32_t, W::STAGE>());
+      auto load_stat = [&](int t, uint32_t at) {
+        if (wave == 0) dma16(at + W::STAT, lane < W::RS / 2 ? lane * 16u : kOutside, make_srd(stat + (long)t * (2 * W::RS)));
+      };
+      if (t0 < t1) {
+        load(t0, lds);
+        load_stat(t0, lds);
       }
-    } else {
-      for (int t = t0; t < t1; ++t) {
-        if (t > t0) wg_barrier();            // the tile before has been read
-        sq.put(lds);
-        sd.put(lds + W::TILE);
-        if (t > t0 && wave == 0) dma16(lds + W::STAT, lane < W::RS / 2 ? lane * 16u : kOutside, make_srd(stat + (long)t * (2 * W::RS)));
-        wait_vm<0>();
-        if (t + 1 < t1) {
-          sq.load(lds, qb, a.q_ts, a.q_hs, a.G, (t + 1) * W::RS, rend, a.D, wave, lane);
-          sd.load(lds + W::TILE, db, a.do_ts, a.do_hs, a.G, (t + 1) * W::RS, rend, a.D, wave, lane);
+      Frags16<N, DP> kf, vf;
+      const uint32_t vat = lds + W::VF + kw * (N * G16<DP>::NC * 1024) + 16 * lane;
+      load_frags16<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
+      if constexpr (ROLE != kOnlyDv) {
+        load_frags16<T, DP>(vf, (const T*)a.v + b * a.v_bs + (long)j * a.v_ts + hk * a.v_hs, key_ok, a.D, lane);
+        if constexpr (W::VLDS) park<N, DP>(vat - 16 * lane, vf, lane);
+        else arrived16(vf);
+      }
+      arrived16(kf);
+      const float c = a.scale * kLog2e;
+      const bool wave_ok = jw <= wave_last;
+      const int wr0 = lo(jw) * a.G, wr1 = wave_ok ? hi(wave_last) * a.G : 0;             // rows some key of this wave is seen by
+      const int fr0 = lo(jw + 31) * a.G, fr1 = jw + 31 < kend ? hi(jw) * a.G : 0;          // rows all of its keys are seen by
+      const int rlo = key_ok ? lo(j) * a.G : 1, rhi = key_ok ? hi(j) * a.G - 1 : 0;        // this lane's key
+      const LaneOff<DP> off(lds, lane);
+      const uint32_t stat_off = lds + W::STAT + 16 * (lane >> 5);
+      auto step = [&](int t, auto st) {
+        constexpr uint32_t S0 = decltype(st)::value;
+        auto sub = [&](auto k) {
+          constexpr int B32 = decltype(k)::value;
+          const int r0 = t * W::RS + 32 * B32;
+          if ((far && NB > 1 && kw / KB != B32) || r0 >= wr1 || r0 + 32 <= wr0) return;
+          dkv_step<T, DP, S0 + B32 * 32 * G16<DP>::PITCH, S0 + B32 * 256, ROLE>(dk, dv, off, stat_off, kf, vf, vat, c, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
+        };
+        sub(std::integral_constant<int, 0>());
+        if constexpr (NB == 2) sub(std::integral_constant<int, 1>());
+      };
+      if constexpr (N == 1) {
+        for (int t = t0; t < t1; t += 2) {
+          wait_vm<0>();
+          wg_barrier();
+          if (t + 1 < t1) load(t + 1, lds + W::STAGE), load_stat(t + 1, lds + W::STAGE);
+          step(t, std::integral_constant<uint32_t, 0>());
+          if (t + 1 >= t1) break;
+          wait_vm<0>();
+          wg_barrier();
+          if (t + 2 < t1) load(t + 2, lds), load_stat(t + 2, lds);
+          step(t + 1, std::integral_constant<uint32_t, W::STAGE>());
         }
-        wg_barrier();
-        step(t, std::integral_constant<uint32_t, 0>());
+      } else {
+        for (int t = t0; t < t1; ++t) {
+          if (t > t0) {
+            wg_barrier();                       // the tile before has been read
+            load_stat(t, lds);
+          }
+          sq.put(lds);
+          sd.put(lds + W::TILE);
+          wait_vm<0>();
+          if (t + 1 < t1) load(t + 1, lds);
+          wg_barrier();
+          step(t, std::integral_constant<uint32_t, 0>());
+        }
       }
     }
-  }
-  bool bad = false;
-  const int h4 = 4 * (lane >> 5);
-  if (far || j < a.sinks) {
-    if (j < a.sink_rows) {
-      float* part = a.part + (((long)bh * a.nparts + (far ? 1 + split * NB + wave / KB : 0)) * a.sink_rows + j) * 2 * DP;
+    bool bad_k = false, bad_v = false;
+    if (far || j < a.sinks) {
+      if (j < a.sink_rows) {
+        float* part = a.part + (((long)bh * a.nparts + (far ? 1 + split * NB + kw / KB : 0)) * a.sink_rows + j) * 2 * DP;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = 32 * d + 8 * e + h4;
+            if constexpr (ROLE != kOnlyDv) *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
+            if constexpr (ROLE != kOnlyDk) *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
+          }
+      }
+    } else if (j < a.Tk) {
+      T* krow = (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs;
+      T* vrow = (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+          float x[4], y[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            x[z] = key_ok ? dk[d][4 * e + z] * a.scale : 0.f;
+            y[z] = key_ok ? dv[d][4 * e + z] : 0.f;
+            bad_k |= x[z] != x[z];
+            bad_v |= y[z] != y[z];
+          }
           const int at = 32 * d + 8 * e + h4;
-          *reinterpret_cast<f32x4*>(part + at) = (f32x4){dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
-          *reinterpret_cast<f32x4*>(part + DP + at) = (f32x4){dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
+          if (ROLE != kOnlyDv && at < a.D) store4<T>(krow + at, x);
+          if (ROLE != kOnlyDk && at < a.D) store4<T>(vrow + at, y);
         }
     }
-  } else if (j < a.Tk) {
-    T* krow = (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs;
-    T* vrow = (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x[4], y[4];
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          x[z] = key_ok ? dk[d][4 * e + z] * a.scale : 0.f;
-          y[z] = key_ok ? dv[d][4 * e + z] : 0.f;
-          bad |= x[z] != x[z] || y[z] != y[z];
-        }
-        const int at = 32 * d + 8 * e + h4;
-        if (at < a.D) store4<T>(krow + at, x), store4<T>(vrow + at, y);
-      }
-  }
-  uint64_t again = __ballot(bad);
-  again = (again | (again >> 32)) & 0xffffffffull;
-  while (again) {
-    const int n = __builtin_ctzll(again);
-    again &= again - 1;
-    dkv_again<T>(a, s, b, hk, jw + n, lane);
+    const uint64_t mk = ROLE == kOnlyDv ? 0 : __ballot(bad_k), mv = ROLE == kOnlyDk ? 0 : __ballot(bad_v);
+    uint64_t again = mk | mv;
+    again = (again | (again >> 32)) & 0xffffffffull;
+    while (again) {
+      const int n = __builtin_ctzll(again);
+      again &= again - 1;
+      dkv_again<T>(a, s, b, hk, jw + n, lane, (mk >> n | mk >> (n + 32)) & 1, (mv >> n | mv >> (n + 32)) & 1);
+    }
+  };
+  if constexpr (W::TWO) {
+    if (wave < 4) work(std::integral_constant<int, kOnlyDv>());
+    else work(std::integral_constant<int, kOnlyDk>());
+  } else {
+    work(std::integral_constant<int, kBoth>());
   }
 #endif
 }
@@ -1551,7 +1623,7 @@ __global__ __launch_bounds__(256) void window_attn_dkv_join_kernel(const WaArgs 
       bad |= v != v;
     }
   }
-  if (__ballot(bad)) dkv_again<T>(a, s, b, hk, j, lane);
+  if (__ballot(bad)) dkv_again<T>(a, s, b, hk, j, lane, true, true);
 #endif
 }
 
@@ -1692,7 +1764,7 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
 template <typename T, int DP>
 int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
   const long bh = (long)a.B * a.Hkv;
-  constexpr int OCC = DP == 128 ? 1 : 2, OCC_Q = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : (DP == 128 ? 2 : DP == 64 ? 3 : 4), KB = 4 / (RowWalk<T, DP>::RS / 32);
+  constexpr int OCC = 2, OCC_Q = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : (DP == 128 ? 2 : DP == 64 ? 3 : 4), KB = 4 / (RowWalk<T, DP>::RS / 32);
   const long rt = ((long)a.Tq * a.G + 127) / 128;
   a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows;
   WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC_Q>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
@@ -1700,7 +1772,7 @@ int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
   if (a.Tk == 0) return TDX_OK;
   a.ntiles = (a.Tk + 127) / 128;
   const long sink_wgs = bh * ((p.sink_rows / 32 + KB - 1) / KB) * p.nsplit;
-  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), sink_wgs + bh * a.ntiles, 256, (RowWalk<T, DP>::LDS), st, a);
+  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), sink_wgs + bh * a.ntiles, (RowWalk<T, DP>::NW * 64), (RowWalk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dkv_kernel");
   if (p.sink_rows) {
     hipLaunchKernelGGL((window_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(bh * std::min(a.sinks, a.Tk))), dim3(256), 0, st, a);
