@@ -423,8 +423,9 @@ __device__ __forceinline__ void arrived16(bf16x8 (&f)[N][M]) {
     }
 }
 
-// One thread's part of staging a ROWS-row tile by 256 threads.  bf16: direct loads into LDS, whose addresses a lane keeps from tile to tile.
-// fp32: loads into registers one tile ahead; put() splits them and writes the planes.
+// One thread's part of staging a ROWS-row tile by 256 threads: direct loads into LDS, whose addresses a lane keeps from tile to tile.  bf16 is
+// used as it arrives; fp32 arrives in a buffer of its own, from which put() writes the planes.  (Held in registers across a tile instead,
+// the numbers spill, and a spill waits for its load.)
 template <typename T, int DP, int ROWS>
 struct Stager;
 template <int DP, int ROWS>
@@ -455,35 +456,45 @@ struct Stager<__bf16, DP, ROWS> {
       dma16n<PER>(lds + wave * 1024, v, srd);
     }
   }
-  __device__ __forceinline__ void put(uint32_t, int) const {}
+  __device__ __forceinline__ void put(uint32_t, uint32_t) const {}
 };
 template <int DP, int ROWS>
 struct Stager<float, DP, ROWS> {
   using G = G16<DP>;
-  static constexpr int ITEMS = ROWS * G::CH, PER = (ITEMS + 255) / 256;
-  static constexpr uint32_t PLANE = ROWS * G::PITCH;
-  u32x4 held[PER][2];
-  uint32_t stride;
-  int dbytes;
-  __device__ __forceinline__ void init(uint32_t s, int d, int, int) { stride = s, dbytes = d; }
-  __device__ __forceinline__ void load(uint32_t, const char* base, int valid, int) {
+  static constexpr int P32 = DP * 4, TOTAL = ROWS * P32 / 1024, PER = TOTAL / 4, ITEMS = ROWS * G::CH;
+  static constexpr uint32_t PLANE = ROWS * G::PITCH, RAW = ROWS * P32;
+  static_assert(TOTAL % 4 == 0, "whole loads for each of the 4 waves");
+  uint32_t voff[PER];
+  int row0;
+  __device__ __forceinline__ static int row_of(int n, int wave, int lane) { return (wave + 4 * n) * (1024 / P32) + lane / (P32 / 16); }
+  __device__ __forceinline__ void init(uint32_t stride, int dbytes, int wave, int lane) {
+    row0 = row_of(0, wave, lane);
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
-      const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
-      const bool ok = row < valid && chunk * 32 < dbytes && item < ITEMS;
-      const char* p = base + (size_t)row * stride + chunk * 32;
-      held[n][0] = ok ? *reinterpret_cast<const u32x4*>(p) : (u32x4){0u, 0u, 0u, 0u};
-      held[n][1] = ok ? *reinterpret_cast<const u32x4*>(p + 16) : (u32x4){0u, 0u, 0u, 0u};
+      const int at = (lane % (P32 / 16)) * 16;
+      voff[n] = at < dbytes ? (uint32_t)row_of(n, wave, lane) * stride + at : kOutside;
     }
   }
-  __device__ __forceinline__ void put(uint32_t lds, int) const {
+  __device__ __forceinline__ void load(uint32_t raw, const char* base, int valid, int wave) const {
+    const u32x4 srd = make_srd(base);
+    if (valid >= ROWS) {
+      dma16n<PER>(raw + wave * 1024, voff, srd);
+    } else {
+      uint32_t v[PER];
 #pragma unroll
-    for (int n = 0; n < PER; ++n) {
+      for (int n = 0; n < PER; ++n) v[n] = row0 + 4 * n * (1024 / P32) < valid ? voff[n] : kOutside;
+      dma16n<PER>(raw + wave * 1024, v, srd);
+    }
+  }
+  __device__ __forceinline__ void put(uint32_t lds, uint32_t raw) const {
+#pragma unroll
+    for (int n = 0; n < (ITEMS + 255) / 256; ++n) {
       const int item = threadIdx.x + 256 * n, row = item / G::CH, chunk = item % G::CH;
       if (ITEMS % 256 == 0 || item < ITEMS) {
         float x[8];
+        const u32x4 u = lds_ld16(raw + item * 32), w = lds_ld16(raw + item * 32 + 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(held[n][0][i]), x[4 + i] = __uint_as_float(held[n][1][i]);
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(u[i]), x[4 + i] = __uint_as_float(w[i]);
         bf16x8 p[3];
         split8<3>(x, p);
         const uint32_t at = lds + row * G::PITCH + ((chunk ^ swz<__bf16, DP>(row)) << 4);
@@ -656,7 +667,7 @@ __device__ __forceinline__ void arrived(F (&f)[N]) {
 template <typename T, int DP>
 struct Walk {
   static constexpr int N = Planes<T>::N, BN = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
-  static constexpr uint32_t PLANE = BN * G16<DP>::PITCH, TILE = N * PLANE, STAGE = 2 * TILE, LDS = NSTAGE * STAGE;
+  static constexpr uint32_t PLANE = BN * G16<DP>::PITCH, TILE = N * PLANE, STAGE = 2 * TILE, RAW = N == 1 ? 0 : BN * DP * 4, LDS = NSTAGE * STAGE + 2 * RAW;
 };
 // Calls f(key, offset of the stage in LDS as a type) for each key tile of `t`, staged
 // (ready() is called once the first tile's loads are on their way)
@@ -672,9 +683,9 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
   auto load = [&](int it, uint32_t at) {
     const int j0 = tile_start(t, it, W::BN);
     sk.load(at, (const char*)(kb + (long)j0 * a.k_ts), s.kl - j0, wave);
-    sv.load(at + W::TILE, (const char*)(vb + (long)j0 * a.v_ts), s.kl - j0, wave);
+    sv.load(at + (W::N == 1 ? W::TILE : W::RAW), (const char*)(vb + (long)j0 * a.v_ts), s.kl - j0, wave);
   };
-  if (n > 0) load(0, lds);
+  if (n > 0) load(0, W::N == 1 ? lds : lds + W::STAGE);
   ready();
   if constexpr (W::N == 1) {
     for (int it = 0; it < n; it += 2) {
@@ -690,11 +701,12 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
     }
   } else {
     for (int it = 0; it < n; ++it) {
-      if (it) wg_barrier();            // the tile before has been read
-      sk.put(lds, 0);
-      sv.put(lds + W::TILE, 0);
-      if (it + 1 < n) load(it + 1, lds);
+      wait_vm<0>();
+      wg_barrier();                    // the numbers are there, the planes of the tile before have been read
+      sk.put(lds, lds + W::STAGE);
+      sv.put(lds + W::TILE, lds + W::STAGE + W::RAW);
       wg_barrier();
+      if (it + 1 < n) load(it + 1, lds + W::STAGE);
       f(tile_start(t, it, W::BN), std::integral_constant<uint32_t, 0>());
     }
   }
