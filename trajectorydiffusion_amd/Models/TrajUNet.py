@@ -198,7 +198,9 @@ class UNetProgram:
 
 
 class TrajUNet(_PackedModel):
-    def __init__(self, channel_schedule: List[int], traj_length: int = 200, diffusion_steps: int = 300, res_blocks: int = 2) -> None:
+    def __init__(self, channel_schedule: List[int], traj_length: int = 200, diffusion_steps: int = 300, res_blocks: int = 2, *, attn_heads: int = 1,
+                 attn_window: Optional[int] = None, attn_sinks: int = 0, attn_rotary: Optional[float] = None) -> None:
+        """attn_* (beyond the reference): the middle block's attention with a window, for long tracks (AttnBlock); same parameters."""
         super().__init__()
         if res_blocks < 2:
             raise TdxError("TrajUNet: res_blocks must be >= 2 (with 1 the reference's decoder feeds a 2C-channel tensor to a C-channel conv)")
@@ -215,7 +217,7 @@ class TrajUNet(_PackedModel):
             layers += [ResnetBlock(cs[i + 1], norm_groups=32) for _ in range(res_blocks - 1)]
             layers.append(nn.Conv1d(cs[i + 1], cs[i + 1], 3, 2, 1))  # downsample
             self.down_blocks.append(nn.ModuleList(layers))
-        self.mid_attn_block = AttnBlock(cs[-1], norm_groups=32)
+        self.mid_attn_block = AttnBlock(cs[-1], norm_groups=32, heads=attn_heads, window=attn_window, sinks=attn_sinks, rotary=attn_rotary)
         self.up_blocks = nn.ModuleList()
         for i in range(self.stages):
             cin, cout = cs[self.stages - i], cs[self.stages - i - 1]

@@ -136,11 +136,17 @@ class ResnetBlock(_HipBlock):
 
 
 class AttnBlock(_HipBlock):
-    """Res -> single-head self-attention -> Res (reference Models/TrajUNetBlocks.py:102-125)."""
+    """Res -> single-head self-attention -> Res (reference Models/TrajUNetBlocks.py:102-125).
 
-    def __init__(self, in_c: int, norm_groups: int) -> None:
+    Beyond the reference, for long tracks (its attention here takes 64 tokens, 16 in training): window = w lets every token see the tokens
+    up to w away, and the first `sinks` of all; heads splits the channels (at most 128 a head); rotary = base turns q and k by the token's
+    index.  The parameters are the same."""
+
+    def __init__(self, in_c: int, norm_groups: int, *, heads: int = 1, window: Optional[int] = None, sinks: int = 0,
+                 rotary: Optional[float] = None) -> None:
         super().__init__()
         self.in_c, self.norm_groups = in_c, norm_groups
+        self.window_spec = engine.WindowSpec.check(in_c, heads, window, sinks, rotary)
         self.res1 = ResnetBlock(in_c, in_c, norm_groups)
         self.qkv_getter = nn.Sequential(nn.GroupNorm(norm_groups, in_c, eps=1e-6), nn.Conv1d(in_c, in_c * 3, 1, 1, 0))
         self.project_out = nn.Conv1d(in_c, in_c, 1, 1, 0)
@@ -165,7 +171,10 @@ class AttnBlock(_HipBlock):
                 3 * Cn, B, L, 3 * Cn, name=key + "qkv")
         pg.release(a)
         o = pg.alloc((B, L, Cn))
-        pg.call(key + "attention", pg.lib.tdx_attention, qkv.data_ptr(), o.data_ptr(), B, L, Cn, pg.code, keep=[qkv, o])
+        if self.window_spec is not None:
+            self.window_spec.emit(pg, key + "attention", qkv, o, None, B, L, Cn)
+        else:
+            pg.call(key + "attention", pg.lib.tdx_attention, qkv.data_ptr(), o.data_ptr(), B, L, Cn, pg.code, keep=[qkv, o])
         pg.release(qkv)
         x2 = pg.alloc((B, L, Cn))
         gn_r2 = engine.block_input_gn(pg, self.res2, key + "res2.", B, L)

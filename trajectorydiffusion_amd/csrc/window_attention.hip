@@ -567,6 +567,18 @@ __device__ __forceinline__ float softmax_max(const float (&s)[16], float& m, flo
   for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
   return softmax_follow<ND>(half_max(t), m, l, o, c, slack);
 }
+// exp2(s c - mc) in one fused step is exact enough while the rounding of mc = m c is small; beyond 2^22 the scores are moved by m first
+template <int NS>
+__device__ __forceinline__ void softmax_huge(float (&s)[NS][16], float m, float& mc) {
+  if (__ballot(__builtin_fabsf(mc) > 4194304.f)) {
+    const float me = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] -= me;
+    mc = 0.f;
+  }
+}
 // elements [A, B) of the scores become exponentials
 template <int A, int B>
 __device__ __forceinline__ void softmax_exp(float (&s)[16], float& l, float off, float c) {
@@ -614,7 +626,7 @@ __device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, i
   const int p = i + s.shift, hi = min(p + a.right, s.kl - 1), lo = max(p - a.left, 0);
   const int d0 = lane, d1 = lane + 64;
   const float q0 = d0 < a.D ? Elem<T>::ld(q + d0) : 0.f, q1 = d1 < a.D ? Elem<T>::ld(q + d1) : 0.f;
-  const float c = a.scale * kLog2e, off = m * c;
+  const float c = a.scale * kLog2e;
   float o0 = 0.f, o1 = 0.f;
   for (int j = 0; j <= hi; ++j) {
     if (j < lo && j >= a.sinks) j = lo;
@@ -622,7 +634,7 @@ __device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, i
     const T *kr = k + j * a.k_ts, *vr = v + j * a.v_ts;
     float d = (d0 < a.D ? q0 * Elem<T>::ld(kr + d0) : 0.f) + (d1 < a.D ? q1 * Elem<T>::ld(kr + d1) : 0.f);
     d = wave_sum(d);
-    const float w = __builtin_amdgcn_exp2f(fmaf(d, c, -off));
+    const float w = __builtin_amdgcn_exp2f((d - m) * c);
     if (d0 < a.D) o0 = fmaf(w, Elem<T>::ld(vr + d0), o0);
     if (d1 < a.D) o1 = fmaf(w, Elem<T>::ld(vr + d1), o1);
   }
@@ -772,7 +784,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 16; ++e) t = fmaxf(t, sc[n][e]);
-        const float mc = softmax_follow<ND>(half_max(t), m, l, o, c, slack);
+        float mc = softmax_follow<ND>(half_max(t), m, l, o, c, slack);
+        softmax_huge<2>(sc, m, mc);
         softmax_exp<0, 16>(sc[0], l, mc, c);
         pack16<N>(pb, sc[0]);
         // the exponentials of the second half stand between the products of the first with V
@@ -791,7 +804,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
         if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
-        softmax_exp<0, 16>(sc[0], l, softmax_max<ND>(sc[0], m, l, o, c, slack), c);
+        float mc = softmax_max<ND>(sc[0], m, l, o, c, slack);
+        softmax_huge<1>(sc, m, mc);
+        softmax_exp<0, 16>(sc[0], l, mc, c);
         pack16<N>(pb, sc[0]);
         cols16<N, DP, S0 + W::TILE, W::PLANE>(o, off, pb);
       }
@@ -898,12 +913,14 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       if (cls) {
         f32x16 acc;
         rows_times<T, DP>(acc, kt, 0, qf, lane);
-        float sc[16];
+        float sc[1][16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = acc[e];
-        if (cls == 1) mask_scores(sc, a, s, j0, p, lane);
-        softmax_exp<0, 16>(sc, l, softmax_max<G::ND>(sc, m, l, o, c, slack), c);
-        cols_times<DP>(o, vt, 0, sc, lane, T());
+        for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
+        if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
+        float mc = softmax_max<G::ND>(sc[0], m, l, o, c, slack);
+        softmax_huge<1>(sc, m, mc);
+        softmax_exp<0, 16>(sc[0], l, mc, c);
+        cols_times<DP>(o, vt, 0, sc[0], lane, T());
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage has been read before the ring comes round to it
     }

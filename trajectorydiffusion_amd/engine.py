@@ -8,6 +8,7 @@ the path is a call into libtrajdiff_hip.so (trajectorydiffusion_amd/_lib.py).
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -437,6 +438,81 @@ def emit_embed(pg: Program, emb, packed: Dict[str, torch.Tensor], B: int, time: 
         pg.release(hd)
     for t in (pe, catvec, deep_in):
         pg.release(t)
+
+
+class WindowSpec:
+    """How a self-attention block with a window attends (AttnBlock's heads / window / sinks / rotary) over qkv rows (B, L, 3 C): descriptors
+    of tdx_rotary_axes and tdx_window_attention on slices of those rows."""
+
+    def __init__(self, heads: int, window: int, sinks: int, rotary: Optional[float]):
+        self.heads, self.window, self.sinks, self.rotary = heads, window, sinks, rotary
+
+    @staticmethod
+    def check(Cn: int, heads: int, window: Optional[int], sinks: int, rotary: Optional[float]) -> Optional["WindowSpec"]:
+        """The spec of a block of Cn channels (None: the reference's attention), or TdxError."""
+        if window is None:
+            if heads != 1 or sinks != 0 or rotary is not None:
+                raise TdxError("AttnBlock: heads, sinks and rotary belong to attention with a window; give one (a window of at least the number of "
+                               "tokens sees all of them)")
+            return None
+        for n, v, lo in (("heads", heads, 1), ("window", window, 0), ("sinks", sinks, 0)):
+            if isinstance(v, bool) or not isinstance(v, int) or v < lo:
+                raise TdxError(f"AttnBlock: {n}={v!r} (a whole number >= {lo})")
+        if Cn % heads or Cn // heads % 8 or Cn // heads > 128:
+            raise TdxError(f"AttnBlock: {Cn} channels in {heads} heads: a head has a multiple of 8 channels, at most 128")
+        if rotary is not None and not (math.isfinite(rotary) and rotary > 0):
+            raise TdxError(f"AttnBlock: rotary={rotary!r} (None, or a base > 0)")
+        return WindowSpec(heads, window, sinks, None if rotary is None else float(rotary))
+
+    def rotary_desc(self, rows: torch.Tensor, pos: torch.Tensor, B: int, L: int, Cn: int, code: int, inverse: bool) -> _lib.RotaryDesc:
+        """q and k of the rows (B, L, 3 Cn), in place, by the token's index."""
+        D = Cn // self.heads
+        d = _lib.RotaryDesc()
+        d.x = d.out = rows.data_ptr()
+        d.pos, d.pos_bs, d.pos_ts, d.pos_as = pos.data_ptr(), 0, 1, 1
+        d.x_bs = d.out_bs = L * 3 * Cn
+        d.x_ts = d.out_ts = 3 * Cn
+        d.x_hs = d.out_hs = D
+        d.B, d.T, d.H, d.D, d.dtype, d.layout, d.inverse, d.naxes = B, L, 2 * self.heads, D, code, 0, int(inverse), 1
+        d.sections[0], d.base[0] = D // 2, self.rotary
+        return d
+
+    def attn_desc(self, rows: torch.Tensor, out: torch.Tensor, lse: Optional[torch.Tensor], B: int, L: int, Cn: int, code: int) -> _lib.WindowAttnDesc:
+        D, es = Cn // self.heads, rows.element_size()
+        d = _lib.WindowAttnDesc()
+        d.q, d.k, d.v, d.out, d.lse = rows.data_ptr(), rows.data_ptr() + Cn * es, rows.data_ptr() + 2 * Cn * es, out.data_ptr(), _lib.ptr(lse)
+        d.q_bs = d.k_bs = d.v_bs = L * 3 * Cn
+        d.q_ts = d.k_ts = d.v_ts = 3 * Cn
+        d.q_hs = d.k_hs = d.v_hs = D
+        d.out_bs, d.out_ts, d.out_hs = L * Cn, Cn, D
+        d.B, d.Tq, d.Tk, d.Hq, d.Hkv, d.D, d.dtype = B, L, L, self.heads, self.heads, D, code
+        d.left = d.right = self.window
+        d.sinks, d.scale = self.sinks, D ** -0.5
+        return d
+
+    def grad_desc(self, d: _lib.WindowAttnDesc, dout: torch.Tensor, drows: torch.Tensor, Cn: int) -> _lib.WindowAttnDesc:
+        """d with the gradient of its output, and its gradients as slices of drows (B, L, 3 Cn)."""
+        es = drows.element_size()
+        d.dout, d.dout_bs, d.dout_ts, d.dout_hs = dout.data_ptr(), d.out_bs, d.out_ts, d.out_hs
+        d.dq, d.dk, d.dv = drows.data_ptr(), drows.data_ptr() + Cn * es, drows.data_ptr() + 2 * Cn * es
+        d.dq_bs = d.dk_bs = d.dv_bs = d.q_bs
+        d.dq_ts = d.dk_ts = d.dv_ts = d.q_ts
+        d.dq_hs = d.dk_hs = d.dv_hs = d.q_hs
+        return d
+
+    def emit(self, pg: Program, name: str, rows: torch.Tensor, out: torch.Tensor, lse: Optional[torch.Tensor], B: int, L: int, Cn: int) -> None:
+        """Record the forward launches.  The rotation replaces q and k in the rows."""
+        if self.rotary is not None:
+            pos = torch.arange(L, dtype=torch.float32, device=pg.device)
+            r = self.rotary_desc(rows, pos, B, L, Cn, pg.code, False)
+            pg.call(name + ".rotary", pg.lib.tdx_rotary_axes, C.byref(r), keep=[r, pos, rows])
+        d = self.attn_desc(rows, out, lse, B, L, Cn, pg.code)
+        n = int(pg.lib.tdx_window_attention_ws_bytes(C.byref(d)))
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=pg.device)
+            d.ws, d.ws_bytes = ws.data_ptr(), n
+            pg.keep.append(ws)
+        pg.call(name, pg.lib.tdx_window_attention, C.byref(d), keep=[d, rows, out, lse])
 
 
 def check_err_flag(err: torch.Tensor, what: str) -> None:

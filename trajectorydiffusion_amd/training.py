@@ -339,6 +339,29 @@ class TrainStep:
                          self.PG(bet).data_ptr() + 4 * p_off, 1, F32, self.red_ws.data_ptr())
         self._back.append(backward)
 
+    def _window_attention(self, name: str, spec, qkv: torch.Tensor, o: torch.Tensor, L: int, Cn: int) -> None:
+        """Attention with a window over qkv rows (B, L, 3 Cn) -> o.  The rotation replaces q and k in the rows, so the backward pass
+        finds them as the forward product saw them, and turns their gradients back in place."""
+        B, lib = self.B, self.lib
+        lse = self._new(B, spec.heads, L)
+        spec.emit(self.fw, name, qkv, o, lse, B, L, Cn)
+
+        def backward():
+            go, gq = self.G(o), self.G(qkv)
+            self.first_write(qkv)
+            d = spec.grad_desc(spec.attn_desc(qkv, o, lse, B, L, Cn, F32), go, gq, Cn)
+            n = int(lib.tdx_window_attention_bwd_ws_bytes(C.byref(d)))
+            ws = self._new(n, dtype=torch.uint8)
+            d.ws, d.ws_bytes = ws.data_ptr(), n
+            self._keep.append(d)
+            self.bw.call(name + ".bwd", lib.tdx_window_attention_bwd, C.byref(d))
+            if spec.rotary is not None:
+                pos = torch.arange(L, dtype=torch.float32, device=self.dev)
+                r = spec.rotary_desc(gq, pos, B, L, Cn, F32, True)
+                self._keep += [r, pos]
+                self.bw.call(name + ".rotary.bwd", lib.tdx_rotary_axes, C.byref(r))
+        self._back.append(backward)
+
     # ---- the network ------------------------------------------------------------------------------------------------------
     def _resblock(self, key: str, blk, srcs: List[Tuple[torch.Tensor, int]], L: int) -> torch.Tensor:
         """ResnetBlock (TrajUNetBlocks.py:92-99); srcs = the (possibly concatenated) raw input as [(rows tensor, channels)]."""
@@ -441,9 +464,12 @@ class TrainStep:
         qkv = self._new(B, lm, 3 * Cn)
         self.conv(key + "qkv", [_Src(a, Cn, lm, ab.qkv_getter[1].weight, taps=1)], 3 * Cn, lm, qkv, biases=[ab.qkv_getter[1].bias])
         o = self._new(B, lm, Cn)
-        self.fw.call(key + "attention", lib.tdx_attention, qkv.data_ptr(), o.data_ptr(), B, lm, Cn, F32)
-        self._back.append(lambda: (self.first_write(qkv), self.bw.call(key + "attention.bwd", lib.tdx_attention_bwd, qkv.data_ptr(), self.G(o).data_ptr(),
-                                                                         self.G(qkv).data_ptr(), B, lm, Cn)))
+        if ab.window_spec is not None:
+            self._window_attention(key + "attention", ab.window_spec, qkv, o, lm, Cn)
+        else:
+            self.fw.call(key + "attention", lib.tdx_attention, qkv.data_ptr(), o.data_ptr(), B, lm, Cn, F32)
+            self._back.append(lambda: (self.first_write(qkv), self.bw.call(key + "attention.bwd", lib.tdx_attention_bwd, qkv.data_ptr(), self.G(o).data_ptr(),
+                                                                             self.G(qkv).data_ptr(), B, lm, Cn)))
         x2 = self._new(B, lm, Cn)
         self.conv(key + "proj", [_Src(o, Cn, lm, ab.project_out.weight, taps=1)], Cn, lm, x2, biases=[ab.project_out.bias], res=x1)
         cur = self._resblock(key + "res2.", ab.res2, [(x2, Cn)], lm)
