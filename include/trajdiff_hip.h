@@ -468,6 +468,8 @@ typedef struct {
   const int32_t *q_lens, *k_lens;
   void* ws;                          /* device scratch of at least the bytes the matching *_ws_bytes() call returns (NULL if 0); */
   int64_t ws_bytes;                  /* written before it is read, so calls that do not overlap may share it */
+  void* out_lo;                      /* bf16 only, or NULL: (B, Tq, Hq, D) contiguous, what the rounding of out left; written by the forward pass,
+                                        read by the backward pass (without it gradients of rows that see a few keys lose up to half a bit more) */
   /* backward only */
   const void* dout;                  /* gradient of out */
   void *dq, *dk, *dv;                /* all three are overwritten (rows i >= q_len, keys j >= k_len: zero) */

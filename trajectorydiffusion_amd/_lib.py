@@ -52,7 +52,7 @@ class WindowAttnDesc(C.Structure):
     _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("q_bs", _i64), ("q_ts", _i64), ("q_hs", _i64), ("k_bs", _i64),
                 ("k_ts", _i64), ("k_hs", _i64), ("v_bs", _i64), ("v_ts", _i64), ("v_hs", _i64), ("out_bs", _i64), ("out_ts", _i64), ("out_hs", _i64),
                 ("B", _i32), ("Tq", _i32), ("Tk", _i32), ("Hq", _i32), ("Hkv", _i32), ("D", _i32), ("dtype", _i32), ("left", _i32), ("right", _i32),
-                ("sinks", _i32), ("scale", _f32), ("reserved", _i32), ("q_lens", _vp), ("k_lens", _vp), ("ws", _vp), ("ws_bytes", _i64), ("dout", _vp),
+                ("sinks", _i32), ("scale", _f32), ("reserved", _i32), ("q_lens", _vp), ("k_lens", _vp), ("ws", _vp), ("ws_bytes", _i64), ("out_lo", _vp), ("dout", _vp),
                 ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dout_bs", _i64), ("dout_ts", _i64), ("dout_hs", _i64), ("dq_bs", _i64), ("dq_ts", _i64),
                 ("dq_hs", _i64), ("dk_bs", _i64), ("dk_ts", _i64), ("dk_hs", _i64), ("dv_bs", _i64), ("dv_ts", _i64), ("dv_hs", _i64)]
 

@@ -237,7 +237,7 @@ def _form(q, k, v, left, right, sinks, scale, q_lens, k_lens) -> _Form:
     return f
 
 
-def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse):
+def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse, out_lo=None):
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     if out.numel() == 0:
@@ -246,7 +246,7 @@ def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse):
     lse = torch.empty(f.lse_shape, dtype=torch.float32, device=dev) if want_lse else None
     d = f.desc
     d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    d.lse = None if lse is None else lse.data_ptr()
+    d.lse, d.out_lo = None if lse is None else lse.data_ptr(), None if out_lo is None else out_lo.data_ptr()
     d.q_lens, d.k_lens = None if q_lens is None else q_lens.data_ptr(), None if k_lens is None else k_lens.data_ptr()
     if f.ws:
         ws = torch.empty(f.ws, dtype=torch.uint8, device=dev)
@@ -258,8 +258,10 @@ def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse):
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, left, right, sinks, scale, q_lens, k_lens):
-        out, lse = _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, True)
-        ctx.save_for_backward(q, k, v, out, lse, q_lens, k_lens)
+        # what bf16 leaves of the result, for the backward pass's row sums of dout times out
+        out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
+        out, lse = _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, True, out_lo)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, k_lens, out_lo)
         ctx.args = (left, right, sinks, scale)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -272,7 +274,7 @@ class _WindowAttention(torch.autograd.Function):
         none = (None,) * 6
         if dout is None:
             return (None, None, None) + none
-        q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
+        q, k, v, out, lse, q_lens, k_lens, out_lo = ctx.saved_tensors
         dev = q.device
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         if dq.numel() == 0 or dk.numel() == 0:
@@ -296,6 +298,7 @@ class _WindowAttention(torch.autograd.Function):
         d.q, d.k, d.v, d.out, d.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
         d.q_lens, d.k_lens = None if q_lens is None else q_lens.data_ptr(), None if k_lens is None else k_lens.data_ptr()
         d.dout, d.dq, d.dk, d.dv, d.ws, d.ws_bytes = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), f.bwd_ws
+        d.out_lo = None if out_lo is None else out_lo.data_ptr()
         _launch(lib.tdx_window_attention_bwd, "tdx_window_attention_bwd", d, q.get_device())
         return (dq, dk, dv) + none
 

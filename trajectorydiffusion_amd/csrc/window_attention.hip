@@ -34,6 +34,7 @@ constexpr uint32_t kOutside = 0x80000000u;
 struct WaArgs {
   const void *q, *k, *v;
   void* out;
+  __bf16* out_lo;                     // or null: what the rounding of out left, (B, Tq, Hq, D)
   float* lse;
   long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;
   int B, Tq, Tk, Hkv, G, D;
@@ -615,6 +616,22 @@ __device__ __forceinline__ void store4<__bf16>(__bf16* p, const float (&v)[4]) {
   *reinterpret_cast<u32x2*>(p) = (u32x2){w[0], w[1]};
 }
 
+// Four channels from d of the result of query i, head hq.  For the backward pass what bf16 leaves of it is stored too: delta = sum dO O from a
+// rounded O alone is off by 2^-9 of |dO| |O|, which for rows that see a few keys is as much as all other roundings of dQ and dK together
+// (their error goes from 2.3 to 1.5 times that of one rounding at two keys, from 1.5 to 1.45 at 64).
+template <typename T>
+__device__ __forceinline__ void store_out(const WaArgs& a, int b, int i, long hq, int d, const float (&v)[4]) {
+  store4<T>((T*)a.out + b * a.o_bs + (long)i * a.o_ts + hq * a.o_hs + d, v);
+  if constexpr (sizeof(T) == 2) {
+    if (a.out_lo) {
+      float lo[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) lo[x] = v[x] - (float)(__bf16)v[x];
+      store4<__bf16>(a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D + d, lo);
+    }
+  }
+}
+
 // A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN.  A row whose sum of exponentials is
 // a number but whose result is not is therefore taken again, over the keys it sees alone: one wave, its lanes split the channels.
 template <typename T>
@@ -622,7 +639,8 @@ __device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, i
   const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + (long)(hk * a.G + g) * a.q_hs;
   const T* k = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
   const T* v = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
-  T* o = (T*)a.out + b * a.o_bs + i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
+  const long hq = (long)(hk * a.G + g);
+  T* o = (T*)a.out + b * a.o_bs + i * a.o_ts + hq * a.o_hs;
   const int p = i + s.shift, hi = min(p + a.right, s.kl - 1), lo = max(p - a.left, 0);
   const int d0 = lane, d1 = lane + 64;
   const float q0 = d0 < a.D ? Elem<T>::ld(q + d0) : 0.f, q1 = d1 < a.D ? Elem<T>::ld(q + d1) : 0.f;
@@ -638,8 +656,16 @@ __device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, i
     if (d0 < a.D) o0 = fmaf(w, Elem<T>::ld(vr + d0), o0);
     if (d1 < a.D) o1 = fmaf(w, Elem<T>::ld(vr + d1), o1);
   }
-  if (d0 < a.D) o[d0] = (T)(o0 / l);
-  if (d1 < a.D) o[d1] = (T)(o1 / l);
+  o0 /= l, o1 /= l;
+  if (d0 < a.D) o[d0] = (T)o0;
+  if (d1 < a.D) o[d1] = (T)o1;
+  if constexpr (sizeof(T) == 2) {
+    if (a.out_lo) {
+      __bf16* r = a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D;
+      if (d0 < a.D) r[d0] = (__bf16)(o0 - (float)(__bf16)o0);
+      if (d1 < a.D) r[d1] = (__bf16)(o1 - (float)(__bf16)o1);
+    }
+  }
 }
 
 // Work item `block` of n = nbh x per -> (batch and key head, item of it), so that the items of one head, which read the same keys, run on one
@@ -817,7 +843,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
   const float inv = row_ok && l != 0.f ? 1.0f / l : 0.f;
   bool bad = false;
   if (r < R) {
-    T* orow = (T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
     const int h4 = 4 * (lane >> 5);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -829,7 +854,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
           v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
           bad |= v[x] != v[x];
         }
-        if (32 * d + 8 * e + h4 < a.D) store4<T>(orow + 32 * d + 8 * e + h4, v);
+        if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
       }
     if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l) : -INFINITY;
   }
@@ -930,7 +955,6 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
     const float inv = row_ok && l != 0.f ? 1.0f / l : 0.f;
     bool bad = false;
     if (r < R) {
-      T* orow = (T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs;
       const int h4 = 4 * (lane >> 5);
 #pragma unroll
       for (int d = 0; d < G::ND; ++d)
@@ -942,7 +966,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
             v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
             bad |= v[x] != v[x];
           }
-          if (32 * d + 8 * e + h4 < a.D) store4<T>(orow + 32 * d + 8 * e + h4, v);
+          if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
         }
       if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l) : -INFINITY;
     }
@@ -1009,7 +1033,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
         v[x] = inv != 0.f ? oo[x] * inv : (ll != ll ? ll : 0.f);
         bad |= v[x] != v[x];
       }
-      if (d < a.D) store4<T>((T*)a.out + b * a.o_bs + (long)ii * a.o_ts + (long)(hk * a.G + gg) * a.o_hs + d, v);
+      if (d < a.D) store_out<T>(a, b, ii, hk * a.G + gg, d, v);
       if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? mm * a.scale + __logf(ll) : -INFINITY;
     }
     uint64_t again = __ballot(bad && ok && ll == ll);
@@ -1087,7 +1111,7 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
     v[x] = inv != 0.f ? O[x] * inv : (L != L ? L : 0.f);
     bad |= v[x] != v[x];
   }
-  if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store4<T>((T*)a.out + b * a.o_bs + (long)i * a.o_ts + (long)(hk * a.G + g) * a.o_hs + 4 * threadIdx.x, v);
+  if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store_out<T>(a, b, i, hk * a.G + g, 4 * threadIdx.x, v);
   if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L) : -INFINITY;
   if (__ballot(bad && ok && L == L)) row_again<T>(a, s, b, hk, i, g, M, L, threadIdx.x);
 #endif
@@ -1169,6 +1193,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
         Elem<T>::unpack(*reinterpret_cast<const u32x4*>(drow + d), dv);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) delta = fmaf(ov[e], dv[e], delta);
+        if constexpr (sizeof(T) == 2) {
+          if (a.out_lo) {
+            Elem<T>::unpack(*reinterpret_cast<const u32x4*>(a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D + d), ov);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) delta = fmaf(ov[e], dv[e], delta);
+          }
+        }
       }
     }
     lse = a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i];
@@ -1687,6 +1718,8 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
   a.v_bs = d->v_bs, a.v_ts = d->v_ts, a.v_hs = d->v_hs, a.o_bs = d->out_bs, a.o_ts = d->out_ts, a.o_hs = d->out_hs;
   a.B = d->B, a.Tq = d->Tq, a.Tk = d->Tk, a.Hkv = d->Hkv, a.G = d->Hq / d->Hkv, a.D = d->D, a.scale = d->scale;
   a.q_lens = d->q_lens, a.k_lens = d->k_lens;
+  a.out_lo = d->dtype == TDX_BF16 ? (__bf16*)d->out_lo : nullptr;
+  TDX_CHECK_ARG(((uintptr_t)a.out_lo & 15) == 0, "%s: misaligned out_lo", fn);
   // a limit beyond every length is none; sinks that hold every key too
   a.left = d->left < 0 || d->left >= d->Tk || d->sinks >= d->Tk ? kFar : d->left;
   a.right = d->right < 0 || (int64_t)d->right >= (int64_t)d->Tk + d->Tq ? kFar : d->right;
