@@ -301,7 +301,7 @@ __device__ __forceinline__ void mma_planes(f32x16& acc, const bf16x8 (&a)[N], co
 // (The six products of a step of fp32 planes cover it by themselves.)
 template <int N>
 __device__ __forceinline__ void pin() {
-  if constexpr (N == 1) __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_sched_barrier(0);
 }
 struct Nothing {
   __device__ __forceinline__ void operator()(int) const {}
@@ -1177,43 +1177,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
   Frags16<N, DP> qf, df;
-  const T* drow = (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs;
-  load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
-  load_frags16<T, DP>(df, drow, row_ok, a.D, lane);
-  float delta = 0.f, lse = -INFINITY;
-  if (row_ok) {
+  float delta = 0.f, lse2 = INFINITY;
+  // the rows' own data, behind the first tile's loads; a row that sees nothing has lse = -inf: +inf makes its probabilities 0
+  auto rows_ready = [&] {
+    load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
+    load_frags16<T, DP>(df, (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs, row_ok, a.D, lane);
     const T* orow = (const T*)a.out + b * a.o_bs + (long)i * a.o_ts + hq * a.o_hs;
-    constexpr int VEC = Elem<T>::kVec;
+    Frags16<N, DP> of, lf;
+    load_frags16<T, DP>(of, orow, row_ok, a.D, lane);
+    if constexpr (N == 1) load_frags16<T, DP>(lf, a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D, row_ok && a.out_lo, a.D, lane);
+    const float lse = row_ok ? a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i] : -INFINITY;
 #pragma unroll
-    for (int x = 0; x < DP / (2 * VEC); ++x) {
-      const int d = (2 * x + (lane >> 5)) * VEC;
-      if (d < a.D) {
-        float ov[VEC], dv[VEC];
-        Elem<T>::unpack(*reinterpret_cast<const u32x4*>(orow + d), ov);
-        Elem<T>::unpack(*reinterpret_cast<const u32x4*>(drow + d), dv);
+    for (int x = 0; x < G16<DP>::NC; ++x) {
+      float ov[8], dv[8];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) delta = fmaf(ov[e], dv[e], delta);
-        if constexpr (sizeof(T) == 2) {
-          if (a.out_lo) {
-            Elem<T>::unpack(*reinterpret_cast<const u32x4*>(a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D + d), ov);
+      for (int e = 0; e < 8; ++e) ov[e] = dv[e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) delta = fmaf(ov[e], dv[e], delta);
-          }
-        }
+      for (int n = N - 1; n >= 0; --n) {   // (the planes of a number add up to it, the smallest first)
+        float ow[8], dw[8];
+        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, of[n][x]), ow);
+        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, df[n][x]), dw);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ov[e] += ow[e], dv[e] += dw[e];
       }
+      if constexpr (N == 1) {
+        float lv[8];
+        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, lf[0][x]), lv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(lv[e], dv[e], delta);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf(ov[e], dv[e], delta);
     }
-    lse = a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i];
-  }
-  delta = half_sum(delta);
-  // a row that sees nothing has lse = -inf: +inf makes its probabilities 0
-  const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
-  if (lse == -INFINITY) delta = 0.f;
-  {
-    float* st = a.stat + ((long)bh * a.ntiles32 + tile * 4 + wave) * 64;
-    st[lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
-  }
-  arrived16(qf);
-  arrived16(df);
+    delta = half_sum(delta);
+    if (lse == -INFINITY) delta = 0.f;
+    else lse2 = lse * kLog2e;
+    arrived16(qf);
+    arrived16(df);
+  };
   const float c = a.scale * kLog2e;
   if (r0 < rend) {
     const LaneOff<DP> off(lds, lane);
@@ -1249,12 +1250,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
       pack16<N>(db, sc);
       cols16<N, DP, A, W::PLANE>(dq, off, db);
     };
-    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [] {}, [&](int j0, auto st) {
+    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, rows_ready,
+                     [&](int j0, auto st) {
       constexpr uint32_t S0 = decltype(st)::value;
       one(j0, std::integral_constant<uint32_t, S0>());
       if constexpr (W::BN == 64) one(j0 + 32, std::integral_constant<uint32_t, S0 + 32 * G16<DP>::PITCH>());
     });
   }
+  a.stat[((long)bh * a.ntiles32 + tile * 4 + wave) * 64 + lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
   bool bad = false;
   if (r < R) {
     T* qrow = (T*)a.dq + b * a.dq_bs + (long)i * a.dq_ts + hq * a.dq_hs;
