@@ -1181,33 +1181,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
   // the rows' own data, behind the first tile's loads; a row that sees nothing has lse = -inf: +inf makes its probabilities 0
   auto rows_ready = [&] {
     load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
-    load_frags16<T, DP>(df, (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs, row_ok, a.D, lane);
     const T* orow = (const T*)a.out + b * a.o_bs + (long)i * a.o_ts + hq * a.o_hs;
-    Frags16<N, DP> of, lf;
-    load_frags16<T, DP>(of, orow, row_ok, a.D, lane);
-    if constexpr (N == 1) load_frags16<T, DP>(lf, a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D, row_ok && a.out_lo, a.D, lane);
+    const T* drow = (const T*)a.dout + b * a.do_bs + (long)i * a.do_ts + hq * a.do_hs;
     const float lse = row_ok ? a.lse[((long)b * a.Hkv * a.G + hq) * a.Tq + i] : -INFINITY;
+    if constexpr (N == 1) {
+      Frags16<1, DP> of, lf;
+      load_frags16<T, DP>(df, drow, row_ok, a.D, lane);
+      load_frags16<T, DP>(of, orow, row_ok, a.D, lane);
+      load_frags16<T, DP>(lf, a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D, row_ok && a.out_lo, a.D, lane);
 #pragma unroll
-    for (int x = 0; x < G16<DP>::NC; ++x) {
-      float ov[8], dv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ov[e] = dv[e] = 0.f;
-#pragma unroll
-      for (int n = N - 1; n >= 0; --n) {   // (the planes of a number add up to it, the smallest first)
-        float ow[8], dw[8];
-        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, of[n][x]), ow);
-        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, df[n][x]), dw);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ov[e] += ow[e], dv[e] += dw[e];
-      }
-      if constexpr (N == 1) {
-        float lv[8];
+      for (int x = 0; x < G16<DP>::NC; ++x) {
+        float ov[8], dv[8], lv[8];
+        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, of[0][x]), ov);
+        Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, df[0][x]), dv);
         Elem<__bf16>::unpack(__builtin_bit_cast(u32x4, lf[0][x]), lv);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta = fmaf(lv[e], dv[e], delta);
-      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf(ov[e], dv[e], delta);
+        for (int e = 0; e < 8; ++e) delta = fmaf(ov[e], dv[e], delta);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < G16<DP>::NC; ++x) {
+        const int d = 16 * x + 8 * (lane >> 5);
+        const bool in = row_ok && d < a.D;
+        float dv[8];
+        u32x4 w[2], o[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          w[k] = in ? *reinterpret_cast<const u32x4*>(drow + d + 4 * k) : (u32x4){0u, 0u, 0u, 0u};
+          o[k] = in ? *reinterpret_cast<const u32x4*>(orow + d + 4 * k) : (u32x4){0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dv[e] = __uint_as_float(w[e >> 2][e & 3]), delta = fmaf(__uint_as_float(o[e >> 2][e & 3]), dv[e], delta);
+        bf16x8 p[N];
+        split8<N>(dv, p);
+#pragma unroll
+        for (int n = 0; n < N; ++n) df[n][x] = p[n];
+      }
     }
     delta = half_sum(delta);
     if (lse == -INFINITY) delta = 0.f;
