@@ -101,7 +101,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, pos, sections, bases, layout, inverse):
         ctx.save_for_backward(pos)
         ctx.args = (sections, bases, layout, inverse)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
         _rotary_launch(x, pos, sections, bases, layout, inverse, out)
         return out
 
@@ -113,7 +113,7 @@ class _Rotary(torch.autograd.Function):
         sections, bases, layout, inverse = ctx.args
         if dout.stride(3) != 1 and dout.shape[3] != 1:
             dout = dout.contiguous()
-        dx = torch.empty(dout.shape, dtype=dout.dtype, device=dout.device)
+        dx = dout.new_empty(dout.shape)
         if dx.numel():
             _rotary_launch(dout, pos, sections, bases, layout, not inverse, dx)   # a rotation's transpose is its inverse
         return dx, None, None, None, None, None
@@ -183,7 +183,7 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
         if x.numel() == 0:
             return x.clone()
         return _Rotary.apply(x, pos, sections, bases, code, bool(inverse))
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(x.shape)
     if x.numel():
         _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
     return out
@@ -238,18 +238,17 @@ def _form(q, k, v, left, right, sinks, scale, q_lens, k_lens) -> _Form:
 
 
 def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse, out_lo=None):
-    dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = q.new_empty(q.shape)
     if out.numel() == 0:
-        return out, torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if want_lse else None
+        return out, q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32) if want_lse else None
     f = _form(q, k, v, left, right, sinks, scale, q_lens, k_lens)
-    lse = torch.empty(f.lse_shape, dtype=torch.float32, device=dev) if want_lse else None
+    lse = q.new_empty(f.lse_shape, dtype=torch.float32) if want_lse else None
     d = f.desc
     d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     d.lse, d.out_lo = None if lse is None else lse.data_ptr(), None if out_lo is None else out_lo.data_ptr()
     d.q_lens, d.k_lens = None if q_lens is None else q_lens.data_ptr(), None if k_lens is None else k_lens.data_ptr()
     if f.ws:
-        ws = torch.empty(f.ws, dtype=torch.uint8, device=dev)
+        ws = q.new_empty(f.ws, dtype=torch.uint8)
         d.ws, d.ws_bytes = ws.data_ptr(), f.ws
     _launch(_lib.lib().tdx_window_attention, "tdx_window_attention", d, q.get_device())
     return out, lse
@@ -259,7 +258,7 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, left, right, sinks, scale, q_lens, k_lens):
         # what bf16 leaves of the result, for the backward pass's row sums of dout times out
-        out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
+        out_lo = q.new_empty(q.shape) if q.dtype == torch.bfloat16 else None
         out, lse = _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, True, out_lo)
         ctx.save_for_backward(q, k, v, out, lse, q_lens, k_lens, out_lo)
         ctx.args = (left, right, sinks, scale)
@@ -275,8 +274,7 @@ class _WindowAttention(torch.autograd.Function):
         if dout is None:
             return (None, None, None) + none
         q, k, v, out, lse, q_lens, k_lens, out_lo = ctx.saved_tensors
-        dev = q.device
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         if dq.numel() == 0 or dk.numel() == 0:
             return (dq.zero_(), dk.zero_(), dv.zero_()) + none
         dout = _fits(dout, 1 << 31)
@@ -290,11 +288,11 @@ class _WindowAttention(torch.autograd.Function):
             d.dk_bs, d.dk_ts, d.dk_hs = _strides(dk)
             d.dv_bs, d.dv_ts, d.dv_hs = _strides(dv)
             d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-            with torch.cuda.device(dev):
+            with torch.cuda.device(q.device):
                 f.bwd_ws = lib.tdx_window_attention_bwd_ws_bytes(C.byref(d))
             f.bwd_key = key
         d = f.bwd
-        ws = torch.empty(f.bwd_ws, dtype=torch.uint8, device=dev)
+        ws = q.new_empty(f.bwd_ws, dtype=torch.uint8)
         d.q, d.k, d.v, d.out, d.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
         d.q_lens, d.k_lens = None if q_lens is None else q_lens.data_ptr(), None if k_lens is None else k_lens.data_ptr()
         d.dout, d.dq, d.dk, d.dv, d.ws, d.ws_bytes = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), f.bwd_ws
