@@ -232,6 +232,24 @@ def test_attention_takes_slices_and_odd_strides(dtype, Tq, Tk):
             R.check(f"{name}: {n}", g, *want[n])
 
 
+def test_rows_far_apart_in_memory():
+    # 64 rows of q and of dout span 2.6 GB: as far as one tile's offsets do not reach
+    A = _att()
+    T, ts = 64, 20 * 1024 * 1024
+    room = torch.empty(T * ts, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = [torch.randn(1, T, 1, 32, generator=g, device="cuda").bfloat16() for _ in range(4)]
+    far = [room[o:].as_strided((1, T, 1, 32), (T * ts, ts, 32, 1)) for o in (0, 1024)]
+    for f, t in zip(far, (x[0], x[3])):
+        f.copy_(t)
+    results = []
+    for q, dout in ((x[0], x[3]), far):
+        q, k, v = (t.detach().requires_grad_() for t in (q, x[1], x[2]))
+        out = A.window_attention(q, k, v, 20, 4, 3)
+        results.append((out.detach(),) + torch.autograd.grad(out, (q, k, v), dout))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("Tq,Tk,few", [(1, 700, True), (150, 150, True), (150, 150, False)])

@@ -163,6 +163,19 @@ def test_c_attention_backward_refuses(kw):
     assert b"tdx_window_attention_bwd" in lib.tdx_last_error()
 
 
+def test_token_strides_beyond_a_stage_are_refused_or_copied():
+    # dK / dV reads 64 rows from one address with 31-bit offsets: 64 token strides must stay below 2 GiB, also where 33 do
+    _lib, att = _mod()
+    lib = _lib.lib()
+    ts = (1 << 30) // 48                                       # elements; x 2 bytes: 33 strides are 1.4 GiB, 65 are 2.7 GiB
+    ts -= ts % 8
+    for kw in (dict(q_ts=ts), dict(dout_ts=ts)):
+        d = _attn_desc(B=1, Tq=64, Tk=64, Hq=1, Hkv=1, dtype=_lib.TDX_BF16, ws=16 * P, ws_bytes=1 << 40, **kw)
+        assert lib.tdx_window_attention_bwd(C.byref(d), None) == 1 and b"too large" in lib.tdx_last_error()
+    t = torch.empty(1, dtype=torch.bfloat16, device="meta").as_strided((1, 64, 1, 32), (64 * ts, ts, 32, 1))
+    assert not att._lies_well(t, 1 << 31)
+
+
 def test_c_attention_workspaces():
     _lib, _ = _mod()
     lib = _lib.lib()

@@ -194,7 +194,7 @@ def _lies_well(t: torch.Tensor, most_token_bytes: int) -> bool:
     """Whether the kernels can take t as it lies, its address aside."""
     bs, ts, hs = _strides(t)
     es = t.element_size()
-    return t.stride(3) == 1 and not ((bs | ts | hs) * es) % 16 and ts * es < most_token_bytes and (33 * ts + t.shape[2] * hs) * es < 1 << 31
+    return t.stride(3) == 1 and not ((bs | ts | hs) * es) % 16 and ts * es < most_token_bytes and (65 * ts + t.shape[2] * hs) * es < 1 << 31
 
 
 def _fits(t: torch.Tensor, most_token_bytes: int) -> torch.Tensor:

@@ -1743,7 +1743,7 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
   TDX_CHECK_ARG(strides_ok(d->q_bs, d->q_ts, d->q_hs, es) && strides_ok(d->k_bs, d->k_ts, d->k_hs, es) && strides_ok(d->v_bs, d->v_ts, d->v_hs, es) &&
                     strides_ok(d->out_bs, d->out_ts, d->out_hs, es), "%s: strides must be multiples of 16 bytes and not negative", fn);
   TDX_CHECK_ARG(d->k_ts * es < (1 << 24) && d->v_ts * es < (1 << 24), "%s: the token strides of k and v must be below 16 MiB", fn);
-  TDX_CHECK_ARG((33 * d->q_ts + a.G * d->q_hs) * es < (1ll << 31), "%s: the strides of q are too large", fn);
+  TDX_CHECK_ARG((65 * d->q_ts + a.G * d->q_hs) * es < (1ll << 31), "%s: the strides of q are too large", fn);
   TDX_CHECK_ARG(((uintptr_t)d->q_lens & 3) == 0 && ((uintptr_t)d->k_lens & 3) == 0, "%s: misaligned lengths", fn);
   return TDX_OK;
 }
@@ -1903,7 +1903,7 @@ extern "C" int tdx_window_attention_bwd(const tdx_window_attn_desc* d, void* str
                 "tdx_window_attention_bwd: null or misaligned pointer");
   TDX_CHECK_ARG(strides_ok(d->dout_bs, d->dout_ts, d->dout_hs, es) && strides_ok(d->dq_bs, d->dq_ts, d->dq_hs, es) && strides_ok(d->dk_bs, d->dk_ts, d->dk_hs, es) &&
                     strides_ok(d->dv_bs, d->dv_ts, d->dv_hs, es), "tdx_window_attention_bwd: strides must be multiples of 16 bytes and not negative");
-  TDX_CHECK_ARG((33 * d->dout_ts + a.G * d->dout_hs) * es < (1ll << 31), "tdx_window_attention_bwd: the strides of dout are too large");
+  TDX_CHECK_ARG((65 * d->dout_ts + a.G * d->dout_hs) * es < (1ll << 31), "tdx_window_attention_bwd: the strides of dout are too large");
   const BwdPlan p = plan_backward(a, es);
   TDX_CHECK_ARG(pointer_ok(d->ws) && d->ws_bytes >= p.stat_bytes + p.part_bytes, "tdx_window_attention_bwd: workspace of %lld bytes needed, got %lld",
                 (long long)(p.stat_bytes + p.part_bytes), (long long)d->ws_bytes);
