@@ -176,6 +176,18 @@ def test_token_strides_beyond_a_stage_are_refused_or_copied():
     assert not att._lies_well(t, 1 << 31)
 
 
+def test_c_launches_of_more_threads_than_a_launch_counts_are_refused():
+    _lib, _ = _mod()
+    lib = _lib.lib()
+    many = 1 << 24                                             # workgroups of 256 threads: 2^32
+    assert lib.tdx_rotary_axes(C.byref(_rotary_desc(B=many, T=8, H=1)), None) == 1 and b"too many" in lib.tdx_last_error()
+    d = _attn_desc(B=many, Tq=1, Tk=4096, Hq=1, Hkv=1, left=-1, sinks=0)
+    assert lib.tdx_window_attention(C.byref(d), None) == 1 and b"too many" in lib.tdx_last_error()
+    for kw in (dict(Tq=1, Tk=8), dict(Tq=1, Tk=8, D=32), dict(Tq=1, Tk=100, sinks=9, left=2, B=many // 8)):
+        d = _attn_desc(**dict(dict(B=many, Hq=1, Hkv=1, ws=16 * P, ws_bytes=1 << 60), **kw))
+        assert lib.tdx_window_attention_bwd(C.byref(d), None) == 1 and b"too many" in lib.tdx_last_error()
+
+
 def test_c_attention_workspaces():
     _lib, _ = _mod()
     lib = _lib.lib()

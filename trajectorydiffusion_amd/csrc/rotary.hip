@@ -146,7 +146,7 @@ extern "C" int tdx_rotary_axes(const tdx_rotary_desc* d, void* stream) {
   // tokens per workgroup: 8 when that still leaves four workgroups a CU, fewer for short calls
   a.tb = 8;
   while (a.tb > 1 && a.tokens < (long)a.tb * 1024) a.tb >>= 1;
-  TDX_CHECK_ARG((a.tokens + a.tb - 1) / a.tb <= 0x7fffffffL, "tdx_rotary_axes: too many tokens");
+  TDX_CHECK_ARG((a.tokens + a.tb - 1) / a.tb * 256 <= 0xffffffffL, "tdx_rotary_axes: too many tokens");
   const int vec = d->dtype == TDX_F32 ? 4 : 8;
   const long str = a.x_bs | a.x_ts | a.x_hs | a.o_bs | a.o_ts | a.o_hs;
   const bool v = (((uintptr_t)a.x | (uintptr_t)a.out) & 15) == 0 && str % vec == 0 && d->D % vec == 0 &&

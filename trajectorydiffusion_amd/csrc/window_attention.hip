@@ -1752,7 +1752,9 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
 struct Plan {
   bool few, one;
   int ntiles, nsplit;
+  int64_t threads;                    // of the largest launch
 };
+constexpr int64_t kMostThreads = 0xffffffffLL;   // a launch counts its threads in 32 bits
 constexpr int kMostSplits = 64;       // (the join kernel holds a row's shares in registers)
 Plan plan_forward(const WaArgs& a) {
   Plan p{};
@@ -1768,6 +1770,7 @@ Plan plan_forward(const WaArgs& a) {
     p.nsplit = (int)std::max<long>(1, std::min<long>(std::min<long>(want, tiles / 8), kMostSplits));
     p.one = tiles <= 2;
   }
+  p.threads = bh * std::max<int64_t>((int64_t)p.ntiles * p.nsplit * (p.one ? 64 : 256), p.nsplit > 1 ? rows * 256 : 0);
   return p;
 }
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
@@ -1819,12 +1822,13 @@ int launch_forward_d(WaArgs& a, const Plan& p, hipStream_t st) {
 // Backward: bytes of the row statistics, and of the sinks' shares
 struct BwdPlan {
   int sink_rows, nsplit, nparts;
-  int64_t stat_bytes, part_bytes;
+  int64_t stat_bytes, part_bytes, threads;
 };
 BwdPlan plan_backward(const WaArgs& a, int es) {
   BwdPlan p{};
   const int64_t rows = (int64_t)a.Tq * a.G, bh = (int64_t)a.B * a.Hkv, dp = padded(a.D);
   p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
+  int64_t sink_wgs = 0;
   if (a.sinks > 0) {
     const int nb = es == 4 ? 1 : 2, kb = 4 / nb;                        // row and key blocks of a workgroup (RowWalk)
     p.sink_rows = (a.sinks + 31) / 32 * 32;
@@ -1833,7 +1837,10 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
     p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((compute_units() + wgs - 1) / wgs, rows / (nb * 32 * 8)));
     p.nparts = 1 + p.nsplit * nb;
     p.part_bytes = bh * p.nparts * p.sink_rows * 2 * dp * 4;
+    sink_wgs = wgs * p.nsplit;
   }
+  const int64_t keys = ((int64_t)a.Tk + 127) / 128;
+  p.threads = std::max({bh * ((rows + 127) / 128) * 256, (sink_wgs + bh * keys) * (dp == 128 ? 512 : 256), bh * std::min(a.sinks, a.Tk) * 256});
   return p;
 }
 
@@ -1881,7 +1888,7 @@ extern "C" int tdx_window_attention(const tdx_window_attn_desc* d, void* stream)
   const Plan p = plan_forward(a);
   const int64_t need = p.nsplit > 1 ? (int64_t)a.B * a.Hkv * p.ntiles * p.nsplit * 32 * (padded(a.D) + 2) * 4 : 0;
   TDX_CHECK_ARG(need == 0 || (pointer_ok(d->ws) && d->ws_bytes >= need), "tdx_window_attention: workspace of %lld bytes needed, got %lld", (long long)need, (long long)d->ws_bytes);
-  TDX_CHECK_ARG((long)a.B * a.Hkv * a.Tq * a.G < 0x7fffffffL, "tdx_window_attention: too many rows");
+  TDX_CHECK_ARG((long)a.B * a.Hkv * a.Tq * a.G < 0x7fffffffL && p.threads <= kMostThreads, "tdx_window_attention: too many rows");
   a.ws = (float*)d->ws;
   return d->dtype == TDX_F32 ? launch_forward_d<float>(a, p, (hipStream_t)stream) : launch_forward_d<__bf16>(a, p, (hipStream_t)stream);
 }
@@ -1907,7 +1914,7 @@ extern "C" int tdx_window_attention_bwd(const tdx_window_attn_desc* d, void* str
   const BwdPlan p = plan_backward(a, es);
   TDX_CHECK_ARG(pointer_ok(d->ws) && d->ws_bytes >= p.stat_bytes + p.part_bytes, "tdx_window_attention_bwd: workspace of %lld bytes needed, got %lld",
                 (long long)(p.stat_bytes + p.part_bytes), (long long)d->ws_bytes);
-  TDX_CHECK_ARG((long)a.B * a.Hkv * std::max<long>((long)a.Tq * a.G, a.Tk) < 0x7fffffffL, "tdx_window_attention_bwd: too many rows");
+  TDX_CHECK_ARG((long)a.B * a.Hkv * std::max<long>((long)a.Tq * a.G, a.Tk) < 0x7fffffffL && p.threads <= kMostThreads, "tdx_window_attention_bwd: too many rows");
   a.dout = d->dout, a.dq = d->dq, a.dk = d->dk, a.dv = d->dv;
   a.do_bs = d->dout_bs, a.do_ts = d->dout_ts, a.do_hs = d->dout_hs, a.dq_bs = d->dq_bs, a.dq_ts = d->dq_ts, a.dq_hs = d->dq_hs;
   a.dk_bs = d->dk_bs, a.dk_ts = d->dk_ts, a.dk_hs = d->dk_hs, a.dv_bs = d->dv_bs, a.dv_ts = d->dv_ts, a.dv_hs = d->dv_hs;
