@@ -97,6 +97,17 @@ def test_rotary_strides_shared_positions_in_place_and_out(dtype):
         assert A.rotary_axes(e, torch.zeros(empty[0], empty[1], 2, device="cuda"), sec).shape == empty
 
 
+def test_rotary_out_beside_x_and_across_it():
+    A = _att()
+    qk = _normal(2, 6, 4, 32, dtype=torch.float32, seed=4).cuda()
+    pos = torch.arange(6.0, device="cuda")[:, None]
+    want = A.rotary_axes(qk[:, :, :2], pos, (16,))
+    A.rotary_axes(qk[:, :, :2], pos, (16,), out=qk[:, :, 2:])          # between each other in one buffer
+    assert torch.equal(qk[:, :, 2:], want)
+    with pytest.raises(A.TdxError, match="overlaps"):
+        A.rotary_axes(qk[:, :-1], pos[:-1], (16,), out=qk[:, 1:])
+
+
 @pytest.mark.parametrize("layout", ["halves", "pairs"])
 def test_rotary_gradient(layout):
     A = _att()

@@ -163,6 +163,31 @@ def test_c_attention_backward_refuses(kw):
     assert b"tdx_window_attention_bwd" in lib.tdx_last_error()
 
 
+def test_an_output_that_overlaps_x_is_told_from_one_beside_it():
+    _, att = _mod()
+    room = torch.zeros(4 * 3 * 2 * 16)
+    whole = room.view(1, 4, 6, 16)
+    q, k = whole[:, :, :2], whole[:, :, 2:4]
+    assert not att._clash(q, k) and not att._clash(k, q) and not att._clash(q, q) and not att._clash(q, whole[:, :, :2])
+    assert att._clash(whole[:, :-1], whole[:, 1:]) and att._clash(whole[:, 1:], whole[:, :-1]) and att._clash(whole[:, :, :2], whole[:, :, 1:3])
+    assert not att._clash(whole[:, :2], whole[:, 2:]) and att._clash(whole[..., :8], whole[..., 4:12]) and not att._clash(whole[..., :8], whole[..., 8:])
+    assert att._clash(whole.view(1, 4, 6, 16), room.view(1, 6, 4, 16).transpose(1, 2))      # other strides
+    assert not att._clash(whole, torch.zeros_like(whole))
+    # against the element numbers themselves
+    ids = torch.arange(200)
+    gen = torch.Generator().manual_seed(5)
+    draw = lambda n: int(torch.randint(0, n, (1,), generator=gen))
+    for _ in range(400):
+        shape = tuple(1 + draw(3) for _ in range(4))
+        stride = tuple([1, 3, 4, 7, 12, 20][draw(6)] for _ in range(4))
+        x, out = (ids.as_strided(shape, stride, draw(40)) for _ in range(2))
+        pairs = {a: i for i, a in enumerate(x.flatten().tolist())}
+        if len(pairs) < x.numel():
+            continue                                            # x repeats its own memory
+        want = any(pairs.get(a, i) != i for i, a in enumerate(out.flatten().tolist()))
+        assert att._clash(x, out) == want, (shape, stride, x.storage_offset(), out.storage_offset())
+
+
 def test_token_strides_beyond_a_stage_are_refused_or_copied():
     # dK / dV reads 64 rows from one address with 31-bit offsets: 64 token strides must stay below 2 GiB, also where 33 do
     _lib, att = _mod()

@@ -138,6 +138,29 @@ def _rotary_args(x, pos, sections, base, layout) -> Tuple:
     return sections, bases, _LAYOUTS[layout]
 
 
+def _clash(x: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether `out` holds an element of x's memory at another place than x does (of one form and type; views of one storage only).
+    Equal strides: some difference of indices leads from one address to the other.  Other strides: the spans meet."""
+    if x.untyped_storage().data_ptr() != out.untyped_storage().data_ptr() or not x.numel():
+        return False
+    far, dims = out.storage_offset() - x.storage_offset(), [(st, n) for st, n in zip(x.stride(), x.shape) if n > 1]
+    if dims != [(st, n) for st, n in zip(out.stride(), out.shape) if n > 1]:
+        span = lambda t: sum((n - 1) * st for st, n in zip(t.stride(), t.shape))
+        return -span(out) <= far <= span(x)
+    dims.sort(reverse=True)
+
+    def reached(far: int, at: int) -> bool:
+        if at == len(dims):
+            return far == 0
+        st, n = dims[at]
+        if st == 0:
+            return reached(far, at + 1)
+        inner = sum((m - 1) * t for t, m in dims[at + 1:])
+        low, high = -((inner - far) // st), (far + inner) // st
+        return any(reached(far - i * st, at + 1) for i in range(max(low, 1 - n), min(high, n - 1) + 1))
+    return far != 0 and reached(far, 0)
+
+
 def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], base: Union[float, Sequence[float]] = 10000.0, layout: str = "halves",
                 inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Turns the channel pairs of every head of x (B, T, H, D <= 256) by angles of the token's position.
@@ -147,7 +170,7 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     base      pair i of n of an axis turns by pos * base^(-i / n); one number, or one for each axis
     layout    "halves": channels (m, m + P) are pair m; "pairs": channels (2 m, 2 m + 1)
     inverse   turn back
-    out       write here (x itself: in place); not differentiable
+    out       write here (x itself: in place; no other overlap); not differentiable
     Differentiable in x.  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
     try:   # a form of call that was checked before?
@@ -176,6 +199,8 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
             raise TdxError(f"{fn}: out= is not differentiable")
         if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
             raise TdxError(f"{fn}: out must not repeat its own memory")
+        if out is not x and _clash(x, out):
+            raise TdxError(f"{fn}: out overlaps x other than in place")
         if x.numel():
             _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
         return out
