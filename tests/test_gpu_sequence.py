@@ -243,6 +243,20 @@ def test_attention_takes_slices_and_odd_strides(dtype, Tq, Tk):
             R.check(f"{name}: {n}", g, *want[n])
 
 
+def test_numbers_given_as_tensors_count_by_their_value():
+    A = _att()
+    x = _normal(2, 40, 2, 32, dtype=torch.float32, seed=6).cuda()
+    pos = torch.arange(40.0, device="cuda")[:, None]
+    scale, base, pairs = torch.tensor(0.25), torch.tensor(100.0), torch.tensor(16)
+    for _ in range(2):
+        assert torch.equal(A.window_attention(x, x, x, 5, 5, 1, scale=scale), A.window_attention(x, x, x, 5, 5, 1, scale=float(scale)))
+        for b in (base, [base]):
+            assert torch.equal(A.rotary_axes(x, pos, [pairs], base=b), A.rotary_axes(x, pos, (int(pairs),), base=float(base)))
+        scale.mul_(3)
+        base.mul_(7)
+        pairs.sub_(4)
+
+
 def test_rows_far_apart_in_memory():
     # 64 rows of q and of dout span 2.6 GB: as far as one tile's offsets do not reach
     A = _att()

@@ -174,9 +174,11 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     Differentiable in x.  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
     try:   # a form of call that was checked before?
-        key = (x.shape, x.dtype, x.device, pos.shape, pos.dtype, pos.device, tuple(sections), base if base.__class__ is float else tuple(base), layout)
+        sections = tuple(map(int, sections))   # (numbers, not what they come from: a tensor's value may change)
+        base = base if base.__class__ is float else tuple(map(float, base)) if isinstance(base, (list, tuple)) else float(base)
+        key = (x.shape, x.dtype, x.device, pos.shape, pos.dtype, pos.device, sections, base, layout)
         args = _known("rotary_args").get(key)
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, ValueError):
         key = args = None
     if args is None:
         args = _rotary_args(x, pos, sections, base, layout)
@@ -381,10 +383,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     query does not see, NaN and infinities too, does not reach it.  Strided tensors are taken as they lie when their channels are
     contiguous and their strides multiples of 16 bytes, else copied.  Differentiable in q, k, v; results are reproducible."""
     try:   # a form of call that was checked before?
+        if scale is not None and scale.__class__ is not float:
+            scale = float(scale)
         key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, left, right, sinks, scale,
                left.__class__, right.__class__, sinks.__class__)
         args = _known("attention_args").get(key)
-    except (AttributeError, TypeError, RuntimeError):
+    except (AttributeError, TypeError, ValueError, RuntimeError):
         key = args = None
     if args is None:
         args = _attention_args(q, k, v, left, right, sinks, scale)
