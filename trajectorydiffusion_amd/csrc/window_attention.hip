@@ -8,8 +8,8 @@
 //   S^T (keys x rows) = K Q^T, the accumulator of lane (n = lane & 31, h = lane >> 5) then holds, for row n, the scores of the keys
 //   8 g + 4 h + r (g, r = 0..3): softmax statistics are one number per lane (and its partner n + 32), and the probabilities are
 //   already where the second product wants its right operand, O^T (channels x rows) = V^T P^T, once its contraction index is
-//   taken in the order the scores are held in.  V^T then has to be read from LDS along the keys: with bf16 by the transposing
-//   LDS read, which hands lane i of 16 lanes column i of a 4 x 16 tile; with fp32 by plain 4-byte reads (one key per lane half).
+//   taken in the order the scores are held in.  V^T then has to be read from LDS along the keys: 16-bit tiles by the transposing
+//   LDS read, which hands lane i of 16 lanes column i of a 4 x 16 tile; fp32 tiles (few rows) by plain 4-byte reads (one key per lane half).
 // K and V tiles are staged in LDS as they lie in memory (direct loads, 16 bytes a lane); the 16-byte pieces of a row are permuted
 // (swz) so that neither the row reads nor the transposed ones meet in a bank.
 #include "tdx_common.h"
@@ -297,9 +297,8 @@ __device__ __forceinline__ void mma_planes(f32x16& acc, const bf16x8 (&a)[N], co
   acc = mfma16(a[0], b[0], acc);
 }
 // Reads run AHEAD steps in front of the matrix instructions that take them, and vector work that is ready stands between these: the order
-// is pinned, since left alone the compiler reads one fragment, waits for it and multiplies, and every step pays the read's latency.
-// (The six products of a step of fp32 planes cover it by themselves.)
-template <int N>
+// is pinned, since left alone the compiler reads one fragment, waits for it and multiplies, and every step pays the read's latency
+// (dK / dV, causal prompts of 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 293 -> 241 us).
 __device__ __forceinline__ void pin() {
   __builtin_amdgcn_sched_barrier(0);
 }
@@ -323,13 +322,13 @@ __device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, cons
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     if (c + AHEAD < NC) read(c + AHEAD);
-    pin<N>();
+    pin();
     bf16x8 bc[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) bc[n] = b[n][c];
     mma_planes<N>(acc, a[c % RING], bc);
     between(c);
-    pin<N>();
+    pin();
   }
 }
 // x as N bf16 planes; an infinity (or what rounds to one) is the first plane alone
@@ -383,10 +382,10 @@ __device__ __forceinline__ void cols16(f32x16 (&acc)[DP / 32], const LaneOff<DP>
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
     if (k + AHEAD < STEPS) read(k + AHEAD);
-    pin<N>();
+    pin();
     mma_planes<N>(acc[k % G::ND], a[k % RING], b[k / G::ND]);
     between(k);
-    pin<N>();
+    pin();
   }
 }
 // a 32-row operand in registers: channels 16 c + 8 h .. + 7 of row `row`, zero beyond the channels or when !ok
@@ -618,7 +617,8 @@ __device__ __forceinline__ void store4<__bf16>(__bf16* p, const float (&v)[4]) {
 
 // Four channels from d of the result of query i, head hq.  For the backward pass what bf16 leaves of it is stored too: delta = sum dO O from a
 // rounded O alone is off by 2^-9 of |dO| |O|, which for rows that see a few keys is as much as all other roundings of dQ and dK together
-// (their error goes from 2.3 to 1.5 times that of one rounding at two keys, from 1.5 to 1.45 at 64).
+// (their error goes from 2.3 to 1.5 times that of one rounding at two keys, from 1.5 to 1.45 at 64).  It costs the forward pass of a training
+// step a second store: 91 -> 104 us at 33 MB of results.
 template <typename T>
 __device__ __forceinline__ void store_out(const WaArgs& a, int b, int i, long hq, int d, const float (&v)[4]) {
   store4<T>((T*)a.out + b * a.o_bs + (long)i * a.o_ts + hq * a.o_hs + d, v);
@@ -701,7 +701,8 @@ __device__ __forceinline__ void arrived(F (&f)[N]) {
   for (int c = 0; c < N; ++c) asm volatile("" : "+v"(f[c]));
 }
 
-// What the many-row kernels walk over the key tiles with: BN keys a tile, bf16 in two stages of direct loads, fp32 in one stage of planes
+// What the many-row kernels walk over the key tiles with: BN keys a tile, bf16 in two stages of direct loads, fp32 in one stage of planes and
+// one of numbers as they arrive (forward at 128 channels: 128 us with the numbers held in registers, 88 so; 64 keys a tile would leave a compute unit one workgroup)
 template <typename T, int DP>
 struct Walk {
   static constexpr int N = Planes<T>::N, BN = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
@@ -751,6 +752,11 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
 }
 
 // ---- forward, many rows: 4 waves x 32 rows ----------------------------------------------------------------------------------------------
+// Bound by the SIMDs, which share their issue between matrix and vector work (a score costs as many cycles of exponential, mask, sum and rounding
+// as of products at 64 channels, half at 128): what helps is waves enough to have both at hand, so registers are held to 2 waves a SIMD at 128
+// channels, 3 or 4 below.  Measured: bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 91 us, 660 TFLOP/s of what is seen (the
+// matrix units are busy 35 % of the time, the vector units 41 %); 16384 tokens, 8 heads of 64 channels, window 1025: 64 us, 540 TFLOP/s; fp32, 8 x
+// 1250 tokens and fewer, 8 heads of 64, window 257: 64 us, 80 TFLOP/s (480 of bf16 products).
 template <typename T, int DP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ? 2 : sizeof(T) == 4 ? (DP == 64 ? 3 : 4) : 4))) void window_attn_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -872,7 +878,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 // Single tokens over a cache are bound by the reads of K and V: every wave streams its own key tiles through a ring of two stages in LDS, so
 // a compute unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.  Where a row tile sees two key
 // tiles at most (short tracks) a workgroup is one wave and keeps its result in registers: more workgroups fit a compute unit, and there is
-// nothing to join.
+// nothing to join (64 x 8 heads x 13 tokens of 128 channels, fp32: 14 us, latency; 29 with two waves and a join each).  fp32 takes the fp32 matrix
+// instructions: its products are not what binds it, and a tile that is read once need not be split first.
+// Measured: 64 streams of up to 8192 cached keys, 4 heads of 128 channels in bf16, window 4096: 98 us, 5.3 TB/s (a copy reaches 5.2); one stream of
+// 32768, window 16384: 13 us and 4 to join, 2.5 TB/s.
 template <typename T, int DP, bool ONE>
 struct Few {
   using G = Geo<T, DP>;
@@ -1123,6 +1132,8 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
 // Two kernels take S and dP again, each in the orientation that leaves its sums in one wave's registers, so nothing is added by atomics
 // and the order of every sum is fixed: dQ walks the keys of 128 rows (like the forward pass), dK / dV walk the rows that see 32 keys a
 // wave.  The sinks are seen by every later row: their rows beyond the window are cut into shares that run as workgroups of their own.
+// dQ, bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 118 us, 766 TFLOP/s; fp32, 16 x 625 tokens and fewer, 8 heads of 128,
+// window 129: 159 us, where one wave has a SIMD to itself (434 registers: the planes of Q and dO alone are 192) and nothing covers its vector work.
 
 // The gradient of one query row, over the keys it sees alone (see row_again)
 template <typename T>
@@ -1399,8 +1410,8 @@ struct RowWalk {
   static constexpr int N = Planes<T>::N, RS = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
   static constexpr uint32_t PLANE = RS * G16<DP>::PITCH, TILE = N * PLANE, STAT = 2 * TILE, STAGE = 2 * TILE + 1024;
   // At 128 channels two waves share 32 keys, one for dV and one for dK: each has one accumulator, so two waves fit a SIMD where one with both
-  // had it alone, for a quarter more matrix instructions (both take S).  bf16, causal prompts of the benchmark's training case: 241 -> see
-  // the launch.  fp32 then holds its V planes in LDS, 24 KB a wave.
+  // had it alone, for a quarter more matrix instructions (both take S).  bf16, 2 x 4096 tokens, 16 / 4 heads, window 1024: 241 -> 223 us.
+  // fp32 then holds its V planes in LDS, 24 KB a wave: 16 x 625 tokens and fewer, 8 heads, window 129: 298 -> 235 us.
   static constexpr bool TWO = DP == 128, VLDS = TWO && N == 3;
   static constexpr int NW = TWO ? 8 : 4;
   static constexpr uint32_t VF = NSTAGE * STAGE, LDS = VF + (VLDS ? 4 * N * G16<DP>::NC * 1024 : 0);
@@ -1492,6 +1503,9 @@ __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP 
 // dK / dV.  Workgroups from nsink on: 128 keys, 32 keys a wave (or pair of waves), the rows inside the keys' windows.  The first nsink
 // workgroups: the rows beyond the window of 32 KB keys that are sinks, a share of them each; the waves are KB key blocks x row blocks of a
 // stage, and every wave leaves its fp32 sums.  Sinks among the 128 keys leave theirs as share 0.
+// Bound by the LDS reads of its tiles (each of the four products reads one) and the waits at its barriers, at two waves a SIMD: matrix units busy
+// 38 % of the time, LDS 25 %.  bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 230 us, 524 TFLOP/s of what is seen; 8192 tokens, 8
+// heads of 64, window 257: 42 us, 420 TFLOP/s.
 template <typename T, int DP, int OCC>
 __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void window_attn_dkv_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
