@@ -259,6 +259,14 @@ def test_model_refuses_one_wide_head_and_keeps_its_parameters():
     assert list(a.state_dict()) == list(b.state_dict()) and all(torch.equal(x, y) for x, y in zip(a.state_dict().values(), b.state_dict().values()))
 
 
+def test_a_block_takes_windows_and_sinks_beyond_every_length():
+    from trajectorydiffusion_amd import engine
+    rows, out = torch.zeros(1, 6, 3 * 64), torch.zeros(1, 6, 64)
+    for n in (6, 1 << 31, (1 << 32) + 2, 1 << 40):               # (a descriptor counts in 32 bits)
+        d = engine.WindowSpec.check(64, 2, n, n, None).attn_desc(rows, out, None, 1, 6, 64, 0)
+        assert d.left >= 6 and d.right >= 6 and d.sinks >= 6
+
+
 def test_the_reference_statement_itself():
     """The 64-bit statement against a loop over single rows, and its gradients against autograd."""
     g = torch.Generator().manual_seed(0)

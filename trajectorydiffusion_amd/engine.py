@@ -445,7 +445,8 @@ class WindowSpec:
     of tdx_rotary_axes and tdx_window_attention on slices of those rows."""
 
     def __init__(self, heads: int, window: int, sinks: int, rotary: Optional[float]):
-        self.heads, self.window, self.sinks, self.rotary = heads, window, sinks, rotary
+        most = 1 << 28     # beyond every length the kernels take
+        self.heads, self.window, self.sinks, self.rotary = heads, min(window, most), min(sinks, most), rotary
 
     @staticmethod
     def check(Cn: int, heads: int, window: Optional[int], sinks: int, rotary: Optional[float]) -> Optional["WindowSpec"]:
