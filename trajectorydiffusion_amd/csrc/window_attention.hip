@@ -875,19 +875,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 }
 
 // ---- forward, few rows: one 32-row tile per workgroup, its waves (and the splits) share the keys -------------------------------------
-// Single tokens over a cache are bound by the reads of K and V: every wave streams its own key tiles through a ring of two stages in LDS, so
-// a compute unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.  Where a row tile sees two key
+// Single tokens over a cache are bound by the reads of K and V: every wave streams its own key tiles through LDS of its own, so a compute
+// unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.  bf16 has two stages a wave, fp32 one, whose halves
+// are reloaded in turn, which leaves room for four waves at 128 channels too (8 x 4 heads over 8192 keys, window 4096: 75 -> 42 us).  Where a row tile sees two key
 // tiles at most (short tracks) a workgroup is one wave and keeps its result in registers: more workgroups fit a compute unit, and there is
-// nothing to join (64 x 8 heads x 13 tokens of 128 channels, fp32: 14 us, latency; 29 with two waves and a join each).  fp32 takes the fp32 matrix
+// nothing to join (64 x 8 heads x 13 tokens of 128 channels, fp32: 14 us, latency; 29 with two waves that join).  fp32 takes the fp32 matrix
 // instructions: its products are not what binds it, and a tile that is read once need not be split first.
 // Measured: 64 streams of up to 8192 cached keys, 4 heads of 128 channels in bf16, window 4096: 98 us, 5.3 TB/s (a copy reaches 5.2); one stream of
-// 32768, window 16384: 13 us and 4 to join, 2.5 TB/s.
+// 32768, window 16384: 13 to 15 us and 4 to join, 2.4 TB/s.
 template <typename T, int DP, bool ONE>
 struct Few {
   using G = Geo<T, DP>;
   static constexpr int STAGE = 2 * 32 * G::PITCH;                               // 32 keys of K and of V
-  static constexpr int NW = ONE ? 1 : G::PITCH > 256 ? 2 : 4;
-  static constexpr int RING = 2 * STAGE;
+  static constexpr int NW = ONE ? 1 : 4;
+  // fp32 has one stage: K of the next tile is loaded behind the scores and lands under the products with V, and V likewise
+  static constexpr bool HALVES = sizeof(T) == 4;
+  static constexpr int RING = HALVES ? STAGE : 2 * STAGE;
   static constexpr int OPITCH = DP + 4;                                          // floats of a row in the exchange
   static constexpr int XCHG = ONE ? 0 : NW * 32 * (OPITCH + 2) * 4;
   static constexpr int LDS = NW * RING > XCHG ? NW * RING : XCHG;
@@ -925,28 +928,43 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
     const int n = t.na + t.nb, per = (n + a.nsplit - 1) / a.nsplit;
     const int first = split * per + wave, last = min(n, (split + 1) * per);
     const uint32_t ring = lds + wave * F::RING;
-    auto stage = [&](int it, int buf) {
+    constexpr int LOADS = 32 * G::PITCH / 1024;                 // of K or V of a tile
+    auto stage_k = [&](int it, int buf) {
       const int j0 = tile_start(t, it, 32);
-      const uint32_t dst = ring + buf * F::STAGE;
-      stage_rows<T, DP, 32, 1>(dst, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, 0, lane);
-      stage_rows<T, DP, 32, 1>(dst + F::STAGE / 2, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, 0, lane);
+      stage_rows<T, DP, 32, 1>(ring + buf * F::STAGE, (const char*)(kb + (long)j0 * a.k_ts), ks, s.kl - j0, dbytes, 0, lane);
     };
-    if (first < last) stage(first, 0);
+    auto stage_v = [&](int it, int buf) {
+      const int j0 = tile_start(t, it, 32);
+      stage_rows<T, DP, 32, 1>(ring + buf * F::STAGE + F::STAGE / 2, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, 0, lane);
+    };
+    if (first < last) stage_k(first, 0), stage_v(first, 0);
     arrived(qf);               // from here on only direct loads are counted
     int buf = 0;
-    for (int it = first; it < last; it += F::NW, buf ^= 1) {
-      if (it + F::NW < last) {
-        stage(it + F::NW, buf ^ 1);
-        wait_vm<2 * 32 * G::PITCH / 1024>();
+    for (int it = first; it < last; it += F::NW, buf ^= !F::HALVES) {
+      const bool more = it + F::NW < last;
+      if constexpr (F::HALVES) {
+        wait_vm<LOADS>();                                       // K is there
+      } else if (more) {
+        stage_k(it + F::NW, buf ^ 1), stage_v(it + F::NW, buf ^ 1);
+        wait_vm<2 * LOADS>();
       } else {
         wait_vm<0>();
       }
       const int j0 = tile_start(t, it, 32);
       const uint32_t kt = ring + buf * F::STAGE, vt = kt + F::STAGE / 2;
       const int cls = seen_class(a, s, j0, p0, p1);
+      f32x16 acc;
+      if (cls) rows_times<T, DP>(acc, kt, 0, qf, lane);
+      if constexpr (F::HALVES) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // K has been read
+        if (more) {
+          stage_k(it + F::NW, 0);
+          wait_vm<LOADS>();                                     // V is there
+        } else {
+          wait_vm<0>();
+        }
+      }
       if (cls) {
-        f32x16 acc;
-        rows_times<T, DP>(acc, kt, 0, qf, lane);
         float sc[1][16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[0][e] = acc[e];
@@ -956,7 +974,8 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
         softmax_exp<0, 16>(sc[0], l, mc, c);
         cols_times<DP>(o, vt, 0, sc[0], lane, T());
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage has been read before the ring comes round to it
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage (fp32: V) has been read before the ring comes round to it
+      if (F::HALVES && more) stage_v(it + F::NW, 0);
     }
     l = half_sum(l);
   }
@@ -1770,24 +1789,38 @@ struct Plan {
 };
 constexpr int64_t kMostThreads = 0xffffffffLL;   // a launch counts its threads in 32 bits
 constexpr int kMostSplits = 64;       // (the join kernel holds a row's shares in registers)
-Plan plan_forward(const WaArgs& a) {
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+template <typename T>
+int few_per_unit(int dp) {              // workgroups of the few-row kernel that fit a compute unit: 160 KB of LDS, 2 waves a SIMD at least below 128 channels
+  const int lds = dp == 32 ? Few<T, 32, false>::LDS : dp == 64 ? Few<T, 64, false>::LDS : Few<T, 128, false>::LDS;
+  return std::max(1, std::min(160 * 1024 / lds, dp == 128 ? 1 : 2));
+}
+int few_per_unit(int es, int dp) { return es == 4 ? few_per_unit<float>(dp) : few_per_unit<__bf16>(dp); }
+Plan plan_forward(const WaArgs& a, int es) {
   Plan p{};
   const long rows = (long)a.Tq * a.G, bh = (long)a.B * a.Hkv;
   p.few = rows <= 32 || bh * ((rows + 127) / 128) < compute_units();
   p.ntiles = (int)((rows + (p.few ? 31 : 127)) / (p.few ? 32 : 128));
   p.nsplit = 1;
   if (p.few) {
-    // key tiles a row tile sees at most; splits until every compute unit has two workgroups, of 8 key tiles at least
+    // key tiles a row tile sees at most
     const long span = a.left == kFar ? a.Tk : std::min<long>(a.Tk, (long)a.left + 32 / a.G + 1 + (a.right == kFar ? a.Tk : a.right) + a.sinks);
     const long tiles = (span + 31) / 32, wgs = bh * p.ntiles;
-    const long want = (2 * (long)compute_units() + wgs - 1) / wgs;
-    p.nsplit = (int)std::max<long>(1, std::min<long>(std::min<long>(want, tiles / 8), kMostSplits));
     p.one = tiles <= 2;
+    // Splits of the keys: the rounds of workgroups over the chip, of so many tiles a wave and two tiles' time to begin with, then the join (one
+    // workgroup a row), in tiles' times.  Measured, fp32, 8 heads of 128 channels, one token: 300 keys 36 -> 16 us with 5 splits, 4096 keys 33 -> 17
+    // with 32 and 27 with 64; bf16, 16 x 8 heads, 512 keys: 13 with 2, 18 with 4; 1000 tokens, 8 heads, window 257: 11 alone, 21 with a join.
+    const long most = std::min<long>(kMostSplits, tiles), fit = (long)compute_units() * few_per_unit(es, padded(a.D));
+    const double join = (2.5 + bh * rows / 1700.) * (es == 4 ? 0.5 : 1);   // (an fp32 tile takes twice as long)
+    double best = 0;
+    for (long n = 1; n <= most && !p.one; ++n) {
+      const double cost = (double)((wgs * n + fit - 1) / fit) * ((tiles + 4 * n - 1) / (4 * n) + 2) + (n > 1 ? join : 0);
+      if (n == 1 || cost < best) best = cost, p.nsplit = (int)n;
+    }
   }
   p.threads = bh * std::max<int64_t>((int64_t)p.ntiles * p.nsplit * (p.one ? 64 : 256), p.nsplit > 1 ? rows * 256 : 0);
   return p;
 }
-int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 template <typename K>
 int reserve_lds(K kernel, size_t bytes, bool& done) {
@@ -1891,7 +1924,7 @@ int launch_backward_d(WaArgs& a, const BwdPlan& p, hipStream_t st) {
 extern "C" int64_t tdx_window_attention_ws_bytes(const tdx_window_attn_desc* d) {
   WaArgs a;
   if (translate(d, a, "tdx_window_attention_ws_bytes") != TDX_OK || a.B == 0 || a.Tq == 0) return 0;
-  const Plan p = plan_forward(a);
+  const Plan p = plan_forward(a, d->dtype == TDX_F32 ? 4 : 2);
   return p.nsplit > 1 ? (int64_t)a.B * a.Hkv * p.ntiles * p.nsplit * 32 * (padded(a.D) + 2) * 4 : 0;
 }
 
@@ -1899,7 +1932,7 @@ extern "C" int tdx_window_attention(const tdx_window_attn_desc* d, void* stream)
   WaArgs a;
   if (const int rc = translate(d, a, "tdx_window_attention")) return rc;
   if (a.B == 0 || a.Tq == 0) return TDX_OK;
-  const Plan p = plan_forward(a);
+  const Plan p = plan_forward(a, d->dtype == TDX_F32 ? 4 : 2);
   const int64_t need = p.nsplit > 1 ? (int64_t)a.B * a.Hkv * p.ntiles * p.nsplit * 32 * (padded(a.D) + 2) * 4 : 0;
   TDX_CHECK_ARG(need == 0 || (pointer_ok(d->ws) && d->ws_bytes >= need), "tdx_window_attention: workspace of %lld bytes needed, got %lld", (long long)need, (long long)d->ws_bytes);
   TDX_CHECK_ARG((long)a.B * a.Hkv * a.Tq * a.G < 0x7fffffffL && p.threads <= kMostThreads, "tdx_window_attention: too many rows");
