@@ -155,6 +155,8 @@ CASES = [  # B, Tq, Tk, Hq, Hkv, D, left, right, sinks, q_lens, k_lens
     (70, 150, 150, 4, 2, 64, 50, 10, 5, "ragged", "ragged"),        # enough workgroups for the many-row kernel
     (40, 140, 140, 8, 8, 128, 70, 0, 40, "ragged", "ragged"),
     (300, 130, 170, 1, 1, 32, 33, 20, 5, None, "ragged"),
+    (1, 700, 700, 8, 1, 128, None, 0, 0, None, None),               # few keys, many rows: the rows of a key tile are cut into shares
+    (2, 520, 600, 12, 2, 48, 200, None, 3, [520, 77], [600, 300]),
 ]
 
 

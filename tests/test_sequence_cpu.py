@@ -232,7 +232,8 @@ def test_c_attention_workspaces():
     a = int(lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(Tq=1000, Tk=1000, sinks=0))))
     b = int(lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(Tq=1000, Tk=1000, sinks=7))))
     assert b > a > 0
-    # sinks or windows that hold every key are no window at all
+    # sinks or windows that hold every key are no window at all (the rows that see a key, and so its shares, depend on the window)
+    a = int(lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(Tq=1000, Tk=1000, left=-1, sinks=0))))
     assert int(lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(Tq=1000, Tk=1000, sinks=1000)))) == a
     assert int(lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(Tq=1000, Tk=1000, sinks=7, left=1000)))) == a
 

@@ -47,8 +47,9 @@ struct WaArgs {
   const void* dout;
   void *dq, *dk, *dv;
   long do_bs, do_ts, do_hs, dq_bs, dq_ts, dq_hs, dk_bs, dk_ts, dk_hs, dv_bs, dv_ts, dv_hs;
-  float *stat, *part;                 // per 32 rows {log2-sum-exp, delta}; shares of the sinks' gradients
+  float *stat, *part, *near;          // per 32 rows {log2-sum-exp, delta}; shares of the sinks' gradients; of all keys' (nrow > 1)
   int ntiles32, nparts, sink_rows;    // row tiles of 32; shares; sinks rounded up to 32 (0: no separate pass over the sinks)
+  int nrow;                           // shares that the rows of a key tile are cut into
 };
 
 // ---- geometry of a staged tile ------------------------------------------------------------------------------------------------
@@ -1521,7 +1522,8 @@ __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP 
 
 // dK / dV.  Workgroups from nsink on: 128 keys, 32 keys a wave (or pair of waves), the rows inside the keys' windows.  The first nsink
 // workgroups: the rows beyond the window of 32 KB keys that are sinks, a share of them each; the waves are KB key blocks x row blocks of a
-// stage, and every wave leaves its fp32 sums.  Sinks among the 128 keys leave theirs as share 0.
+// stage, and every wave leaves its fp32 sums.  Sinks among the 128 keys leave theirs as the first shares.  Where the keys are too few to fill the chip
+// (grouped heads, small batches), the rows of 128 keys are cut into nrow shares too.
 // Bound by the LDS reads of its tiles (each of the four products reads one) and the waits at its barriers, at two waves a SIMD: matrix units busy
 // 38 % of the time, LDS 25 %.  bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 230 us, 524 TFLOP/s of what is seen; 8192 tokens, 8
 // heads of 64, window 257: 42 us, 420 TFLOP/s.
@@ -1536,16 +1538,17 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
   const int nst = (a.sink_rows / 32 + KB - 1) / KB;                      // sink tiles of a (batch, key head)
   const int nsink = a.B * a.Hkv * nst * a.nsplit;
   const bool far = (int)blockIdx.x < nsink;
-  int bh, jw, split = 0;
+  int bh, jw, split = 0;                                                  // (near: of nrow shares of the rows)
   if (far) {
     const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, nst * a.nsplit);
     split = item.at % a.nsplit;
     bh = item.bh;
     jw = (item.at / a.nsplit) * KB * 32 + (kw % KB) * 32;
   } else {
-    const Item item = xcd_item(blockIdx.x - nsink, a.B * a.Hkv, a.ntiles);
+    const Item item = xcd_item(blockIdx.x - nsink, a.B * a.Hkv, a.ntiles * a.nrow);
+    split = item.at % a.nrow;
     bh = item.bh;
-    jw = item.at * 128 + kw * 32;
+    jw = (item.at / a.nrow) * 128 + kw * 32;
   }
   const int hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
@@ -1569,11 +1572,9 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
       for (int e = 0; e < 16; ++e) dk[d][e] = 0.f, dv[d][e] = 0.f;
     if (block_first <= block_last) {
       int t0 = lo(block_first) * a.G / W::RS, t1 = (hi(block_last) * a.G + W::RS - 1) / W::RS;
-      if (far) {
-        const int per = (max(0, t1 - t0) + a.nsplit - 1) / a.nsplit;
-        t0 += split * per;
-        t1 = min(t1, t0 + per);
-      }
+      const int shares = far ? a.nsplit : a.nrow, per = (max(0, t1 - t0) + shares - 1) / shares;
+      t0 += split * per;
+      t1 = min(t1, t0 + per);
       const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
       const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
       const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
@@ -1645,9 +1646,11 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
       }
     }
     bool bad_k = false, bad_v = false;
-    if (far || j < a.sinks) {
-      if (j < a.sink_rows) {
-        float* part = a.part + (((long)bh * a.nparts + (far ? 1 + split * NB + kw / KB : 0)) * a.sink_rows + j) * 2 * DP;
+    const bool sink = far || j < a.sinks;
+    if (sink || a.nrow > 1) {
+      if (sink ? j < a.sink_rows : j < a.Tk) {
+        float* part = sink ? a.part + (((long)bh * a.nparts + (far ? a.nrow + split * NB + kw / KB : split)) * a.sink_rows + j) * 2 * DP
+                           : a.near + (((long)bh * a.nrow + split) * a.Tk + j) * 2 * DP;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1695,35 +1698,50 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
 #endif
 }
 
-// The sinks' shares, in order: one workgroup a key row, its 4 waves take the shares in turn
+// The shares, in order: one workgroup a sink, its 4 waves take the shares in turn; then (nrow > 1) one wave a key
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void window_attn_dkv_join_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int PER = 2 * DP / 64;
   __shared__ float share[4][2 * DP];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nk = min(a.sinks, a.Tk);
-  const int j = blockIdx.x % nk, bh = blockIdx.x / nk, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nk = min(a.sinks, a.Tk), per = nk + (a.nrow > 1 ? (a.Tk - nk + 3) / 4 : 0);
+  const int at0 = blockIdx.x % per, bh = blockIdx.x / per, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
+  const bool sink = at0 < nk;
+  const int j = sink ? at0 : nk + 4 * (at0 - nk) + wave;
   float sum[PER];
 #pragma unroll
   for (int x = 0; x < PER; ++x) sum[x] = 0.f;
-  const float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP + lane;
+  if (sink) {
+    const float* part = a.part + ((long)bh * a.nparts * a.sink_rows + j) * 2 * DP + lane;
 #pragma unroll 4
-  for (int n = wave; n < a.nparts; n += 4)
+    for (int n = wave; n < a.nparts; n += 4)
 #pragma unroll
-    for (int x = 0; x < PER; ++x) sum[x] += part[(long)n * a.sink_rows * 2 * DP + 64 * x];
+      for (int x = 0; x < PER; ++x) sum[x] += part[(long)n * a.sink_rows * 2 * DP + 64 * x];
 #pragma unroll
-  for (int x = 0; x < PER; ++x) share[wave][64 * x + lane] = sum[x];
-  __syncthreads();
-  if (wave) return;
+    for (int x = 0; x < PER; ++x) share[wave][64 * x + lane] = sum[x];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+      const int at = 64 * x + lane;
+      sum[x] = (share[0][at] + share[1][at]) + (share[2][at] + share[3][at]);
+    }
+  } else {
+    if (j >= a.Tk) return;
+    const float* part = a.near + ((long)bh * a.nrow * a.Tk + j) * 2 * DP + lane;
+#pragma unroll 4
+    for (int n = 0; n < a.nrow; ++n)
+#pragma unroll
+      for (int x = 0; x < PER; ++x) sum[x] += part[(long)n * a.Tk * 2 * DP + 64 * x];
+  }
   bool bad = false;
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
     const int at = 64 * x + lane, d = at % DP;
     const bool isk = at < DP;
-    const float t = (share[0][at] + share[1][at]) + (share[2][at] + share[3][at]);
-    const float v = j < s.kl ? (isk ? t * a.scale : t) : 0.f;
+    const float v = j < s.kl ? (isk ? sum[x] * a.scale : sum[x]) : 0.f;
     T* row = isk ? (T*)a.dk + b * a.dk_bs + (long)j * a.dk_ts + hk * a.dk_hs : (T*)a.dv + b * a.dv_bs + (long)j * a.dv_ts + hk * a.dv_hs;
     if (d < a.D) {
       row[d] = (T)v;
@@ -1866,15 +1884,33 @@ int launch_forward_d(WaArgs& a, const Plan& p, hipStream_t st) {
   }
 }
 
-// Backward: bytes of the row statistics, and of the sinks' shares
+// Backward: bytes of the row statistics, of the sinks' shares and of all keys'
 struct BwdPlan {
-  int sink_rows, nsplit, nparts;
-  int64_t stat_bytes, part_bytes, threads;
+  int sink_rows, nsplit, nparts, nrow;
+  int64_t stat_bytes, part_bytes, near_bytes, threads;
+  int64_t bytes() const { return stat_bytes + part_bytes + near_bytes; }
 };
 BwdPlan plan_backward(const WaArgs& a, int es) {
   BwdPlan p{};
   const int64_t rows = (int64_t)a.Tq * a.G, bh = (int64_t)a.B * a.Hkv, dp = padded(a.D);
   p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
+  const int64_t keys = ((int64_t)a.Tk + 127) / 128;
+  {
+    // Shares of the rows: the rounds of workgroups over the chip, of so many stages and two stages' time to begin with, then the join, in stages'
+    // times (2 us, fp32 4; the join 4 us and its bytes twice at 4 TB/s).  bf16, 4096 tokens, 8 / 1 heads of 128 channels, causal (32 workgroups
+    // without shares): 1112 -> 173 us and 7 to join; 4 x 955, 16 / 4 heads of 64 (128 workgroups): 148 -> 51 and 8; fp32, 2048, 8 / 1 heads of 64,
+    // causal (16 workgroups): 2029 -> 123 and 7.
+    const int64_t seen = a.left == kFar || a.right == kFar ? a.Tq : std::min<int64_t>(a.Tq, (int64_t)a.left + a.right + 128);
+    const int64_t stages = (seen * a.G + (es == 4 ? 31 : 63)) / (es == 4 ? 32 : 64), wgs = bh * keys, fit = (int64_t)compute_units() * (dp == 128 ? 1 : 2);
+    double best = 0;
+    p.nrow = 1;
+    for (int64_t n = 1; n <= std::min<int64_t>(64, stages) && a.Tk > 0; ++n) {
+      const double join = n > 1 ? (2 + (double)(bh * n * a.Tk) * dp * 2 * 4 * 2 / 8e6) * (es == 4 ? 0.5 : 1) : 0;
+      const double cost = (double)((wgs * n + fit - 1) / fit) * ((stages + n - 1) / n + 2) + join;
+      if (n == 1 || cost < best) best = cost, p.nrow = (int)n;
+    }
+    if (p.nrow > 1) p.near_bytes = bh * p.nrow * a.Tk * 2 * dp * 4;
+  }
   int64_t sink_wgs = 0;
   if (a.sinks > 0) {
     const int nb = es == 4 ? 1 : 2, kb = 4 / nb;                        // row and key blocks of a workgroup (RowWalk)
@@ -1882,12 +1918,11 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
     const int64_t wgs = bh * ((p.sink_rows / 32 + kb - 1) / kb);
     // one workgroup a compute unit, 8 stages each at least
     p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((compute_units() + wgs - 1) / wgs, rows / (nb * 32 * 8)));
-    p.nparts = 1 + p.nsplit * nb;
+    p.nparts = p.nrow + p.nsplit * nb;
     p.part_bytes = bh * p.nparts * p.sink_rows * 2 * dp * 4;
     sink_wgs = wgs * p.nsplit;
   }
-  const int64_t keys = ((int64_t)a.Tk + 127) / 128;
-  p.threads = std::max({bh * ((rows + 127) / 128) * 256, (sink_wgs + bh * keys) * (dp == 128 ? 512 : 256), bh * std::min(a.sinks, a.Tk) * 256});
+  p.threads = std::max({bh * ((rows + 127) / 128) * 256, (sink_wgs + bh * keys * p.nrow) * (dp == 128 ? 512 : 256), bh * (std::min(a.sinks, a.Tk) + (p.nrow > 1 ? (a.Tk + 3) / 4 : 0)) * 256});
   return p;
 }
 
@@ -1896,16 +1931,17 @@ int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
   const long bh = (long)a.B * a.Hkv;
   constexpr int OCC = 2, OCC_Q = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : (DP == 128 ? 2 : DP == 64 ? 3 : 4), KB = 4 / (RowWalk<T, DP>::RS / 32);
   const long rt = ((long)a.Tq * a.G + 127) / 128;
-  a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows;
+  a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows, a.nrow = p.nrow;
   WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC_Q>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dq_kernel");
   if (a.Tk == 0) return TDX_OK;
   a.ntiles = (a.Tk + 127) / 128;
   const long sink_wgs = bh * ((p.sink_rows / 32 + KB - 1) / KB) * p.nsplit;
-  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), sink_wgs + bh * a.ntiles, (RowWalk<T, DP>::NW * 64), (RowWalk<T, DP>::LDS), st, a);
+  WA_LAUNCH((window_attn_dkv_kernel<T, DP, OCC>), sink_wgs + bh * a.ntiles * a.nrow, (RowWalk<T, DP>::NW * 64), (RowWalk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dkv_kernel");
-  if (p.sink_rows) {
-    hipLaunchKernelGGL((window_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(bh * std::min(a.sinks, a.Tk))), dim3(256), 0, st, a);
+  if (p.sink_rows || p.nrow > 1) {
+    const int nk = std::min(a.sinks, a.Tk);
+    hipLaunchKernelGGL((window_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(bh * (nk + (p.nrow > 1 ? (a.Tk - nk + 3) / 4 : 0)))), dim3(256), 0, st, a);
     TDX_CHECK_LAUNCH("window_attn_dkv_join_kernel");
   }
   return TDX_OK;
@@ -1944,7 +1980,7 @@ extern "C" int64_t tdx_window_attention_bwd_ws_bytes(const tdx_window_attn_desc*
   WaArgs a;
   if (translate(d, a, "tdx_window_attention_bwd_ws_bytes") != TDX_OK || a.B == 0 || a.Tq == 0) return 0;
   const BwdPlan p = plan_backward(a, d->dtype == TDX_F32 ? 4 : 2);
-  return p.stat_bytes + p.part_bytes;
+  return p.bytes();
 }
 
 extern "C" int tdx_window_attention_bwd(const tdx_window_attn_desc* d, void* stream) {
@@ -1959,12 +1995,12 @@ extern "C" int tdx_window_attention_bwd(const tdx_window_attn_desc* d, void* str
                     strides_ok(d->dv_bs, d->dv_ts, d->dv_hs, es), "tdx_window_attention_bwd: strides must be multiples of 16 bytes and not negative");
   TDX_CHECK_ARG((65 * d->dout_ts + a.G * d->dout_hs) * es < (1ll << 31), "tdx_window_attention_bwd: the strides of dout are too large");
   const BwdPlan p = plan_backward(a, es);
-  TDX_CHECK_ARG(pointer_ok(d->ws) && d->ws_bytes >= p.stat_bytes + p.part_bytes, "tdx_window_attention_bwd: workspace of %lld bytes needed, got %lld",
-                (long long)(p.stat_bytes + p.part_bytes), (long long)d->ws_bytes);
+  TDX_CHECK_ARG(pointer_ok(d->ws) && d->ws_bytes >= p.bytes(), "tdx_window_attention_bwd: workspace of %lld bytes needed, got %lld",
+                (long long)p.bytes(), (long long)d->ws_bytes);
   TDX_CHECK_ARG((long)a.B * a.Hkv * std::max<long>((long)a.Tq * a.G, a.Tk) < 0x7fffffffL && p.threads <= kMostThreads, "tdx_window_attention_bwd: too many rows");
   a.dout = d->dout, a.dq = d->dq, a.dk = d->dk, a.dv = d->dv;
   a.do_bs = d->dout_bs, a.do_ts = d->dout_ts, a.do_hs = d->dout_hs, a.dq_bs = d->dq_bs, a.dq_ts = d->dq_ts, a.dq_hs = d->dq_hs;
   a.dk_bs = d->dk_bs, a.dk_ts = d->dk_ts, a.dk_hs = d->dk_hs, a.dv_bs = d->dv_bs, a.dv_ts = d->dv_ts, a.dv_hs = d->dv_hs;
-  a.stat = (float*)d->ws, a.part = (float*)((char*)d->ws + p.stat_bytes);
+  a.stat = (float*)d->ws, a.part = (float*)((char*)d->ws + p.stat_bytes), a.near = a.part + p.part_bytes / 4;
   return d->dtype == TDX_F32 ? launch_backward_d<float>(a, p, (hipStream_t)stream) : launch_backward_d<__bf16>(a, p, (hipStream_t)stream);
 }
