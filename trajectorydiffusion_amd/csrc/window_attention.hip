@@ -47,9 +47,9 @@ struct WaArgs {
   const void* dout;
   void *dq, *dk, *dv;
   long do_bs, do_ts, do_hs, dq_bs, dq_ts, dq_hs, dk_bs, dk_ts, dk_hs, dv_bs, dv_ts, dv_hs;
-  float *stat, *part, *near;          // per 32 rows {log2-sum-exp, delta}; shares of the sinks' gradients; of all keys' (nrow > 1)
+  float *stat, *part, *near;          // per 32 rows {log2-sum-exp, delta}; shares of the sinks' gradients; of all rows' (nkey > 1), then of all keys' (nrow > 1)
   int ntiles32, nparts, sink_rows;    // row tiles of 32; shares; sinks rounded up to 32 (0: no separate pass over the sinks)
-  int nrow;                           // shares that the rows of a key tile are cut into
+  int nrow, nkey;                     // shares that the rows of a key tile (dK / dV) and the keys of a row tile (dQ) are cut into
 };
 
 // ---- geometry of a staged tile ------------------------------------------------------------------------------------------------
@@ -709,26 +709,25 @@ struct Walk {
   static constexpr int N = Planes<T>::N, BN = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
   static constexpr uint32_t PLANE = BN * G16<DP>::PITCH, TILE = N * PLANE, STAGE = 2 * TILE, RAW = N == 1 ? 0 : BN * DP * 4, LDS = NSTAGE * STAGE + 2 * RAW;
 };
-// Calls f(key, offset of the stage in LDS as a type) for each key tile of `t`, staged
+// Calls f(key, offset of the stage in LDS as a type) for the key tiles [first, n) of `t`, staged
 // (ready() is called once the first tile's loads are on their way)
 template <typename T, int DP, typename R, typename F>
-__device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const Tiles& t, const T* kb, const T* vb, uint32_t lds, int wave, int lane, R&& ready,
+__device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const Tiles& t, int first, int n, const T* kb, const T* vb, uint32_t lds, int wave, int lane, R&& ready,
                                           F&& f) {
   using W = Walk<T, DP>;
   constexpr int ES = sizeof(T);
   Stager<T, DP, W::BN> sk, sv;
   sk.init(a.k_ts * ES, a.D * ES, wave, lane);
   sv.init(a.v_ts * ES, a.D * ES, wave, lane);
-  const int n = t.na + t.nb;
   auto load = [&](int it, uint32_t at) {
     const int j0 = tile_start(t, it, W::BN);
     sk.load(at, (const char*)(kb + (long)j0 * a.k_ts), s.kl - j0, wave);
     sv.load(at + (W::N == 1 ? W::TILE : W::RAW), (const char*)(vb + (long)j0 * a.v_ts), s.kl - j0, wave);
   };
-  if (n > 0) load(0, W::N == 1 ? lds : lds + W::STAGE);
+  if (first < n) load(first, W::N == 1 ? lds : lds + W::STAGE);
   ready();
   if constexpr (W::N == 1) {
-    for (int it = 0; it < n; it += 2) {
+    for (int it = first; it < n; it += 2) {
       wait_vm<0>();
       wg_barrier();
       if (it + 1 < n) load(it + 1, lds + W::STAGE);
@@ -740,7 +739,7 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
       f(tile_start(t, it + 1, W::BN), std::integral_constant<uint32_t, W::STAGE>());
     }
   } else {
-    for (int it = 0; it < n; ++it) {
+    for (int it = first; it < n; ++it) {
       wait_vm<0>();
       wg_barrier();                    // the numbers are there, the planes of the tile before have been read
       sk.put(lds, lds + W::STAGE);
@@ -788,7 +787,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
     const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;   // positions of this wave's rows
     const bool wave_ok = rw < rend;
     const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, W::BN);
-    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&] { arrived16(qf); },
+    walk_keys<T, DP>(a, s, t, 0, t.na + t.nb, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, [&] { arrived16(qf); },
                      [&](int j0, auto st) {
       // a tile is taken whole: with a path of its own for a half the accumulators would be copied where the paths meet
       constexpr uint32_t S0 = decltype(st)::value;
@@ -1194,8 +1193,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, a.ntiles);
-  const int tile = item.at, bh = item.bh, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Item item = xcd_item(blockIdx.x, a.B * a.Hkv, a.ntiles * a.nkey);
+  const int tile = item.at / a.nkey, share = item.at % a.nkey, bh = item.bh, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Seq s = seq_of(a, b);
   const int R = a.Tq * a.G, r0 = tile * 128, rw = r0 + wave * 32;
   const int rend = min(r0 + 128, s.ql * a.G);
@@ -1292,14 +1291,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
       pack16<N>(db, sc);
       cols16<N, DP, A, W::PLANE>(dq, off, db);
     };
-    walk_keys<T, DP>(a, s, t, (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, rows_ready,
+    const int n = t.na + t.nb, per = (n + a.nkey - 1) / a.nkey;
+    walk_keys<T, DP>(a, s, t, share * per, min(n, (share + 1) * per), (const T*)a.k + b * a.k_bs + hk * a.k_hs, (const T*)a.v + b * a.v_bs + hk * a.v_hs, lds, wave, lane, rows_ready,
                      [&](int j0, auto st) {
       constexpr uint32_t S0 = decltype(st)::value;
       one(j0, std::integral_constant<uint32_t, S0>());
       if constexpr (W::BN == 64) one(j0 + 32, std::integral_constant<uint32_t, S0 + 32 * G16<DP>::PITCH>());
     });
   }
-  a.stat[((long)bh * a.ntiles32 + tile * 4 + wave) * 64 + lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
+  if (share == 0) a.stat[((long)bh * a.ntiles32 + tile * 4 + wave) * 64 + lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
+  if (a.nkey > 1) {
+    if (r < R) {
+      float* part = a.near + (((long)bh * a.nkey + share) * R + r) * DP + 4 * (lane >> 5);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4*>(part + 32 * d + 8 * e) = (f32x4){dq[d][4 * e], dq[d][4 * e + 1], dq[d][4 * e + 2], dq[d][4 * e + 3]};
+    }
+    return;
+  }
   bool bad = false;
   if (r < R) {
     T* qrow = (T*)a.dq + b * a.dq_bs + (long)i * a.dq_ts + hq * a.dq_hs;
@@ -1324,6 +1334,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
     again &= again - 1;
     dq_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(lse2, n, 64), __shfl(delta, n, 64), lane);
   }
+#endif
+}
+
+// The shares of dQ (nkey > 1), in order: one wave a row
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void window_attn_dq_join_kernel(const WaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int R = a.Tq * a.G, per = (R + 3) / 4;
+  const int r = 4 * (int)(blockIdx.x % per) + wave, bh = blockIdx.x / per, hk = bh % a.Hkv, b = bh / a.Hkv;
+  if (r >= R) return;
+  const Seq s = seq_of(a, b);
+  const int i = r / a.G, g = r - i * a.G;
+  float sum[2] = {0.f, 0.f};
+  const float* part = a.near + ((long)bh * a.nkey * R + r) * DP + lane;
+#pragma unroll 4
+  for (int n = 0; n < a.nkey; ++n)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (64 * x + lane < DP) sum[x] += part[(long)n * R * DP + 64 * x];
+  T* row = (T*)a.dq + b * a.dq_bs + (long)i * a.dq_ts + (long)(hk * a.G + g) * a.dq_hs;
+  bool bad = false;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const float v = i < s.ql ? sum[x] * a.scale : 0.f;
+    if (64 * x + lane < a.D) {
+      row[64 * x + lane] = (T)v;
+      bad |= v != v;
+    }
+  }
+  const float* stat = a.stat + ((long)bh * a.ntiles32 + (r >> 5)) * 64 + (r & 31);
+  const float lse2 = stat[0], delta = stat[32];
+  if (__ballot(bad) && lse2 == lse2 && delta == delta) dq_again<T>(a, s, b, hk, i, g, lse2, delta, lane);
 #endif
 }
 
@@ -1886,31 +1929,38 @@ int launch_forward_d(WaArgs& a, const Plan& p, hipStream_t st) {
 
 // Backward: bytes of the row statistics, of the sinks' shares and of all keys'
 struct BwdPlan {
-  int sink_rows, nsplit, nparts, nrow;
+  int sink_rows, nsplit, nparts, nrow, nkey;
   int64_t stat_bytes, part_bytes, near_bytes, threads;
   int64_t bytes() const { return stat_bytes + part_bytes + near_bytes; }
 };
+// Into how many shares `wgs` workgroups of `stages` stages are cut: the rounds over the chip, of so many stages and two stages' time to begin with,
+// then the join, in stages' times (2 us, fp32 4; the join 4 us and its `bytes` a share twice at 4 TB/s).  A compute unit counts for two workgroups
+// below 128 channels, for one there (dQ with two beside each other: 110 -> 97 us, and 13 to join).
+int shares(int64_t wgs, int64_t stages, int64_t dp, int64_t bytes, int es) {
+  const int64_t chip = (int64_t)compute_units() * (dp == 128 ? 1 : 2);
+  double best = 0;
+  int best_n = 1;
+  for (int64_t n = 1; n <= std::min<int64_t>(64, stages); ++n) {
+    const double join = n > 1 ? (2 + (double)(n * bytes) * 2 / 8e6) * (es == 4 ? 0.5 : 1) : 0;
+    const double cost = (double)((wgs * n + chip - 1) / chip) * ((stages + n - 1) / n + 2) + join;
+    if (n == 1 || cost < best) best = cost, best_n = (int)n;
+  }
+  return best_n;
+}
 BwdPlan plan_backward(const WaArgs& a, int es) {
   BwdPlan p{};
   const int64_t rows = (int64_t)a.Tq * a.G, bh = (int64_t)a.B * a.Hkv, dp = padded(a.D);
   p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
-  const int64_t keys = ((int64_t)a.Tk + 127) / 128;
-  {
-    // Shares of the rows: the rounds of workgroups over the chip, of so many stages and two stages' time to begin with, then the join, in stages'
-    // times (2 us, fp32 4; the join 4 us and its bytes twice at 4 TB/s).  bf16, 4096 tokens, 8 / 1 heads of 128 channels, causal (32 workgroups
-    // without shares): 1112 -> 173 us and 7 to join; 4 x 955, 16 / 4 heads of 64 (128 workgroups): 148 -> 51 and 8; fp32, 2048, 8 / 1 heads of 64,
-    // causal (16 workgroups): 2029 -> 123 and 7.
-    const int64_t seen = a.left == kFar || a.right == kFar ? a.Tq : std::min<int64_t>(a.Tq, (int64_t)a.left + a.right + 128);
-    const int64_t stages = (seen * a.G + (es == 4 ? 31 : 63)) / (es == 4 ? 32 : 64), wgs = bh * keys, fit = (int64_t)compute_units() * (dp == 128 ? 1 : 2);
-    double best = 0;
-    p.nrow = 1;
-    for (int64_t n = 1; n <= std::min<int64_t>(64, stages) && a.Tk > 0; ++n) {
-      const double join = n > 1 ? (2 + (double)(bh * n * a.Tk) * dp * 2 * 4 * 2 / 8e6) * (es == 4 ? 0.5 : 1) : 0;
-      const double cost = (double)((wgs * n + fit - 1) / fit) * ((stages + n - 1) / n + 2) + join;
-      if (n == 1 || cost < best) best = cost, p.nrow = (int)n;
-    }
-    if (p.nrow > 1) p.near_bytes = bh * p.nrow * a.Tk * 2 * dp * 4;
-  }
+  const int64_t keys = ((int64_t)a.Tk + 127) / 128, tiles = (rows + 127) / 128;
+  // dK / dV, bf16, 4096 tokens, 8 / 1 heads of 128 channels, causal (32 workgroups without shares): 1112 -> 173 us and 7 to join; 4 x 955, 16 / 4 heads
+  // of 64 (128 workgroups): 148 -> 51 and 8; fp32, 2048, 8 / 1 heads of 64, causal (16 workgroups): 2029 -> 123 and 7.  dQ of the last (128
+  // workgroups): 149 -> 65 and 7.
+  const int64_t seen = a.left == kFar || a.right == kFar ? a.Tq : std::min<int64_t>(a.Tq, (int64_t)a.left + a.right + 128);
+  p.nrow = shares(bh * keys, (seen * a.G + (es == 4 ? 31 : 63)) / (es == 4 ? 32 : 64), dp, bh * a.Tk * dp * 2 * 4, es);
+  const int64_t span = a.left == kFar || a.right == kFar ? a.Tk : std::min<int64_t>(a.Tk, (int64_t)a.left + a.right + 128 / a.G + a.sinks);
+  p.nkey = shares(bh * tiles, (span + (es == 4 ? 31 : 63)) / (es == 4 ? 32 : 64), dp, bh * rows * dp * 4, es);
+  // one after the other, the two need the same memory
+  p.near_bytes = std::max(p.nrow > 1 ? bh * p.nrow * a.Tk * 2 * dp * 4 : 0, p.nkey > 1 ? bh * p.nkey * rows * dp * 4 : 0);
   int64_t sink_wgs = 0;
   if (a.sinks > 0) {
     const int nb = es == 4 ? 1 : 2, kb = 4 / nb;                        // row and key blocks of a workgroup (RowWalk)
@@ -1922,7 +1972,7 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
     p.part_bytes = bh * p.nparts * p.sink_rows * 2 * dp * 4;
     sink_wgs = wgs * p.nsplit;
   }
-  p.threads = std::max({bh * ((rows + 127) / 128) * 256, (sink_wgs + bh * keys * p.nrow) * (dp == 128 ? 512 : 256), bh * (std::min(a.sinks, a.Tk) + (p.nrow > 1 ? (a.Tk + 3) / 4 : 0)) * 256});
+  p.threads = std::max({bh * tiles * p.nkey * 256, p.nkey > 1 ? bh * ((rows + 3) / 4) * 256 : 0, (sink_wgs + bh * keys * p.nrow) * (dp == 128 ? 512 : 256), bh * (std::min(a.sinks, a.Tk) + (p.nrow > 1 ? (a.Tk + 3) / 4 : 0)) * 256});
   return p;
 }
 
@@ -1931,9 +1981,13 @@ int launch_backward(WaArgs& a, const BwdPlan& p, hipStream_t st) {
   const long bh = (long)a.B * a.Hkv;
   constexpr int OCC = 2, OCC_Q = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : (DP == 128 ? 2 : DP == 64 ? 3 : 4), KB = 4 / (RowWalk<T, DP>::RS / 32);
   const long rt = ((long)a.Tq * a.G + 127) / 128;
-  a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows, a.nrow = p.nrow;
-  WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC_Q>), bh * rt, 256, (Walk<T, DP>::LDS), st, a);
+  a.ntiles = (int)rt, a.ntiles32 = (int)rt * 4, a.nsplit = p.nsplit, a.nparts = p.nparts, a.sink_rows = p.sink_rows, a.nrow = p.nrow, a.nkey = p.nkey;
+  WA_LAUNCH((window_attn_dq_kernel<T, DP, OCC_Q>), bh * rt * a.nkey, 256, (Walk<T, DP>::LDS), st, a);
   TDX_CHECK_LAUNCH("window_attn_dq_kernel");
+  if (a.nkey > 1) {
+    hipLaunchKernelGGL((window_attn_dq_join_kernel<T, DP>), dim3((unsigned)(bh * (((long)a.Tq * a.G + 3) / 4))), dim3(256), 0, st, a);
+    TDX_CHECK_LAUNCH("window_attn_dq_join_kernel");
+  }
   if (a.Tk == 0) return TDX_OK;
   a.ntiles = (a.Tk + 127) / 128;
   const long sink_wgs = bh * ((p.sink_rows / 32 + KB - 1) / KB) * p.nsplit;
