@@ -334,3 +334,48 @@ def test_what_is_not_seen_does_not_reach_a_row(dtype, bad, Tq, Tk, few):
             name = ("dq", "dk", "dv")[n]
             R.check(f"{name} of keys it does not see", grads[n][:, far], ref[name][0][:, far], ref[name][1][:, far])
             assert torch.isnan(grads[n][:, ~far]).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+def test_shares_keep_out_what_is_not_seen(dtype, D):
+    """Few key heads: rows and keys are cut into shares, and the launches that join them take bad rows again."""
+    import ctypes as C
+
+    from test_sequence_cpu import _attn_desc
+
+    from trajectorydiffusion_amd import _lib
+    A = _att()
+    T, G, window = 900, 8, (400, 0, 3)
+    desc = _attn_desc(B=1, Tq=T, Tk=T, Hq=G, Hkv=1, D=D, dtype=A._CODES[dtype], left=400, right=0, sinks=0)
+    rows, keys = -(-T * G // 128) * 128 * 8, T * D * 8            # bytes of the row statistics, of a share of dK and dV
+    assert int(_lib.lib().tdx_window_attention_bwd_ws_bytes(C.byref(desc))) >= rows + 2 * keys
+    q, k, v, do, _, _ = _case(1, T, T, G, 1, D, dtype, None, None, seed=8)
+    ok = R.seen(1, T, T, *window)
+    ref = R.attention(q, k, v, ok, dout=do)
+
+    def grads(q, k, v):
+        x = [t.cuda().requires_grad_() for t in (q, k, v)]
+        out = A.window_attention(*x, *window)
+        g = torch.autograd.grad(out, x, do.cuda(), retain_graph=True)
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(g, torch.autograd.grad(out, x, do.cuda())))
+        return (out,) + g
+
+    names = ("out", "dq", "dk", "dv")
+    for n, g in zip(names, grads(q, k, v)):
+        R.check(n, g, *ref[n])
+    for bad in (math.nan, math.inf):
+        vd = v.clone()
+        vd[:, 50] = bad
+        hit = ok[0, :, 50]
+        far = ~ok[0][hit].any(0)
+        assert (~hit).any() and far.any()
+        got = grads(q, k, vd)
+        for n, g, keep in zip(names, got, (~hit, ~hit, far, far)):
+            R.check(f"{n}, {bad} in a value", g[:, keep], ref[n][0][:, keep], ref[n][1][:, keep])
+    qd = q.clone()
+    qd[:, 700] = math.nan
+    others, far = torch.arange(T) != 700, ~ok[0][700]
+    got = grads(qd, k, v)
+    for n, g, keep in zip(names, got, (others, others, far, far)):
+        R.check(f"{n}, a row of NaN", g[:, keep], ref[n][0][:, keep], ref[n][1][:, keep])
+        assert torch.isnan(g[:, ~keep]).all()
