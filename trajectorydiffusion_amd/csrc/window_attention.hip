@@ -1842,7 +1842,10 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
   return TDX_OK;
 }
 
-// Which forward kernel: the few-row kernel while the many-row kernel (128 rows a workgroup) would leave compute units idle
+// Which forward kernel: the few-row kernel for a token or so, and while the many-row kernel (128 rows a workgroup) would leave 3 of 8 compute units
+// idle, 5 of 8 for bf16 at 128 channels.  Measured, us, many-row / few-row: 252 workgroups (2 x 2000 tokens, 8 / 2 heads, window 512) bf16 17 / 27 at 64
+// channels, 23 / 63 at 128, fp32 42 / 62 and 67 / 141; 192 (3000, 8 heads, window 257) 16 / 21, 19 / 41, 35 / 43, 53 / 79; 128 (2048, 8 / 1 heads, causal)
+// 32 / 25, 43 / 54, 127 / 81, 204 / 172; 64 (1000, 8 heads, window 257) 16 / 11, 19 / 15, 34 / 16, 52 / 27.
 struct Plan {
   bool few, one;
   int ntiles, nsplit;
@@ -1860,7 +1863,7 @@ int few_per_unit(int es, int dp) { return es == 4 ? few_per_unit<float>(dp) : fe
 Plan plan_forward(const WaArgs& a, int es) {
   Plan p{};
   const long rows = (long)a.Tq * a.G, bh = (long)a.B * a.Hkv;
-  p.few = rows <= 32 || bh * ((rows + 127) / 128) < compute_units();
+  p.few = rows <= 32 || bh * ((rows + 127) / 128) < compute_units() * (es == 2 && padded(a.D) == 128 ? 3 : 5) / 8;
   p.ntiles = (int)((rows + (p.few ? 31 : 127)) / (p.few ? 32 : 128));
   p.nsplit = 1;
   if (p.few) {
