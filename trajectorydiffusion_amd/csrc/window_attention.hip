@@ -1874,12 +1874,12 @@ Plan plan_forward(const WaArgs& a, int es) {
     // Splits of the keys: the rounds of workgroups over the chip, of so many tiles a wave and two tiles' time to begin with, then the join (one
     // workgroup a row), in tiles' times.  Measured, fp32, 8 heads of 128 channels, one token: 300 keys 36 -> 16 us with 5 splits, 4096 keys 33 -> 17
     // with 32 and 27 with 64; bf16, 16 x 8 heads, 512 keys: 13 with 2, 18 with 4; 1000 tokens, 8 heads, window 257: 11 alone, 21 with a join.
-    const long most = std::min<long>(kMostSplits, tiles), fit = (long)compute_units() * few_per_unit(es, padded(a.D));
+    const int fit = compute_units() * few_per_unit(es, padded(a.D)), most = (int)std::min({(long)kMostSplits, tiles, 2 * fit / wgs});
     const double join = (2.5 + bh * rows / 1700.) * (es == 4 ? 0.5 : 1);   // (an fp32 tile takes twice as long)
     double best = 0;
-    for (long n = 1; n <= most && !p.one; ++n) {
-      const double cost = (double)((wgs * n + fit - 1) / fit) * ((tiles + 4 * n - 1) / (4 * n) + 2) + (n > 1 ? join : 0);
-      if (n == 1 || cost < best) best = cost, p.nsplit = (int)n;
+    for (int n = 1; n <= most && !p.one; ++n) {
+      const double cost = (double)(((int)wgs * n + fit - 1) / fit) * (((int)tiles + 4 * n - 1) / (4 * n) + 2) + (n > 1 ? join : 0);
+      if (n == 1 || cost < best) best = cost, p.nsplit = n;
     }
   }
   p.threads = bh * std::max<int64_t>((int64_t)p.ntiles * p.nsplit * (p.one ? 64 : 256), p.nsplit > 1 ? rows * 256 : 0);
@@ -1943,10 +1943,11 @@ int shares(int64_t wgs, int64_t stages, int64_t dp, int64_t bytes, int es) {
   const int64_t chip = (int64_t)compute_units() * (dp == 128 ? 1 : 2);
   double best = 0;
   int best_n = 1;
-  for (int64_t n = 1; n <= std::min<int64_t>(64, stages); ++n) {
+  const int most = (int)std::min({(int64_t)64, stages, 2 * chip / std::max<int64_t>(wgs, 1)});   // (two rounds: more shares only add to the join)
+  for (int n = 1; n <= most; ++n) {
     const double join = n > 1 ? (2 + (double)(n * bytes) * 2 / 8e6) * (es == 4 ? 0.5 : 1) : 0;
-    const double cost = (double)((wgs * n + chip - 1) / chip) * ((stages + n - 1) / n + 2) + join;
-    if (n == 1 || cost < best) best = cost, best_n = (int)n;
+    const double cost = (double)(((int)wgs * n + (int)chip - 1) / (int)chip) * (((int)stages + n - 1) / n + 2) + join;
+    if (n == 1 || cost < best) best = cost, best_n = n;
   }
   return best_n;
 }
