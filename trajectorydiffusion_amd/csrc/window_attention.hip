@@ -1477,6 +1477,9 @@ struct RowWalk {
   // fp32 then holds its V planes in LDS, 24 KB a wave: 16 x 625 tokens and fewer, 8 heads, window 129: 298 -> 235 us.
   static constexpr bool TWO = DP == 128, VLDS = TWO && N == 3;
   static constexpr int NW = TWO ? 8 : 4;
+  // fp32: the dV wave, which has registers and time left, stages for its pair (the dK wave spilled what it held for it:
+  // 239 -> 229 us)
+  static constexpr int STAGERS = VLDS ? 4 : NW;
   static constexpr uint32_t VF = NSTAGE * STAGE, LDS = VF + (VLDS ? 4 * N * G16<DP>::NC * 1024 : 0);
 };
 // Fragments a lane parks in LDS: piece (n, c) at base + (c N + n) 1024 + 16 lane
@@ -1622,8 +1625,10 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
       const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
       const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
       const int rend = s.ql * a.G;
-      PackedStager<T, DP, W::RS, W::NW> sq, sd;
+      constexpr bool STAGES = !(W::VLDS && ROLE == kOnlyDk);
+      PackedStager<T, DP, W::RS, W::STAGERS> sq, sd;
       auto load = [&](int t, uint32_t at) {
+        if constexpr (!STAGES) return;
         sq.load(at, qb, a.q_ts, a.q_hs, a.G, t * W::RS, rend, a.D, wave, lane);
         sd.load(at + W::TILE, db, a.do_ts, a.do_hs, a.G, t * W::RS, rend, a.D, wave, lane);
       };
@@ -1679,8 +1684,10 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
             wg_barrier();                       // the tile before has been read
             load_stat(t, lds);
           }
-          sq.put(lds);
-          sd.put(lds + W::TILE);
+          if constexpr (STAGES) {
+            sq.put(lds);
+            sd.put(lds + W::TILE);
+          }
           wait_vm<0>();
           if (t + 1 < t1) load(t + 1, lds);
           wg_barrier();
