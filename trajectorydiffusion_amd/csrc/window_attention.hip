@@ -1474,8 +1474,9 @@ struct RowWalk {
   static constexpr uint32_t PLANE = RS * G16<DP>::PITCH, TILE = N * PLANE, STAT = 2 * TILE, STAGE = 2 * TILE + 1024;
   // At 128 channels two waves share 32 keys, one for dV and one for dK: each has one accumulator, so two waves fit a SIMD where one with both
   // had it alone, for a quarter more matrix instructions (both take S).  bf16, 2 x 4096 tokens, 16 / 4 heads, window 1024: 241 -> 223 us.
-  // fp32 then holds its V planes in LDS, 24 KB a wave: 16 x 625 tokens and fewer, 8 heads, window 129: 298 -> 235 us.
-  static constexpr bool TWO = DP == 128, VLDS = TWO && N == 3;
+  // fp32 holds its V planes in LDS, 24 KB a wave: 16 x 625 tokens and fewer, 8 heads, window 129: 298 -> 235 us.  At 64 channels too, 12 KB a wave,
+  // where nothing spills any more: 2048 tokens, 8 / 1 heads, causal: 122 -> 82 us.
+  static constexpr bool TWO = DP == 128, VLDS = DP >= 64 && N == 3;
   static constexpr int NW = TWO ? 8 : 4;
   // fp32: the dV wave, which has registers and time left, stages for its pair (the dK wave spilled what it held for it:
   // 239 -> 229 us)
@@ -1964,7 +1965,7 @@ BwdPlan plan_backward(const WaArgs& a, int es) {
   p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
   const int64_t keys = ((int64_t)a.Tk + 127) / 128, tiles = (rows + 127) / 128;
   // dK / dV, bf16, 4096 tokens, 8 / 1 heads of 128 channels, causal (32 workgroups without shares): 1112 -> 173 us and 7 to join; 4 x 955, 16 / 4 heads
-  // of 64 (128 workgroups): 148 -> 51 and 8; fp32, 2048, 8 / 1 heads of 64, causal (16 workgroups): 2029 -> 123 and 7.  dQ of the last (128
+  // of 64 (128 workgroups): 148 -> 51 and 8; fp32, 2048, 8 / 1 heads of 64, causal (16 workgroups): 2029 -> 82 and 7.  dQ of the last (128
   // workgroups): 149 -> 65 and 7.
   const int64_t seen = a.left == kFar || a.right == kFar ? a.Tq : std::min<int64_t>(a.Tq, (int64_t)a.left + a.right + 128);
   p.nrow = shares(bh * keys, (seen * a.G + (es == 4 ? 31 : 63)) / (es == 4 ? 32 : 64), dp, bh * a.Tk * dp * 2 * 4, es);
