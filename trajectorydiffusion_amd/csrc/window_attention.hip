@@ -1475,7 +1475,7 @@ struct RowWalk {
   // At 128 channels two waves share 32 keys, one for dV and one for dK: each has one accumulator, so two waves fit a SIMD where one with both
   // had it alone, for a quarter more matrix instructions (both take S).  bf16, 2 x 4096 tokens, 16 / 4 heads, window 1024: 241 -> 223 us.
   // fp32 holds its V planes in LDS, 24 KB a wave: 16 x 625 tokens and fewer, 8 heads, window 129: 298 -> 235 us.  At 64 channels too, 12 KB a wave,
-  // where nothing spills any more: 2048 tokens, 8 / 1 heads, causal: 122 -> 82 us.
+  // where 57 spilled registers become 7: 2048 tokens, 8 / 1 heads, causal: 122 -> 82 us.
   static constexpr bool TWO = DP == 128, VLDS = DP >= 64 && N == 3;
   static constexpr int NW = TWO ? 8 : 4;
   // fp32: the dV wave, which has registers and time left, stages for its pair (the dK wave spilled what it held for it:
