@@ -1,0 +1,46 @@
+"""CPU: what the sequence operators tell autograd, and the contexts they refuse.  The launch itself is replaced by a note of its name."""
+import contextlib
+
+import pytest
+import torch
+
+
+class _Library:
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The names of the launches that a call makes; CPU tensors pass for device tensors."""
+    from trajectorydiffusion_amd import _lib, attention
+    names = []
+    monkeypatch.setattr(_lib, "require_device", lambda t, name: None)
+    monkeypatch.setattr(_lib, "lib", lambda: _Library())
+    monkeypatch.setattr(attention, "_launch", lambda fn, name, d, index: names.append(name))
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    attention._seen.__dict__.clear()
+    yield names
+    attention._seen.__dict__.clear()
+
+
+def test_a_rotation_into_a_tensor_counts_as_a_change_in_place(launches):
+    from trajectorydiffusion_amd import attention as A
+    x, pos = torch.randn(1, 4, 2, 16), torch.zeros(1, 4, 1)
+    for out in (x, torch.empty_like(x), torch.empty(1, 4, 6, 16)[:, :, 2:4]):
+        weight = torch.ones_like(out, requires_grad=True)
+        y = (weight * out).sum()                          # keeps `out` for the gradient of weight
+        A.rotary_axes(x, pos, (8,), out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.no_grad():                                 # a tensor that requires grad may be rotated where nothing is recorded
+        leaf = torch.randn(1, 4, 2, 16, requires_grad=True)
+        before = leaf._version
+        A.rotary_axes(leaf, pos, (8,), out=leaf)
+        assert leaf._version == before + 1
+    assert launches == ["tdx_rotary_axes"] * 4
+    with torch.inference_mode():                          # these count no versions
+        t = torch.randn(1, 4, 2, 16)
+        A.rotary_axes(t, pos, (8,), out=t)
+    empty = torch.empty(0, 4, 2, 16)
+    assert A.rotary_axes(empty, torch.zeros(4, 1), (8,), out=empty) is empty

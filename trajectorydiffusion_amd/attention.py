@@ -205,6 +205,7 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
             raise TdxError(f"{fn}: out overlaps x other than in place")
         if x.numel():
             _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
+            torch.autograd.graph.increment_version(out)   # the launch writes behind autograd's back
         return out
     if x.requires_grad and torch.is_grad_enabled():
         if x.numel() == 0:
