@@ -44,3 +44,30 @@ def test_a_rotation_into_a_tensor_counts_as_a_change_in_place(launches):
         A.rotary_axes(t, pos, (8,), out=t)
     empty = torch.empty(0, 4, 2, 16)
     assert A.rotary_axes(empty, torch.zeros(4, 1), (8,), out=empty) is empty
+
+
+def _both(A, pos):
+    return {"rotary_axes": lambda t: A.rotary_axes(t, pos, (8,)), "window_attention": lambda t: A.window_attention(t, t, t, 2, 2)}
+
+
+@pytest.mark.parametrize("name", ["rotary_axes", "window_attention"])
+def test_forward_mode_derivatives_are_refused(launches, name):
+    import torch.autograd.forward_ad as forward_ad
+
+    from trajectorydiffusion_amd import attention as A
+    x, pos = torch.randn(1, 4, 2, 16), torch.zeros(1, 4, 1)
+    f = _both(A, pos)[name]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for t in (dual, forward_ad.make_dual(x.clone().requires_grad_(), torch.ones_like(x))):
+            with pytest.raises(A.TdxError, match=f"{name}: forward-mode"):
+                f(t)
+        others = [lambda: A.window_attention(x, dual, x, 2, 2), lambda: A.window_attention(x, x, dual, 2, 2),
+                  lambda: A.rotary_axes(x, forward_ad.make_dual(pos, torch.ones_like(pos)), (8,)), lambda: A.rotary_axes(x, pos, (8,), out=forward_ad.make_dual(x.clone(), x))]
+        for g in others:
+            with pytest.raises(A.TdxError, match="forward-mode"):
+                g()
+        assert not launches
+        f(x)                                              # no tangent: an ordinary call
+    f(x)
+    assert len(launches) == 2

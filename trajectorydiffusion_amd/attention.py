@@ -25,6 +25,7 @@ import threading
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import RotaryDesc, TdxError, WindowAttnDesc
@@ -56,6 +57,13 @@ def _launch(fn, name: str, d, index: int) -> None:
             rc = fn(C.byref(d), torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
+
+
+def _refuse_tangents(fn: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises where a tensor carries a forward-mode tangent: the launches would drop it."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise TdxError(f"{fn}: forward-mode derivatives are not provided")
 
 
 def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
@@ -171,8 +179,10 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     layout    "halves": channels (m, m + P) are pair m; "pairs": channels (2 m, 2 m + 1)
     inverse   turn back
     out       write here (x itself: in place; no other overlap); not differentiable
-    Differentiable in x.  Returns a contiguous tensor of x's type."""
+    Differentiable in x (backward only).  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(fn, x, pos, out)
     try:   # a form of call that was checked before?
         sections = tuple(map(int, sections))   # (numbers, not what they come from: a tensor's value may change)
         base = base if base.__class__ is float else tuple(map(float, base)) if isinstance(base, (list, tuple)) else float(base)
@@ -382,7 +392,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     Hq a multiple of Hkv (query head h reads key head h // (Hq / Hkv)); D a multiple of 8, at most 128.  Queries that see nothing, and
     those behind q_len, get zeros (lse -inf) and pass no gradient; gradients of keys behind k_len are zero.  Whatever stands at keys a
     query does not see, NaN and infinities too, does not reach it.  Strided tensors are taken as they lie when their channels are
-    contiguous and their strides multiples of 16 bytes, else copied.  Differentiable in q, k, v; results are reproducible."""
+    contiguous and their strides multiples of 16 bytes, else copied.  Differentiable in q, k, v (backward only); results are reproducible."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("window_attention", q, k, v)
     try:   # a form of call that was checked before?
         if scale is not None and scale.__class__ is not float:
             scale = float(scale)
