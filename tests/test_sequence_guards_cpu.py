@@ -71,3 +71,41 @@ def test_forward_mode_derivatives_are_refused(launches, name):
         f(x)                                              # no tangent: an ordinary call
     f(x)
     assert len(launches) == 2
+
+
+@pytest.mark.parametrize("name", ["rotary_axes", "window_attention"])
+def test_tracing_is_refused(launches, name):
+    """A trace holds torch's operators alone: without the launch its result is memory that nothing wrote."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from trajectorydiffusion_amd import attention as A
+    x, pos = torch.randn(1, 4, 2, 16), torch.zeros(1, 4, 1)
+    f = _both(A, pos)[name]
+    ways = {"proxies": lambda t: make_fx(f)(t), "proxies ahead of dispatch": lambda t: make_fx(f, pre_dispatch=True)(t),
+            "proxies over fake tensors": lambda t: make_fx(f, tracing_mode="fake")(t), "jit": lambda t: torch.jit.trace(f, t, check_trace=False),
+            "proxies of a copy": lambda t: make_fx(lambda u: f(u.detach().clone()))(t)}
+    for way, g in ways.items():
+        for t in (x, x.clone().requires_grad_()):
+            with pytest.raises(A.TdxError, match=f"{name}: cannot be traced"):
+                g(t)
+    assert not launches
+    leaf = x.clone().requires_grad_()
+    y = f(leaf)
+    with pytest.raises(A.TdxError, match=f"{name}: cannot be traced"):
+        make_fx(lambda g: torch.autograd.grad(y, leaf, g))(torch.ones_like(y))
+    assert len(launches) == 1
+
+
+def test_modes_that_only_watch_are_no_trace(launches):
+    from torch.utils.checkpoint import checkpoint
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from trajectorydiffusion_amd import attention as A
+    x, pos = torch.randn(1, 4, 2, 16), torch.zeros(1, 4, 1)
+    with FlopCounterMode(display=False):
+        for f in _both(A, pos).values():
+            f(x)
+    assert launches == ["tdx_rotary_axes", "tdx_window_attention"]
+    y = checkpoint(_both(A, pos)["window_attention"], x.clone().requires_grad_(), use_reentrant=False)
+    y.sum().backward()
+    assert launches[2:] == ["tdx_window_attention"] * 2 + ["tdx_window_attention_bwd"]

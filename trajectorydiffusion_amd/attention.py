@@ -59,6 +59,17 @@ def _launch(fn, name: str, d, index: int) -> None:
         _lib.check(rc, name)
 
 
+# What a call asks before anything else: is a trace being recorded?  (proxies by dispatch mode, ahead of dispatch, or torch.jit)
+_modes, _modes_ahead, _jit = torch._C._len_torch_dispatch_stack, torch._ops._len_torch_dispatch_stack_pre_dispatch, torch._C._get_tracing_state
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _refuse_traces(fn: str) -> None:
+    """Raises under a trace, which holds torch's operators and not the launch: its result would be memory that nothing wrote."""
+    if _jit() is not None or torch._C._get_dispatch_mode(_PROXY) is not None or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None:
+        raise TdxError(f"{fn}: cannot be traced; call it outside of the traced function")
+
+
 def _refuse_tangents(fn: str, *tensors: Optional[torch.Tensor]) -> None:
     """Raises where a tensor carries a forward-mode tangent: the launches would drop it."""
     for t in tensors:
@@ -117,6 +128,7 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dout):
         if torch.is_grad_enabled():
             raise TdxError("rotary_axes: second derivatives are not provided")
+        _refuse_traces("rotary_axes")
         pos, = ctx.saved_tensors
         sections, bases, layout, inverse = ctx.args
         if dout.stride(3) != 1 and dout.shape[3] != 1:
@@ -181,6 +193,8 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     out       write here (x itself: in place; no other overlap); not differentiable
     Differentiable in x (backward only).  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
+    if _modes() or _modes_ahead() or _jit() is not None:
+        _refuse_traces(fn)
     if forward_ad._current_level >= 0:
         _refuse_tangents(fn, x, pos, out)
     try:   # a form of call that was checked before?
@@ -308,6 +322,7 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if torch.is_grad_enabled():
             raise TdxError("window_attention: second derivatives are not provided")
+        _refuse_traces("window_attention")
         none = (None,) * 6
         if dout is None:
             return (None, None, None) + none
@@ -393,6 +408,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     those behind q_len, get zeros (lse -inf) and pass no gradient; gradients of keys behind k_len are zero.  Whatever stands at keys a
     query does not see, NaN and infinities too, does not reach it.  Strided tensors are taken as they lie when their channels are
     contiguous and their strides multiples of 16 bytes, else copied.  Differentiable in q, k, v (backward only); results are reproducible."""
+    if _modes() or _modes_ahead() or _jit() is not None:
+        _refuse_traces("window_attention")
     if forward_ad._current_level >= 0:
         _refuse_tangents("window_attention", q, k, v)
     try:   # a form of call that was checked before?
