@@ -109,3 +109,45 @@ def test_modes_that_only_watch_are_no_trace(launches):
     y = checkpoint(_both(A, pos)["window_attention"], x.clone().requires_grad_(), use_reentrant=False)
     y.sum().backward()
     assert launches[2:] == ["tdx_window_attention"] * 2 + ["tdx_window_attention_bwd"]
+
+
+def test_a_result_over_the_positions_is_refused(launches):
+    from trajectorydiffusion_amd import attention as A
+    room = torch.zeros(2 * 4 * 32)
+    x = torch.randn(1, 4, 2, 16)
+    whole = room.view(2, 4, 2, 16)
+    for out, pos in ((whole[:1], room[3:19].view(4, 4)[:, :1]), (whole[:1], room[127:131].view(4, 1)), (whole[1:], room[127:131].view(4, 1)),
+                     (whole[1:], room[250:251].expand(4, 1))):
+        with pytest.raises(A.TdxError, match="overlaps pos"):
+            A.rotary_axes(x, pos, (8,), out=out)
+    with pytest.raises(A.TdxError, match="overlaps pos"):                     # views that share memory without sharing a storage
+        A.rotary_axes(x, torch.from_dlpack(room[120:124]).view(4, 1), (8,), out=whole[:1])
+    with pytest.raises(A.TdxError, match="overlaps x"):
+        A.rotary_axes(torch.from_dlpack(room[8:136]).view(1, 4, 2, 16), torch.zeros(4, 1), (8,), out=whole[:1])
+    assert not launches
+    A.rotary_axes(x, room[128:132].view(4, 1), (8,), out=whole[:1])
+    A.rotary_axes(x, room[:4].view(4, 1), (8,), out=whole[1:])
+    A.rotary_axes(torch.from_dlpack(room[128:]).view(1, 4, 2, 16), torch.zeros(4, 1), (8,), out=whole[:1])
+    assert len(launches) == 3
+    rows = torch.zeros(2, 5, 3 + 32 + 3)                                        # positions and heads side by side in each row
+    A.rotary_axes(torch.randn(2, 5, 2, 16), rows[:, :, :3], (4, 2, 2), out=rows[:, :, 3:35].unflatten(2, (2, 16)))
+    assert len(launches) == 4
+
+
+def test_shared_bytes_are_told_from_bytes_between_each_other():
+    """Against the byte numbers themselves, over drawn forms."""
+    from trajectorydiffusion_amd import attention as A
+    gen = torch.Generator().manual_seed(7)
+    draw = lambda n: int(torch.randint(0, n, (1,), generator=gen))  # noqa: E731
+    room = torch.zeros(800, dtype=torch.uint8)
+    ids = torch.arange(800)
+    found = [0, 0]
+    for _ in range(600):
+        views, held = [], []
+        for es, rank in ((2 if draw(2) else 4, 4), (4, 3)):
+            shape, stride, at = tuple(1 + draw(3) for _ in range(rank)), tuple((0, 1, 3, 4, 7, 12, 20)[draw(7)] for _ in range(rank)), draw(20)
+            views.append(room.view({2: torch.bfloat16, 4: torch.float32}[es]).as_strided(shape, stride, at))
+            held.append(set((ids.as_strided(shape + (es,), tuple(es * s for s in stride) + (1,), es * at)).flatten().tolist()))
+        assert A._touch(*views) == bool(held[0] & held[1])
+        found[bool(held[0] & held[1])] += 1
+    assert min(found) > 50

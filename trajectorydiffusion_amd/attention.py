@@ -158,27 +158,56 @@ def _rotary_args(x, pos, sections, base, layout) -> Tuple:
     return sections, bases, _LAYOUTS[layout]
 
 
-def _clash(x: torch.Tensor, out: torch.Tensor) -> bool:
-    """Whether `out` holds an element of x's memory at another place than x does (of one form and type; views of one storage only).
-    Equal strides: some difference of indices leads from one address to the other.  Other strides: the spans meet."""
-    if x.untyped_storage().data_ptr() != out.untyped_storage().data_ptr() or not x.numel():
-        return False
-    far, dims = out.storage_offset() - x.storage_offset(), [(st, n) for st, n in zip(x.stride(), x.shape) if n > 1]
-    if dims != [(st, n) for st, n in zip(out.stride(), out.shape) if n > 1]:
-        span = lambda t: sum((n - 1) * st for st, n in zip(t.stride(), t.shape))
-        return -span(out) <= far <= span(x)
-    dims.sort(reverse=True)
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte of t's elements and the one behind the last."""
+    at = t.data_ptr()
+    return at, at + (sum((n - 1) * st for st, n in zip(t.stride(), t.shape)) + 1) * t.element_size()
 
-    def reached(far: int, at: int) -> bool:
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory between the first and the last element of each has bytes in common."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _reached(far: int, dims: Sequence[Tuple[int, int, int]]) -> bool:
+    """Whether a sum of stride * i with i in [lo, hi], over the (stride, lo, hi) of dims, is `far`."""
+    merged = {}
+    for st, lo, hi in dims:                    # equal strides are one dimension
+        if st == 0:
+            continue
+        was = merged.get(st, (0, 0))
+        merged[st] = (was[0] + lo, was[1] + hi)
+    dims = sorted(((st, lo, hi) for st, (lo, hi) in merged.items()), reverse=True)
+
+    def search(far: int, at: int) -> bool:
         if at == len(dims):
             return far == 0
-        st, n = dims[at]
-        if st == 0:
-            return reached(far, at + 1)
-        inner = sum((m - 1) * t for t, m in dims[at + 1:])
-        low, high = -((inner - far) // st), (far + inner) // st
-        return any(reached(far - i * st, at + 1) for i in range(max(low, 1 - n), min(high, n - 1) + 1))
-    return far != 0 and reached(far, 0)
+        st, lo, hi = dims[at]
+        least, most = (sum(t * n[k] for t, *n in dims[at + 1:]) for k in (0, 1))    # of the dimensions behind
+        return any(search(far - i * st, at + 1) for i in range(max(lo, -((most - far) // st)), min(hi, (far - least) // st) + 1))
+    return search(far, 0)
+
+
+def _touch(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the two share a byte."""
+    ea, eb = a.element_size(), b.element_size()
+    dims = [(st * ea, 0, n - 1) for st, n in zip(a.stride(), a.shape)] + [(st * eb, 1 - n, 0) for st, n in zip(b.stride(), b.shape)]
+    return _meet(a, b) and _reached(b.data_ptr() - a.data_ptr(), dims + [(1, 1 - eb, ea - 1)])
+
+
+def _clash(x: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether `out` holds an element of x's memory at another place than x does (of one form and type).
+    Equal strides: some difference of indices leads from one address to the other.  Other strides: the spans meet."""
+    if not _meet(x, out):
+        return False
+    dims = [(st, n) for st, n in zip(x.stride(), x.shape) if n > 1]
+    far, part = divmod(out.data_ptr() - x.data_ptr(), x.element_size())
+    if part or dims != [(st, n) for st, n in zip(out.stride(), out.shape) if n > 1]:
+        return True
+    return far != 0 and _reached(far, [(st, 1 - n, n - 1) for st, n in dims])
 
 
 def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], base: Union[float, Sequence[float]] = 10000.0, layout: str = "halves",
@@ -190,7 +219,7 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     base      pair i of n of an axis turns by pos * base^(-i / n); one number, or one for each axis
     layout    "halves": channels (m, m + P) are pair m; "pairs": channels (2 m, 2 m + 1)
     inverse   turn back
-    out       write here (x itself: in place; no other overlap); not differentiable
+    out       write here (x itself: in place; no other overlap with x, none with pos); not differentiable
     Differentiable in x (backward only).  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
     if _modes() or _modes_ahead() or _jit() is not None:
@@ -227,6 +256,8 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
             raise TdxError(f"{fn}: out must not repeat its own memory")
         if out is not x and _clash(x, out):
             raise TdxError(f"{fn}: out overlaps x other than in place")
+        if _touch(out, pos):
+            raise TdxError(f"{fn}: out overlaps pos")
         if x.numel():
             _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
             torch.autograd.graph.increment_version(out)   # the launch writes behind autograd's back
