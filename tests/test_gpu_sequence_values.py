@@ -30,3 +30,143 @@ def test_a_key_that_attention_kept_may_not_be_rotated_before_the_backward_pass()
     A.rotary_axes(k, pos, (16,), out=k)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+# ---- scores of every size ----------------------------------------------------------------------------------------------------------------
+# A probability is rebuilt in the backward pass as 2^(s c - lse2) while |lse2| <= T (T = 128 for fp32, 2048 for bf16), from a log-sum lse2 that has been
+# rounded four times (m scale, + log l, log2 e, c) and two more of this size in the exponent: 6 v T ln 2 off; beyond, from the distance to the row's maximum
+# and the row's own sum, which are exact where one key, or several alike, hold all of a row.
+BUILT = {torch.float32: 6 * R.V * 128 * math.log(2), torch.bfloat16: 6 * R.V * 2048 * math.log(2)}
+
+
+def _tops(q, table, which, ok):
+    """(highest score of each row, the keys that have it, the largest |q| |k| scale, whether the next score is further away than what 32-bit scores may be off,
+    and 100)"""
+    B, Tq, Hq, D = q.shape
+    Q, each = q.double().permute(0, 2, 1, 3), table.double().permute(0, 2, 1, 3).repeat_interleave(Hq // table.shape[2], dim=1)
+    scale, m = D ** -0.5, ok[:, None].expand(B, Hq, Tq, len(which))
+    S = torch.where(m, (Q @ each.transpose(2, 3) * scale)[..., which], torch.full((1,), -math.inf, dtype=torch.float64))
+    a = float((Q.abs() @ each.abs().transpose(2, 3) * scale).max())
+    top = S.amax(-1, keepdim=True)
+    near = (S == top) & m
+    gap = torch.where(near, torch.full_like(S, -math.inf), S).amax(-1, keepdim=True)
+    return top, near, a, ((top - gap) > 2 * (D + 4) * R.V * a + 100)[..., 0] | ~m.any(-1)
+
+
+def _peaked(q, table, which, v, ok, do):
+    """name -> (value, bound) like R.attention, for keys table[which]: every row's probabilities are 1 / n at n equal keys and 0 elsewhere."""
+    u = R.HALF[q.dtype]
+    u1 = u if q.dtype != torch.float32 else 0.0
+    e = BUILT[q.dtype] + 2.0 ** -18
+    B, Tq, Hq, D = q.shape
+    Tk, Hkv = v.shape[1], v.shape[2]
+    G, scale = Hq // Hkv, D ** -0.5
+    Q, dO = (t.double().permute(0, 2, 1, 3) for t in (q, do))
+    W, K = (t.double().permute(0, 2, 1, 3).repeat_interleave(G, dim=1) for t in (v, table[:, which]))
+    m = ok[:, None].expand(B, Hq, Tq, Tk)
+    top, near, a, sure = _tops(q, table, which, ok)
+    assert sure.all(), "a row whose probabilities are not certain"
+    n = near.sum(-1, keepdim=True)
+    P = near.double() / n.clamp(min=1)
+    lse = torch.where(n > 0, top + n.double().log(), top)[..., 0]
+    out, PW = P @ W, P @ W.abs()
+    e_out = u * out.abs() + (u1 + e + Tk * R.V) * PW * (1 + u)
+    back = lambda t: t.permute(0, 2, 1, 3)  # noqa: E731
+    got = {"out": (back(out), back(e_out)), "lse": (lse, 2 * (D + 4) * R.V * a + 4 * R.V * lse.abs().nan_to_num(0, 0, 0) + e)}
+    dO = dO * m.any(-1)[..., None]
+    dP, delta = dO @ W.transpose(2, 3), (dO * out).sum(-1, keepdim=True)
+    dS = P * (dP - delta)
+    e_dp = D * R.V * (dO.abs() @ W.abs().transpose(2, 3)) + (dO.abs() * (e_out + D * R.V * out.abs())).sum(-1, keepdim=True) + 4 * R.V * (dP.abs() + delta.abs())
+    e_ds = (u1 + e) * dS.abs() + (1 + u1 + e) * P * e_dp
+    group = lambda t: t.reshape(B, Hkv, G, *t.shape[2:]).sum(2)  # noqa: E731
+    rows = Tq * G * R.V
+    dq, e_dq = dS @ K * scale, (e_ds + Tk * R.V * dS.abs()) @ K.abs() * scale
+    dk, e_dk = group(dS.transpose(2, 3) @ Q) * scale, group((e_ds + rows * dS.abs()).transpose(2, 3) @ Q.abs()) * scale
+    dv, e_dv = group(P.transpose(2, 3) @ dO), group(((u1 + e + rows) * P).transpose(2, 3) @ dO.abs())
+    for name, g, eg in (("dq", dq, e_dq), ("dk", dk, e_dk), ("dv", dv, e_dv)):
+        got[name] = (back(g), back(u * (g.abs() + eg) + eg + 4 * R.V * g.abs()))
+    return got
+
+
+FORMS = [  # B, Tq, Tk, Hq, Hkv, D, left, right, sinks
+    (2, 13, 13, 8, 8, 128, None, None, 0),
+    (2, 13, 13, 2, 1, 24, 2, 1, 3),
+    (2, 130, 130, 2, 2, 32, 17, 9, 4),
+    (1, 70, 70, 4, 2, 64, 5, 0, 3),
+    (1, 300, 300, 8, 1, 96, 100, 30, 16),
+    (1, 900, 900, 8, 1, 64, 400, 0, 3),              # rows and keys in shares
+    (1, 900, 900, 8, 1, 128, None, 0, 0),
+    (80, 150, 150, 4, 2, 64, 20, 2, 3),              # enough workgroups for the many-row kernel
+    (40, 140, 140, 8, 4, 128, 70, 0, 40),
+    (300, 130, 130, 1, 1, 32, 33, 20, 5),
+]
+
+
+def _sized(B, Tq, Tk, Hq, Hkv, D, size, dtype, kinds, seed):
+    """q, table of keys, which key stands where, v, dout: scaled scores of about `size`."""
+    q, table = (_normal(B, T, H, D, seed=seed + n) * size ** 0.5 for n, (T, H) in enumerate(((Tq, Hq), (kinds, Hkv))))
+    v, do = (_normal(B, T, H, D, seed=seed + 2 + n) for n, (T, H) in enumerate(((Tk, Hkv), (Tq, Hq))))
+    which = torch.randint(0, kinds, (Tk,), generator=torch.Generator().manual_seed(seed)) if kinds < Tk else torch.arange(Tk)
+    return q.to(dtype), table.to(dtype), which, v.to(dtype), do.to(dtype)
+
+
+def _settled(q, table, which, ok, size, seed):
+    """q with other rows in the place of those whose probabilities are not certain."""
+    for turn in range(20):
+        sure = _tops(q, table, which, ok)[3].transpose(1, 2)
+        if sure.all():
+            break
+        other = (_normal(*q.shape, seed=1000 + 20 * seed + turn) * size ** 0.5).to(q.dtype)
+        q = torch.where(sure[..., None], q, other)
+    return q
+
+
+def _compare(ref, q, k, v, do, args, **kwargs):
+    """The bounds hold for normal numbers; the hardware's exp2 gives 0 for results below 2^-126, and so may the rounding of a score gradient to bf16.  A probability
+    is therefore off by another 2^-126, a score gradient by that times 1 + |dP - delta|, and sums by as much for each of their terms."""
+    A, tiny = _att(), 2.0 ** -126
+    most = [float(t.double().abs().nan_to_num(0, 0, 0).max()) for t in (q, k, v, do)]
+    grads, scale = 1 + 2 * q.shape[3] * most[2] * most[3], kwargs.get("scale") or q.shape[3] ** -0.5
+    rows = q.shape[1] * q.shape[2] // k.shape[2]
+    for n, more in (("out", k.shape[1] * most[2]), ("dq", k.shape[1] * grads * most[1] * scale), ("dk", rows * grads * most[0] * scale), ("dv", rows * most[3])):
+        ref[n] = (ref[n][0], ref[n][1] + tiny * more)
+    x = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out, lse = A.window_attention(*x, *args, return_lse=True, **kwargs)
+    R.check("out", out, *ref["out"])
+    R.check("lse", lse, *ref["lse"])
+    grads = torch.autograd.grad(out, x, do.cuda(), retain_graph=True)
+    for n, g in zip(("dq", "dk", "dv"), grads):
+        R.check(n, g, *ref[n])
+    for a, b in zip(grads, torch.autograd.grad(out, x, do.cuda())):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("size", [1.0, 1e3, 1e7, 1e30])
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_that_see_one_key(form, size, dtype):
+    """Their probability is 1, so dv is dout, and dq and dk are what rounding leaves of nothing."""
+    B, Tq, Tk, Hq, Hkv, D = form[:6]
+    q, table, which, v, do = _sized(B, Tq, Tk, Hq, Hkv, D, size, dtype, Tk, 3)
+    _compare(_peaked(q, table, which, v, R.seen(B, Tq, Tk, 0, 0, 0), do), q, table, v, do, (0, 0, 0))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("size", [1e7, 1e30])
+@pytest.mark.parametrize("form", FORMS)
+def test_gradients_of_huge_scores(form, size, dtype):
+    """Rows over several keys, some of them alike: these share the probability."""
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    q, table, which, v, do = _sized(B, Tq, Tk, Hq, Hkv, D, size, dtype, min(Tk, 8), 11)
+    k, ok = table[:, which].contiguous(), R.seen(B, Tq, Tk, left, right, sinks)
+    q = _settled(q, table, which, ok, size, 11)
+    _compare(_peaked(q, table, which, v, ok, do), q, k, v, do, (left, right, sinks))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("size", [1e3])
+@pytest.mark.parametrize("form", FORMS)
+def test_gradients_of_large_scores(form, size, dtype):
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    q, table, which, v, do = _sized(B, Tq, Tk, Hq, Hkv, D, size, dtype, Tk, 17)
+    _compare(R.attention(q, table, v, R.seen(B, Tq, Tk, left, right, sinks), dout=do), q, table, v, do, (left, right, sinks))

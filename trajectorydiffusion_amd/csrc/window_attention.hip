@@ -47,7 +47,7 @@ struct WaArgs {
   const void* dout;
   void *dq, *dk, *dv;
   long do_bs, do_ts, do_hs, dq_bs, dq_ts, dq_hs, dk_bs, dk_ts, dk_hs, dv_bs, dv_ts, dv_hs;
-  float *stat, *part, *near;          // per 32 rows {log2-sum-exp, delta}; shares of the sinks' gradients; of all rows' (nkey > 1), then of all keys' (nrow > 1)
+  float *stat, *part, *near;          // per 32 rows kStat numbers (see there); shares of the sinks' gradients; of all rows' (nkey > 1), then of all keys' (nrow > 1)
   int ntiles32, nparts, sink_rows;    // row tiles of 32; shares; sinks rounded up to 32 (0: no separate pass over the sinks)
   int nrow, nkey;                     // shares that the rows of a key tile (dK / dV) and the keys of a row tile (dQ) are cut into
 };
@@ -55,11 +55,8 @@ struct WaArgs {
 // ---- geometry of a staged tile ------------------------------------------------------------------------------------------------
 template <typename T, int DP>
 struct Geo {
-  static constexpr int ES = sizeof(T), PITCH = DP * ES, CH = PITCH / 16, NC = PITCH / 32, ND = DP / 32, RPI = 1024 / PITCH;
+  static constexpr int ES = sizeof(T), PITCH = DP * ES, CH = PITCH / 16, ND = DP / 32, RPI = 1024 / PITCH;
 };
-// a 32-row operand held in registers: row lane & 31, the 16-byte pieces of one lane half
-template <typename T, int DP>
-using Frags = u32x4[Geo<T, DP>::NC];
 // Permutation of the 16-byte pieces of row `row`.  Row reads (16 rows, one piece): the bank groups must differ over 16 rows.
 // Transposed reads: bf16 takes 4 rows x 64 bytes at a time (rows 4a .. 4a+3 must differ in the 64-byte block), fp32 the 128 bytes of
 // rows R and R + 4 (they must differ in the 128-byte block).
@@ -165,38 +162,7 @@ __device__ __forceinline__ void stage_rows(uint32_t lds, const char* base, uint3
 }
 
 // ---- matrix steps ---------------------------------------------------------------------------------------------------------------
-// acc += A B over the 32 bytes of channels that a fragment pair holds (lane half h: bytes 16 h .. 16 h + 15 of the piece, both sides alike)
-__device__ __forceinline__ void mma_piece(f32x16& acc, const u32x4& a, const u32x4& b, __bf16) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
-}
-__device__ __forceinline__ void mma_piece(f32x16& acc, const u32x4& a, const u32x4& b, float) {
-#pragma unroll
-  for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[s]), __uint_as_float(b[s]), acc, 0, 0, 0);
-}
-// acc (32 tile rows x 32 columns) = tile rows [row0, row0 + 32) times the fragments b
-template <typename T, int DP>
-__device__ __forceinline__ void rows_times(f32x16& acc, uint32_t tile, int row0, const Frags<T, DP>& b, int lane) {
-  using G = Geo<T, DP>;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  const int row = row0 + (lane & 31);
-  const uint32_t a0 = tile + row * G::PITCH;
-  const int c0 = (lane >> 5) ^ swz<T, DP>(row);
-  // reads run AHEAD pieces in front of the instructions that take them (see rows16)
-  constexpr int AHEAD = sizeof(T) == 4 ? 2 : G::NC < 4 ? G::NC : 4, RING = AHEAD + 1;
-  u32x4 p[RING];
-  auto read = [&](int c) { p[c % RING] = lds_ld16(a0 + ((c0 ^ (2 * c)) << 4)); };
-#pragma unroll
-  for (int c = 0; c < AHEAD; ++c) read(c);
-#pragma unroll
-  for (int c = 0; c < G::NC; ++c) {
-    if (c + AHEAD < G::NC) read(c + AHEAD);
-    __builtin_amdgcn_sched_barrier(0);
-    mma_piece(acc, p[c % RING], b[c], T());
-    __builtin_amdgcn_sched_barrier(0);
-  }
-}
-// acc[dt] (channels 32 dt .. + 31 x 32 columns) += (tile rows [row0, row0 + 32))^T p, p as rows_times left it: element i of a lane is tile
+// acc[dt] (channels 32 dt .. + 31 x 32 columns) += (tile rows [row0, row0 + 32))^T p, p as few_scores left it: element i of a lane is tile
 // row row0 + 8 (i / 4) + 4 h + i % 4
 template <int DP>
 __device__ __forceinline__ void cols_times(f32x16 (&acc)[DP / 32], uint32_t tile, int row0, const float (&p)[16], int lane, __bf16) {
@@ -251,6 +217,12 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
 // ---- tiles in 16 bits: bf16 as it is, fp32 as three bf16 planes ------------------------------------------------------------------------
 // The many-row kernels multiply fp32 as sums of bf16 products: x = hi + mid + lo, each the bf16 nearest to what the ones before it leave, holds
 // all 24 bits, and of the nine products the six down to 2^-16 are taken (the three others are below 2^-25 of |x y| together: less than the
@@ -286,14 +258,16 @@ struct LaneOff {
 };
 
 __device__ __forceinline__ f32x16 mfma16(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-template <int N>
+// SWAP: in the order that gives the bits of the product with a and b exchanged
+template <int N, bool SWAP = false>
 __device__ __forceinline__ void mma_planes(f32x16& acc, const bf16x8 (&a)[N], const bf16x8 (&b)[N]) {
   if constexpr (N == 3) {   // the smallest products first
-    acc = mfma16(a[2], b[0], acc);
-    acc = mfma16(a[0], b[2], acc);
+    constexpr int X = SWAP ? 0 : 2, Y = 2 - X, Z = SWAP ? 0 : 1, W = 1 - Z;
+    acc = mfma16(a[X], b[Y], acc);
+    acc = mfma16(a[Y], b[X], acc);
     acc = mfma16(a[1], b[1], acc);
-    acc = mfma16(a[1], b[0], acc);
-    acc = mfma16(a[0], b[1], acc);
+    acc = mfma16(a[Z], b[W], acc);
+    acc = mfma16(a[W], b[Z], acc);
   }
   acc = mfma16(a[0], b[0], acc);
 }
@@ -307,8 +281,8 @@ struct Nothing {
   __device__ __forceinline__ void operator()(int) const {}
 };
 // acc (32 tile rows x 32 columns) = the 32 tile rows at IMM times the fragments b; planes of a tile are PLANE bytes apart.
-// between(c) is called behind the instructions of step c < NC.
-template <int N, int DP, uint32_t IMM, uint32_t PLANE, typename F = Nothing>
+// between(c) is called behind the instructions of step c < NC.  SWAP: see mma_planes.
+template <int N, int DP, uint32_t IMM, uint32_t PLANE, bool SWAP = false, typename F = Nothing>
 __device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, const Frags16<N, DP>& b, F&& between = F()) {
   constexpr int NC = G16<DP>::NC, AHEAD = N == 3 ? 1 : NC < 4 ? NC : 4, RING = AHEAD + 1;
   bf16x8 a[RING][N];
@@ -327,7 +301,7 @@ __device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, cons
     bf16x8 bc[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) bc[n] = b[n][c];
-    mma_planes<N>(acc, a[c % RING], bc);
+    mma_planes<N, SWAP>(acc, a[c % RING], bc);
     between(c);
     pin();
   }
@@ -389,26 +363,47 @@ __device__ __forceinline__ void cols16(f32x16 (&acc)[DP / 32], const LaneOff<DP>
     pin();
   }
 }
-// a 32-row operand in registers: channels 16 c + 8 h .. + 7 of row `row`, zero beyond the channels or when !ok
+// piece c of a 32-row operand from memory: channels 16 c + 8 h .. + 7 of the lane's row `row`, zero beyond the channels or when !ok
+template <typename T>
+__device__ __forceinline__ void load_piece16(bf16x8 (&f)[Planes<T>::N], const T* row, int c, bool ok, int D, int lane) {
+  const int d = 16 * c + 8 * (lane >> 5);
+  const bool in = ok && d < D;
+  if constexpr (sizeof(T) == 2) {
+    f[0] = __builtin_bit_cast(bf16x8, in ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u});
+  } else {
+    float x[8];
+    const u32x4 a = in ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u};
+    const u32x4 b = in ? *reinterpret_cast<const u32x4*>(row + d + 4) : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(a[i]), x[4 + i] = __uint_as_float(b[i]);
+    split8<3>(x, f);
+  }
+}
+// a 32-row operand in registers
 template <typename T, int DP>
 __device__ __forceinline__ void load_frags16(Frags16<Planes<T>::N, DP>& f, const T* row, bool ok, int D, int lane) {
 #pragma unroll
   for (int c = 0; c < G16<DP>::NC; ++c) {
-    const int d = 16 * c + 8 * (lane >> 5);
-    const bool in = ok && d < D;
-    if constexpr (sizeof(T) == 2) {
-      f[0][c] = __builtin_bit_cast(bf16x8, in ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u});
-    } else {
-      float x[8];
-      const u32x4 a = in ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u};
-      const u32x4 b = in ? *reinterpret_cast<const u32x4*>(row + d + 4) : (u32x4){0u, 0u, 0u, 0u};
+    bf16x8 p[Planes<T>::N];
+    load_piece16<T>(p, row, c, ok, D, lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(a[i]), x[4 + i] = __uint_as_float(b[i]);
-      bf16x8 p[3];
-      split8<3>(x, p);
-      f[0][c] = p[0], f[1][c] = p[1], f[2][c] = p[2];
-    }
+    for (int n = 0; n < Planes<T>::N; ++n) f[n][c] = p[n];
   }
+}
+// The product of row `held` (the same for all lanes) with the lane's own row, both from memory, in the bits of rows16 with `held` in the tile (SWAP: the other
+// row); lanes n and n + 32 have the same row.
+template <typename T, bool SWAP = false>
+__device__ __forceinline__ float row_times(const T* held, const T* row, bool ok, int D, int lane) {
+  f32x16 acc;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  for (int c = 0; 16 * c < D; ++c) {
+    bf16x8 a[Planes<T>::N], b[Planes<T>::N];
+    load_piece16<T>(a, held, c, true, D, lane);
+    load_piece16<T>(b, row, c, ok, D, lane);
+    mma_planes<Planes<T>::N, SWAP>(acc, a, b);
+  }
+  return acc[0];
 }
 // Uses the fragments, so that the compiler's wait for their loads stands here and not inside a loop, where it would also wait for the
 // direct loads in flight.
@@ -505,6 +500,43 @@ struct Stager<float, DP, ROWS> {
     }
   }
 };
+
+// acc (32 keys x 32 columns) = the 32 rows of a tile as it lies in memory (swz) times the fragments b, in the bits of rows16: fp32 rows are split into planes here
+template <typename T, int DP>
+__device__ __forceinline__ void few_scores(f32x16& acc, uint32_t tile, const Frags16<Planes<T>::N, DP>& b, int lane) {
+  constexpr int N = Planes<T>::N, NC = G16<DP>::NC, AHEAD = N == 3 ? 1 : NC < 4 ? NC : 4, RING = AHEAD + 1, PIECES = N == 3 ? 2 : 1;   // 16-byte pieces of a step
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  const int row = lane & 31;
+  const uint32_t a0 = tile + row * Geo<T, DP>::PITCH;
+  const int c0 = (PIECES * (lane >> 5)) ^ swz<T, DP>(row);
+  // reads run AHEAD steps in front of the instructions that take them (see rows16)
+  u32x4 p[RING][PIECES];
+  auto read = [&](int c) {
+#pragma unroll
+    for (int x = 0; x < PIECES; ++x) p[c % RING][x] = lds_ld16(a0 + ((c0 ^ (2 * PIECES * c + x)) << 4));
+  };
+#pragma unroll
+  for (int c = 0; c < AHEAD; ++c) read(c);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (c + AHEAD < NC) read(c + AHEAD);
+    pin();
+    bf16x8 ac[N], bc[N];
+    if constexpr (N == 1) {
+      ac[0] = __builtin_bit_cast(bf16x8, p[c % RING][0]);
+    } else {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(p[c % RING][0][i]), x[4 + i] = __uint_as_float(p[c % RING][1][i]);
+      split8<N>(x, ac);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) bc[n] = b[n][c];
+    mma_planes<N>(acc, ac, bc);
+    pin();
+  }
+}
 
 // ---- one sequence ---------------------------------------------------------------------------------------------------------------
 struct Seq {
@@ -685,23 +717,6 @@ __device__ __forceinline__ Item xcd_item(int block, int nbh, int per) {
   return {bh, item - bh * per};
 }
 
-// Q (or dO) fragments of row `row` (a query head's row), zero beyond the channels or when !ok
-template <typename T, int DP>
-__device__ __forceinline__ void load_frags(Frags<T, DP>& f, const T* row, bool ok, int D, int lane) {
-#pragma unroll
-  for (int c = 0; c < Geo<T, DP>::NC; ++c) {
-    const int d = (32 * c + 16 * (lane >> 5)) / (int)sizeof(T);
-    f[c] = ok && d < D ? *reinterpret_cast<const u32x4*>(row + d) : (u32x4){0u, 0u, 0u, 0u};
-  }
-}
-
-// (see arrived16)
-template <typename F, int N>
-__device__ __forceinline__ void arrived(F (&f)[N]) {
-#pragma unroll
-  for (int c = 0; c < N; ++c) asm volatile("" : "+v"(f[c]));
-}
-
 // What the many-row kernels walk over the key tiles with: BN keys a tile, bf16 in two stages of direct loads, fp32 in one stage of planes and
 // one of numbers as they arrive (forward at 128 channels: 128 us with the numbers held in registers, 88 so; 64 keys a tile would leave a compute unit one workgroup)
 template <typename T, int DP>
@@ -879,8 +894,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 // unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.  bf16 has two stages a wave, fp32 one, whose halves
 // are reloaded in turn, which leaves room for four waves at 128 channels too (8 x 4 heads over 8192 keys, window 4096: 75 -> 42 us).  Where a row tile sees two key
 // tiles at most (short tracks) a workgroup is one wave and keeps its result in registers: more workgroups fit a compute unit, and there is
-// nothing to join (64 x 8 heads x 13 tokens of 128 channels, fp32: 14 us, latency; 29 with two waves that join).  fp32 takes the fp32 matrix
-// instructions: its products are not what binds it, and a tile that is read once need not be split first.
+// nothing to join (64 x 8 heads x 13 tokens of 128 channels, fp32: 14 us, latency; 29 with two waves that join).  fp32 splits a tile into
+// planes as it reads it for the scores, which so have the bits that the backward pass sees again; the product with V takes the fp32 matrix instructions: it is
+// not what binds it, and a tile that is read once need not be split first.
 // Measured: 64 streams of up to 8192 cached keys, 4 heads of 128 channels in bf16, window 4096: 98 us, 5.3 TB/s (a copy reaches 5.2); one stream of
 // 32768, window 16384: 13 to 15 us and 4 to join, 2.4 TB/s.
 template <typename T, int DP, bool ONE>
@@ -921,8 +937,8 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * kLog2e, slack = 8.0f / c;
   if (r0 < rend) {
-    Frags<T, DP> qf;
-    load_frags<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
+    Frags16<Planes<T>::N, DP> qf;
+    load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
     const int p = i + s.shift, p0 = r0 / a.G + s.shift, p1 = (rend - 1) / a.G + s.shift;
     const Tiles t = tiles_of(a, s, p0, p1, 32);
     const int n = t.na + t.nb, per = (n + a.nsplit - 1) / a.nsplit;
@@ -938,7 +954,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       stage_rows<T, DP, 32, 1>(ring + buf * F::STAGE + F::STAGE / 2, (const char*)(vb + (long)j0 * a.v_ts), vs, s.kl - j0, dbytes, 0, lane);
     };
     if (first < last) stage_k(first, 0), stage_v(first, 0);
-    arrived(qf);               // from here on only direct loads are counted
+    arrived16(qf);             // from here on only direct loads are counted
     int buf = 0;
     for (int it = first; it < last; it += F::NW, buf ^= !F::HALVES) {
       const bool more = it + F::NW < last;
@@ -954,7 +970,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
       const uint32_t kt = ring + buf * F::STAGE, vt = kt + F::STAGE / 2;
       const int cls = seen_class(a, s, j0, p0, p1);
       f32x16 acc;
-      if (cls) rows_times<T, DP>(acc, kt, 0, qf, lane);
+      if (cls) few_scores<T, DP>(acc, kt, qf, lane);
       if constexpr (F::HALVES) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // K has been read
         if (more) {
@@ -1148,15 +1164,64 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
 // With P = exp(scale q k^T - lse), delta = sum_d dO O, dP = dO V^T, dS = P (dP - delta):
 //   dV = P^T dO,   dQ = scale dS K,   dK = scale dS^T Q.
+// The exponent s c - lse2 (c = scale log2 e, lse2 = lse log2 e) is off by what lse was rounded by, at most 6 2^-24 |lse2|: up to |lse2| = kBuilt that is less than
+// the scores' own sums are off (fp32: 3e-5 of P) or a fraction of P's rounding (bf16: 5e-4).  Beyond, P would neither sum to 1 nor stay finite (one key that a row
+// sees alone: P = 1.02 at a score of 1e5, 9 at 1e7): dQ's waves take the maximum m and the sum l of such rows again from the scores as they see them, and
+// P = 2^((s - m) c - log2 l) then.  The forward kernels, dQ and dK / dV have the same bits of s: all add the same products in the same order.  The way there costs
+// rows that do not need it up to 3 % (dK / dV 41.4 -> 42.8 us at 8192 tokens, 8 heads of 64 channels, window 257, bf16; 229 -> 230 at the next line's size).
 // Two kernels take S and dP again, each in the orientation that leaves its sums in one wave's registers, so nothing is added by atomics
 // and the order of every sum is fixed: dQ walks the keys of 128 rows (like the forward pass), dK / dV walk the rows that see 32 keys a
 // wave.  The sinks are seen by every later row: their rows beyond the window are cut into shares that run as workgroups of their own.
 // dQ, bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 118 us, 766 TFLOP/s; fp32, 16 x 625 tokens and fewer, 8 heads of 128,
 // window 129: 159 us, where one wave has a SIMD to itself (434 registers: the planes of Q and dO alone are 192) and nothing covers its vector work.
 
-// The gradient of one query row, over the keys it sees alone (see row_again)
 template <typename T>
-__device__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, int g, float lse2, float delta, int lane) {
+constexpr float kBuilt = sizeof(T) == 4 ? 128.f : 2048.f;
+// Numbers of 32 rows: exponents' offsets [32], delta [32], what is taken off the scores first [32] (0, or a far row's maximum), and 1 if any of these is not 0
+constexpr int kStat = 100;
+
+// Maximum and sum of exponentials of a wave's 32 rows (planes qf, lane n and n + 32: row n at position p; all of them at [p0, p1]), from scores in the bits of
+// rows16, straight from memory
+template <typename T, int DP>
+__device__ __forceinline__ void rows_max_sum(const WaArgs& a, const Seq& s, const T* kb, int p, int p0, int p1, const Frags16<Planes<T>::N, DP>& qf, float c, int lane,
+                                             float& m, float& l) {
+  constexpr int N = Planes<T>::N;
+  const Tiles t = tiles_of(a, s, p0, p1, 32);
+  m = -INFINITY, l = 0.f;
+  for (int it = 0; it < t.na + t.nb; ++it) {
+    const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < G16<DP>::NC; ++x) {
+      bf16x8 k[N], q[N];
+      load_piece16<T>(k, kb + (long)j * a.k_ts, x, j < s.kl, a.D, lane);
+#pragma unroll
+      for (int n = 0; n < N; ++n) q[n] = qf[n][x];
+      mma_planes<N>(acc, k, q);
+    }
+    float sc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+    mask_scores(sc, a, s, j0, p, lane);
+    float top = sc[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[e]);
+    top = fmaxf(half_max(top), m);
+    if (top == -INFINITY) continue;
+    l *= __builtin_amdgcn_exp2f((m - top) * c);
+    m = top;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) l += __builtin_amdgcn_exp2f((sc[e] - m) * c);
+  }
+  l = half_sum(l);
+}
+
+// The gradient of one query row, over the keys it sees alone (see row_again), 32 at a time: their scores' maximum and sum first, so that the probabilities sum
+// to 1 whatever the scores
+template <typename T>
+__device__ __forceinline__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, int g, float delta, int lane) {
   const long hq = (long)(hk * a.G + g);
   const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + hq * a.q_hs;
   const T* dO = (const T*)a.dout + b * a.do_bs + i * a.do_ts + hq * a.do_hs;
@@ -1164,23 +1229,36 @@ __device__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, in
   const T* v = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
   T* dq = (T*)a.dq + b * a.dq_bs + i * a.dq_ts + hq * a.dq_hs;
   const int p = i + s.shift, hi = min(p + a.right, s.kl - 1), lo = max(p - a.left, 0);
+  const float c = a.scale * kLog2e;
+  const Tiles t = tiles_of(a, s, p, p, 32);
   const int d0 = lane, d1 = lane + 64;
   const bool on0 = d0 < a.D, on1 = d1 < a.D;
-  const float q0 = on0 ? Elem<T>::ld(q + d0) : 0.f, q1 = on1 ? Elem<T>::ld(q + d1) : 0.f;
-  const float g0 = on0 ? Elem<T>::ld(dO + d0) : 0.f, g1 = on1 ? Elem<T>::ld(dO + d1) : 0.f;
-  const float c = a.scale * kLog2e;
-  float r0 = 0.f, r1 = 0.f;
-  for (int j = 0; j <= hi; ++j) {
-    if (j < lo && j >= a.sinks) j = lo;
-    if (j > hi) break;
-    const T *kr = k + j * a.k_ts, *vr = v + j * a.v_ts;
-    const float k0 = on0 ? Elem<T>::ld(kr + d0) : 0.f, k1 = on1 ? Elem<T>::ld(kr + d1) : 0.f;
-    const float sc = wave_sum((on0 ? q0 * k0 : 0.f) + (on1 ? q1 * k1 : 0.f));
-    const float dp = wave_sum((on0 ? g0 * Elem<T>::ld(vr + d0) : 0.f) + (on1 ? g1 * Elem<T>::ld(vr + d1) : 0.f));
-    const float ds = __builtin_amdgcn_exp2f(fmaf(sc, c, -lse2)) * (dp - delta);
-    r0 = fmaf(ds, k0, r0);
-    r1 = fmaf(ds, k1, r1);
-  }
+  float m = -INFINITY, l = 0.f, r0 = 0.f, r1 = 0.f;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int it = 0; it < t.na + t.nb; ++it) {
+      const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
+      const bool seen = j <= hi && (j >= lo || j < a.sinks);
+      const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
+      if (pass == 0) {
+        float top = seen ? sc : -INFINITY;
+        top = fmaxf(wave_max(top), m);
+        if (top == -INFINITY) continue;
+        l = l * __builtin_amdgcn_exp2f((m - top) * c) + 0.5f * wave_sum(seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f);   // (both halves hold the keys)
+        m = top;
+        continue;
+      }
+      const float dp = row_times<T>(dO, v + (long)j * a.v_ts, j < s.kl, a.D, lane);
+      const float ds = seen && l != 0.f ? __builtin_amdgcn_exp2f((sc - m) * c) / l * (dp - delta) : 0.f;
+      const uint32_t mask = (uint32_t)__ballot(seen);
+#pragma unroll 4
+      for (int n = 0; n < 32; ++n) {
+        const T* kr = k + (long)(j0 + n) * a.k_ts;
+        const bool in = mask >> n & 1;
+        const float w = __shfl(ds, n, 64), k0 = in && on0 ? Elem<T>::ld(kr + d0) : 0.f, k1 = in && on1 ? Elem<T>::ld(kr + d1) : 0.f;
+        r0 = fmaf(w, k0, r0);
+        r1 = fmaf(w, k1, r1);
+      }
+    }
   if (on0) dq[d0] = (T)(r0 * a.scale);
   if (on1) dq[d1] = (T)(r1 * a.scale);
 }
@@ -1207,7 +1285,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
   Frags16<N, DP> qf, df;
-  float delta = 0.f, lse2 = INFINITY;
+  float delta = 0.f, lse2 = INFINITY, off_s = 0.f;                          // (off_s, lse2: see kStat)
+  bool far = false;                                                        // of any row of the wave
+  const int p = i + s.shift;
+  const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;
+  const float c = a.scale * kLog2e;
   // the rows' own data, behind the first tile's loads; a row that sees nothing has lse = -inf: +inf makes its probabilities 0
   auto rows_ready = [&] {
     load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + hq * a.q_hs, row_ok, a.D, lane);
@@ -1255,12 +1337,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
     else lse2 = lse * kLog2e;
     arrived16(qf);
     arrived16(df);
+    const bool mine = lse > -INFINITY && __builtin_fabsf(lse2) > kBuilt<T>;
+    if (__ballot(mine)) {
+      far = true;
+      float m, l;
+      rows_max_sum<T, DP>(a, s, (const T*)a.k + b * a.k_bs + hk * a.k_hs, p, wp0, wp1, qf, c, lane, m, l);
+      if (mine) off_s = l == 0.f ? 0.f : m, lse2 = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+    }
   };
-  const float c = a.scale * kLog2e;
   if (r0 < rend) {
     const LaneOff<DP> off(lds, lane);
-    const int p = i + s.shift;
-    const int wp0 = rw / a.G + s.shift, wp1 = (min(rw + 32, rend) - 1) / a.G + s.shift;
     const bool wave_ok = rw < rend;
     const Tiles t = tiles_of(a, s, r0 / a.G + s.shift, (rend - 1) / a.G + s.shift, W::BN);
     auto one = [&](int j0, auto at) {
@@ -1271,6 +1357,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
       float sc[16];
       constexpr int NC = G16<DP>::NC;
       rows16<N, DP, A, W::PLANE>(acc, off, qf);
+      if (__builtin_expect(far, 0)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] -= off_s;
+      }
       rows16<N, DP, A + W::TILE, W::PLANE>(dp, off, df, [&](int k) {
 #pragma unroll
         for (int e = k * 16 / NC; e < (k + 1) * 16 / NC; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, -lse2));
@@ -1299,7 +1389,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
       if constexpr (W::BN == 64) one(j0 + 32, std::integral_constant<uint32_t, S0 + 32 * G16<DP>::PITCH>());
     });
   }
-  if (share == 0) a.stat[((long)bh * a.ntiles32 + tile * 4 + wave) * 64 + lane] = lane < 32 ? lse2 : delta;   // (both lane halves hold the row's numbers)
+  if (share == 0) {                                                        // (both lane halves hold the row's numbers)
+    float* stat = a.stat + ((long)bh * a.ntiles32 + tile * 4 + wave) * kStat;
+    stat[lane] = lane < 32 ? lse2 : delta;
+    if (lane < 32) stat[64 + lane] = off_s;
+    if (lane == 0) stat[96] = far ? 1.f : 0.f;
+  }
   if (a.nkey > 1) {
     if (r < R) {
       float* part = a.near + (((long)bh * a.nkey + share) * R + r) * DP + 4 * (lane >> 5);
@@ -1332,7 +1427,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
   while (again) {
     const int n = __builtin_ctzll(again);
     again &= again - 1;
-    dq_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(lse2, n, 64), __shfl(delta, n, 64), lane);
+    dq_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(delta, n, 64), lane);
   }
 #endif
 }
@@ -1364,9 +1459,9 @@ __global__ __launch_bounds__(256) void window_attn_dq_join_kernel(const WaArgs a
       bad |= v != v;
     }
   }
-  const float* stat = a.stat + ((long)bh * a.ntiles32 + (r >> 5)) * 64 + (r & 31);
+  const float* stat = a.stat + ((long)bh * a.ntiles32 + (r >> 5)) * kStat + (r & 31);
   const float lse2 = stat[0], delta = stat[32];
-  if (__ballot(bad) && lse2 == lse2 && delta == delta) dq_again<T>(a, s, b, hk, i, g, lse2, delta, lane);
+  if (__ballot(bad) && lse2 == lse2 && delta == delta) dq_again<T>(a, s, b, hk, i, g, delta, lane);
 #endif
 }
 
@@ -1429,35 +1524,40 @@ struct PackedStager<float, DP, ROWS, NW> {
   }
 };
 
-// The gradients of one key (and value) row over the query rows that see it alone (see row_again)
+// The gradients of one key (and value) row over the query rows that see it alone (see row_again), 32 at a time, with scores in the bits of dQ's
 template <typename T>
-__device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, int lane, bool want_dk, bool want_dv) {
+__device__ __forceinline__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, int lane, bool want_dk, bool want_dv) {
   const T* k = (const T*)a.k + b * a.k_bs + j * a.k_ts + hk * a.k_hs;
   const T* v = (const T*)a.v + b * a.v_bs + j * a.v_ts + hk * a.v_hs;
   const int d0 = lane, d1 = lane + 64;
   const bool on0 = d0 < a.D, on1 = d1 < a.D;
-  const float k0 = on0 ? Elem<T>::ld(k + d0) : 0.f, k1 = on1 ? Elem<T>::ld(k + d1) : 0.f;
-  const float v0 = on0 ? Elem<T>::ld(v + d0) : 0.f, v1 = on1 ? Elem<T>::ld(v + d1) : 0.f;
   const float c = a.scale * kLog2e;
   const int ilo = max(0, j - a.right - s.shift), ihi = j < a.sinks ? s.ql - 1 : min(s.ql - 1, j + a.left - s.shift);
-  const float* stat = a.stat + (long)(b * a.Hkv + hk) * a.ntiles32 * 64;
+  const int rlo = ilo * a.G, rhi = (ihi + 1) * a.G;
   float dk0 = 0.f, dk1 = 0.f, dv0 = 0.f, dv1 = 0.f;
-  for (int r = ilo * a.G; r < (ihi + 1) * a.G; ++r) {
-    const int i = r / a.G, g = r - i * a.G;
-    const long hq = (long)(hk * a.G + g);
-    const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + hq * a.q_hs;
-    const T* dO = (const T*)a.dout + b * a.do_bs + i * a.do_ts + hq * a.do_hs;
-    const float q0 = on0 ? Elem<T>::ld(q + d0) : 0.f, q1 = on1 ? Elem<T>::ld(q + d1) : 0.f;
-    const float g0 = on0 ? Elem<T>::ld(dO + d0) : 0.f, g1 = on1 ? Elem<T>::ld(dO + d1) : 0.f;
-    const float sc = wave_sum((on0 ? q0 * k0 : 0.f) + (on1 ? q1 * k1 : 0.f));
-    const float dp = wave_sum((on0 ? g0 * v0 : 0.f) + (on1 ? g1 * v1 : 0.f));
-    const float lse2 = stat[(r >> 5) * 64 + (r & 31)], delta = stat[(r >> 5) * 64 + 32 + (r & 31)];
-    const float p = __builtin_amdgcn_exp2f(fmaf(sc, c, -lse2)), ds = p * (dp - delta);
-    dv0 = fmaf(p, g0, dv0);
-    dv1 = fmaf(p, g1, dv1);
-    dk0 = fmaf(ds, q0, dk0);
-    dk1 = fmaf(ds, q1, dk1);
-    if (__all(dk0 != dk0 && dv0 != dv0 && (!on1 || (dk1 != dk1 && dv1 != dv1)))) break;   // it is what it is
+  for (int r0 = rlo & ~31; r0 < rhi; r0 += 32) {
+    const int r = r0 + (lane & 31), i = r / a.G;
+    const bool in = r >= rlo && r < rhi;
+    const long hq = (long)hk * a.G + (r - i * a.G);
+    const float* stat = a.stat + ((long)(b * a.Hkv + hk) * a.ntiles32 + (r0 >> 5)) * kStat + (lane & 31);
+    const float sc = row_times<T>(k, (const T*)a.q + b * a.q_bs + i * a.q_ts + hq * a.q_hs, in, a.D, lane);
+    const float dp = row_times<T>(v, (const T*)a.dout + b * a.do_bs + i * a.do_ts + hq * a.do_hs, in, a.D, lane);
+    const float p = in ? __builtin_amdgcn_exp2f(fmaf(sc - stat[64], c, -stat[0])) : 0.f, ds = in ? p * (dp - stat[32]) : 0.f;
+    const uint32_t mask = (uint32_t)__ballot(in);
+#pragma unroll 4
+    for (int n = 0; n < 32; ++n) {
+      if (!(mask >> n & 1)) continue;
+      const int at = (r0 + n) / a.G;
+      const long hn = (long)hk * a.G + (r0 + n - at * a.G);
+      const T* q = (const T*)a.q + b * a.q_bs + at * a.q_ts + hn * a.q_hs;
+      const T* dO = (const T*)a.dout + b * a.do_bs + at * a.do_ts + hn * a.do_hs;
+      const float pn = __shfl(p, n, 64), dn = __shfl(ds, n, 64);
+      dv0 = fmaf(pn, on0 ? Elem<T>::ld(dO + d0) : 0.f, dv0);
+      dv1 = fmaf(pn, on1 ? Elem<T>::ld(dO + d1) : 0.f, dv1);
+      dk0 = fmaf(dn, on0 ? Elem<T>::ld(q + d0) : 0.f, dk0);
+      dk1 = fmaf(dn, on1 ? Elem<T>::ld(q + d1) : 0.f, dk1);
+    }
+    if (__all((!on0 || (dk0 != dk0 && dv0 != dv0)) && (!on1 || (dk1 != dk1 && dv1 != dv1)))) break;   // it is what it is
   }
   T* dk = (T*)a.dk + b * a.dk_bs + j * a.dk_ts + hk * a.dk_hs;
   T* dv = (T*)a.dv + b * a.dv_bs + j * a.dv_ts + hk * a.dv_hs;
@@ -1467,7 +1567,7 @@ __device__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, i
   if (on1 && want_dv) dv[d1] = (T)dv1;
 }
 
-// What the dK / dV kernel walks over the rows with: RS rows a stage (q, dout and their {log2-sum-exp, delta}), two stages for bf16
+// What the dK / dV kernel walks over the rows with: RS rows a stage (q, dout and their statistics), two stages for bf16
 template <typename T, int DP>
 struct RowWalk {
   static constexpr int N = Planes<T>::N, RS = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
@@ -1510,7 +1610,7 @@ enum { kBoth = 0, kOnlyDv = 1, kOnlyDk = 2 };
 // lane's key; [rlo, rhi] are the packed rows (of the whole sequence) that see the lane's key, checked when `part`.
 template <typename T, int DP, uint32_t A, uint32_t ST, int ROLE>
 __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32], const LaneOff<DP>& off, uint32_t stat,
-                                         const Frags16<Planes<T>::N, DP>& kf, const Frags16<Planes<T>::N, DP>& vf, uint32_t vat, float c, bool part, int r0,
+                                         const Frags16<Planes<T>::N, DP>& kf, const Frags16<Planes<T>::N, DP>& vf, uint32_t vat, float c, bool moved, bool part, int r0,
                                          int rlo, int rhi, int lane) {
   using W = RowWalk<T, DP>;
   constexpr int NC = G16<DP>::NC, STEPS = DP / 16;
@@ -1526,10 +1626,18 @@ __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP 
       if (row < rlo || row > rhi) x[e] = 0.f;
     }
   };
-  rows16<W::N, DP, A, W::PLANE>(acc, off, kf, [&](int k) {
+  rows16<W::N, DP, A, W::PLANE, true>(acc, off, kf, [&](int k) {
 #pragma unroll
     for (int e = k * 4 / NC; e < (k + 1) * 4 / NC; ++e) l4[e] = lds_ld16(stat + ST + 32 * e);
   });
+  if (__builtin_expect(moved, 0)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const u32x4 m4 = lds_ld16(stat + ST + 256 + 32 * e);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[4 * e + x] -= __uint_as_float(m4[x]);
+    }
+  }
   // the exponentials stand between the products for dP, the score gradients between those for dV
   auto exps = [&](int k) {
 #pragma unroll
@@ -1624,7 +1732,7 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
       t1 = min(t1, t0 + per);
       const T* qb = (const T*)a.q + b * a.q_bs + (long)hk * a.G * a.q_hs;
       const T* db = (const T*)a.dout + b * a.do_bs + (long)hk * a.G * a.do_hs;
-      const float* stat = a.stat + (long)bh * a.ntiles32 * 64;
+      const float* stat = a.stat + (long)bh * a.ntiles32 * kStat;
       const int rend = s.ql * a.G;
       constexpr bool STAGES = !(W::VLDS && ROLE == kOnlyDk);
       PackedStager<T, DP, W::RS, W::STAGERS> sq, sd;
@@ -1634,12 +1742,15 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
         sd.load(at + W::TILE, db, a.do_ts, a.do_hs, a.G, t * W::RS, rend, a.D, wave, lane);
       };
       auto load_stat = [&](int t, uint32_t at) {
-        if (wave == 0) dma16(at + W::STAT, lane < W::RS / 2 ? lane * 16u : kOutside, make_srd(stat + (long)t * (2 * W::RS)));
+        if (wave == 0) dma16(at + W::STAT, lane < W::RS / 32 * (kStat / 4) ? lane * 16u : kOutside, make_srd(stat + (long)t * (W::RS / 32 * kStat)));
       };
       if (t0 < t1) {
         load(t0, lds);
         load_stat(t0, lds);
       }
+      bool moved = false;                                                  // scores of any of these rows, see kStat
+      for (int x = t0 * NB + lane; x < t1 * NB; x += 64) moved |= stat[(long)x * kStat + 96] != 0.f;
+      moved = __ballot(moved) != 0;
       Frags16<N, DP> kf, vf;
       const uint32_t vat = lds + W::VF + kw * (N * G16<DP>::NC * 1024) + 16 * lane;
       load_frags16<T, DP>(kf, (const T*)a.k + b * a.k_bs + (long)j * a.k_ts + hk * a.k_hs, key_ok, a.D, lane);
@@ -1662,7 +1773,7 @@ __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_wa
           constexpr int B32 = decltype(k)::value;
           const int r0 = t * W::RS + 32 * B32;
           if ((far && NB > 1 && kw / KB != B32) || r0 >= wr1 || r0 + 32 <= wr0) return;
-          dkv_step<T, DP, S0 + B32 * 32 * G16<DP>::PITCH, S0 + B32 * 256, ROLE>(dk, dv, off, stat_off, kf, vf, vat, c, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
+          dkv_step<T, DP, S0 + B32 * 32 * G16<DP>::PITCH, S0 + B32 * kStat * 4, ROLE>(dk, dv, off, stat_off, kf, vf, vat, c, moved, r0 < fr0 || r0 + 32 > fr1, r0, rlo, rhi, lane);
         };
         sub(std::integral_constant<int, 0>());
         if constexpr (NB == 2) sub(std::integral_constant<int, 1>());
@@ -1962,7 +2073,7 @@ int shares(int64_t wgs, int64_t stages, int64_t dp, int64_t bytes, int es) {
 BwdPlan plan_backward(const WaArgs& a, int es) {
   BwdPlan p{};
   const int64_t rows = (int64_t)a.Tq * a.G, bh = (int64_t)a.B * a.Hkv, dp = padded(a.D);
-  p.stat_bytes = bh * ((rows + 127) / 128) * 128 * 2 * 4;
+  p.stat_bytes = bh * ((rows + 127) / 128) * 4 * kStat * 4;
   const int64_t keys = ((int64_t)a.Tk + 127) / 128, tiles = (rows + 127) / 128;
   // dK / dV, bf16, 4096 tokens, 8 / 1 heads of 128 channels, causal (32 workgroups without shares): 1112 -> 173 us and 7 to join; 4 x 955, 16 / 4 heads
   // of 64 (128 workgroups): 148 -> 51 and 8; fp32, 2048, 8 / 1 heads of 64, causal (16 workgroups): 2029 -> 82 and 7.  dQ of the last (128
