@@ -170,3 +170,33 @@ def test_gradients_of_large_scores(form, size, dtype):
     B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
     q, table, which, v, do = _sized(B, Tq, Tk, Hq, Hkv, D, size, dtype, Tk, 17)
     _compare(R.attention(q, table, v, R.seen(B, Tq, Tk, left, right, sinks), dout=do), q, table, v, do, (left, right, sinks))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("size", [1.0, 1e10])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("form", [(2, 130, 130, 2, 2, 32, 17, 9, 4), (1, 900, 900, 8, 1, 64, 400, 0, 3), (80, 150, 150, 4, 2, 64, 20, 2, 3), (40, 140, 140, 8, 4, 128, 50, 0, 40),
+                                  (2, 1, 700, 4, 2, 128, 20, 2, 3)])
+def test_what_is_not_seen_does_not_reach_a_row_of_huge_scores(form, bad, size, dtype):
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    A = _att()
+    q, table, which, v, do = _sized(B, Tq, Tk, Hq, Hkv, D, size, dtype, Tk if size == 1 else 8, 23)
+    k = table[:, which].contiguous()
+    kl = torch.full((B,), Tk - 11, dtype=torch.int32)
+    ql = torch.full((B,), max(1, Tq - 11), dtype=torch.int32)
+    ok = R.seen(B, Tq, Tk, left, right, sinks, ql, kl)
+    q = q if size == 1 else _settled(q, table, which, ok, size, 23)
+    ref = R.attention(q, k, v, ok, dout=do) if size == 1 else _peaked(q, table, which, v, ok, do)
+    for t in (k, v):
+        t[:, Tk - 11:] = bad
+    for t in (q, do):
+        t[:, int(ql[0]):] = bad
+    _compare(ref, q, k, v, do, (left, right, sinks), q_lens=ql.cuda(), k_lens=kl.cuda())
+    # a value that some rows see: the others keep their results, and so do keys that none of these rows sees
+    v[:, 60], hit = bad, ok[0, :, 60]
+    far = ~ok[0][hit].any(0)
+    x = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out = A.window_attention(*x, left, right, sinks, ql.cuda(), kl.cuda())
+    got = (out,) + torch.autograd.grad(out, x, do.cuda())
+    for name, g, keep in zip(("out", "dq", "dk", "dv"), got, (~hit, ~hit, far, far)):
+        R.check(f"{name}, {bad} in a value", g[:, keep], ref[name][0][:, keep], ref[name][1][:, keep])

@@ -665,38 +665,58 @@ __device__ __forceinline__ void store_out(const WaArgs& a, int b, int i, long hq
   }
 }
 
+// What is computed from `lane` from here on is computed here, not kept in registers from where the kernel's loops computed it
+__device__ __forceinline__ void fresh(int& lane) { asm volatile("" : "+v"(lane)); }
+
 // A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN.  A row whose sum of exponentials is
-// a number but whose result is not is therefore taken again, over the keys it sees alone: one wave, its lanes split the channels.
+// a number but whose result is not is therefore taken again, over the keys it sees alone: one wave, 32 keys at a time, their scores' maximum and sum first,
+// so that the probabilities sum to 1 whatever the scores; then its lanes split the channels.
 template <typename T>
-__device__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int i, int g, float m, float l, int lane) {
+__device__ __forceinline__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int r, int lane) {
+  fresh(lane);
+  const int i = r / a.G, g = r - i * a.G;
   const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + (long)(hk * a.G + g) * a.q_hs;
   const T* k = (const T*)a.k + b * a.k_bs + hk * a.k_hs;
   const T* v = (const T*)a.v + b * a.v_bs + hk * a.v_hs;
   const long hq = (long)(hk * a.G + g);
   T* o = (T*)a.out + b * a.o_bs + i * a.o_ts + hq * a.o_hs;
   const int p = i + s.shift, hi = min(p + a.right, s.kl - 1), lo = max(p - a.left, 0);
-  const int d0 = lane, d1 = lane + 64;
-  const float q0 = d0 < a.D ? Elem<T>::ld(q + d0) : 0.f, q1 = d1 < a.D ? Elem<T>::ld(q + d1) : 0.f;
   const float c = a.scale * kLog2e;
-  float o0 = 0.f, o1 = 0.f;
-  for (int j = 0; j <= hi; ++j) {
-    if (j < lo && j >= a.sinks) j = lo;
-    if (j > hi) break;
-    const T *kr = k + j * a.k_ts, *vr = v + j * a.v_ts;
-    float d = (d0 < a.D ? q0 * Elem<T>::ld(kr + d0) : 0.f) + (d1 < a.D ? q1 * Elem<T>::ld(kr + d1) : 0.f);
-    d = wave_sum(d);
-    const float w = __builtin_amdgcn_exp2f((d - m) * c);
-    if (d0 < a.D) o0 = fmaf(w, Elem<T>::ld(vr + d0), o0);
-    if (d1 < a.D) o1 = fmaf(w, Elem<T>::ld(vr + d1), o1);
-  }
+  const Tiles t = tiles_of(a, s, p, p, 32);
+  const int d0 = lane, d1 = lane + 64;
+  const bool on0 = d0 < a.D, on1 = d1 < a.D;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int it = 0; it < t.na + t.nb; ++it) {
+      const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
+      const bool seen = j <= hi && (j >= lo || j < a.sinks);
+      const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
+      if (pass == 0) {
+        const float top = fmaxf(wave_max(seen ? sc : -INFINITY), m);
+        if (top == -INFINITY) continue;
+        l = l * __builtin_amdgcn_exp2f((m - top) * c) + 0.5f * wave_sum(seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f);   // (both halves hold the keys)
+        m = top;
+        continue;
+      }
+      const float w = seen ? __builtin_amdgcn_exp2f((sc - m) * c) : 0.f;
+      const uint32_t mask = (uint32_t)__ballot(seen);
+#pragma unroll 4
+      for (int n = 0; n < 32; ++n) {
+        const T* vr = v + (long)(j0 + n) * a.v_ts;
+        const bool in = mask >> n & 1;
+        const float wn = __shfl(w, n, 64), v0 = in && on0 ? Elem<T>::ld(vr + d0) : 0.f, v1 = in && on1 ? Elem<T>::ld(vr + d1) : 0.f;
+        o0 = fmaf(wn, v0, o0);
+        o1 = fmaf(wn, v1, o1);
+      }
+    }
   o0 /= l, o1 /= l;
-  if (d0 < a.D) o[d0] = (T)o0;
-  if (d1 < a.D) o[d1] = (T)o1;
+  if (on0) o[d0] = (T)o0;
+  if (on1) o[d1] = (T)o1;
   if constexpr (sizeof(T) == 2) {
     if (a.out_lo) {
       __bf16* r = a.out_lo + (((long)b * a.Tq + i) * (a.Hkv * a.G) + hq) * a.D;
-      if (d0 < a.D) r[d0] = (__bf16)(o0 - (float)(__bf16)o0);
-      if (d1 < a.D) r[d1] = (__bf16)(o1 - (float)(__bf16)o1);
+      if (on0) r[d0] = (__bf16)(o0 - (float)(__bf16)o0);
+      if (on1) r[d1] = (__bf16)(o1 - (float)(__bf16)o1);
     }
   }
 }
@@ -884,7 +904,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
   while (again) {
     const int n = __builtin_ctzll(again);
     again &= again - 1;
-    row_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(m, n, 64), __shfl(l, n, 64), lane);
+    row_again<T>(a, s, b, hk, rw + n, lane);
   }
 #endif
 }
@@ -1019,7 +1039,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
     while (again) {
       const int n = __builtin_ctzll(again);
       again &= again - 1;
-      row_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(m, n, 64), __shfl(l, n, 64), lane);
+      row_again<T>(a, s, b, hk, r0 + n, lane);
     }
     return;
   }
@@ -1084,7 +1104,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
     while (again) {                                                              // D4 (8 .. 32) lanes hold a row
       const int f = __builtin_ctzll(again), row_lane = f - f % D4;
       again &= ~(((D4 == 64 ? 0ull : (1ull << D4)) - 1) << row_lane);
-      row_again<T>(a, s, b, hk, __shfl(ii, f, 64), __shfl(gg, f, 64), __shfl(mm, f, 64), __shfl(ll, f, 64), lane);
+      row_again<T>(a, s, b, hk, __builtin_amdgcn_readlane(rr, f), lane);
     }
   }
 #endif
@@ -1157,7 +1177,7 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
   }
   if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store_out<T>(a, b, i, hk * a.G + g, 4 * threadIdx.x, v);
   if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L) : -INFINITY;
-  if (__ballot(bad && ok && L == L)) row_again<T>(a, s, b, hk, i, g, M, L, threadIdx.x);
+  if (__ballot(bad && ok && L == L)) row_again<T>(a, s, b, hk, rr, threadIdx.x);
 #endif
 }
 
@@ -1221,7 +1241,9 @@ __device__ __forceinline__ void rows_max_sum(const WaArgs& a, const Seq& s, cons
 // The gradient of one query row, over the keys it sees alone (see row_again), 32 at a time: their scores' maximum and sum first, so that the probabilities sum
 // to 1 whatever the scores
 template <typename T>
-__device__ __forceinline__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int i, int g, float delta, int lane) {
+__device__ __forceinline__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int r, float delta, int lane) {
+  fresh(lane);
+  const int i = r / a.G, g = r - i * a.G;
   const long hq = (long)(hk * a.G + g);
   const T* q = (const T*)a.q + b * a.q_bs + i * a.q_ts + hq * a.q_hs;
   const T* dO = (const T*)a.dout + b * a.do_bs + i * a.do_ts + hq * a.do_hs;
@@ -1240,8 +1262,7 @@ __device__ __forceinline__ void dq_again(const WaArgs& a, const Seq& s, int b, i
       const bool seen = j <= hi && (j >= lo || j < a.sinks);
       const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
       if (pass == 0) {
-        float top = seen ? sc : -INFINITY;
-        top = fmaxf(wave_max(top), m);
+        const float top = fmaxf(wave_max(seen ? sc : -INFINITY), m);
         if (top == -INFINITY) continue;
         l = l * __builtin_amdgcn_exp2f((m - top) * c) + 0.5f * wave_sum(seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f);   // (both halves hold the keys)
         m = top;
@@ -1427,7 +1448,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
   while (again) {
     const int n = __builtin_ctzll(again);
     again &= again - 1;
-    dq_again<T>(a, s, b, hk, __shfl(i, n, 64), __shfl(g, n, 64), __shfl(delta, n, 64), lane);
+    dq_again<T>(a, s, b, hk, rw + n, __shfl(delta, n, 64), lane);
   }
 #endif
 }
@@ -1461,7 +1482,7 @@ __global__ __launch_bounds__(256) void window_attn_dq_join_kernel(const WaArgs a
   }
   const float* stat = a.stat + ((long)bh * a.ntiles32 + (r >> 5)) * kStat + (r & 31);
   const float lse2 = stat[0], delta = stat[32];
-  if (__ballot(bad) && lse2 == lse2 && delta == delta) dq_again<T>(a, s, b, hk, i, g, delta, lane);
+  if (__ballot(bad) && lse2 == lse2 && delta == delta) dq_again<T>(a, s, b, hk, r, delta, lane);
 #endif
 }
 
@@ -1527,6 +1548,7 @@ struct PackedStager<float, DP, ROWS, NW> {
 // The gradients of one key (and value) row over the query rows that see it alone (see row_again), 32 at a time, with scores in the bits of dQ's
 template <typename T>
 __device__ __forceinline__ void dkv_again(const WaArgs& a, const Seq& s, int b, int hk, int j, int lane, bool want_dk, bool want_dv) {
+  fresh(lane);
   const T* k = (const T*)a.k + b * a.k_bs + j * a.k_ts + hk * a.k_hs;
   const T* v = (const T*)a.v + b * a.v_bs + j * a.v_ts + hk * a.v_hs;
   const int d0 = lane, d1 = lane + 64;
