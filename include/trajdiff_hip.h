@@ -451,7 +451,7 @@ int tdx_rotary_axes(const tdx_rotary_desc* host_desc, void* stream);
  *   out = softmax over the seen keys of (scale q k^T) times v,   lse = log sum exp of the same scores (natural logarithm, fp32),
  * rows that see nothing (rows i >= q_len among them) get out = 0 and lse = -inf.  q_lens / k_lens: device int32 (B), or NULL = Tq / Tk;
  * values are clamped to [0, Tq] / [0, Tk].  What is stored at keys that a row does not see (infinities and NaN too) does not reach it.
- * D: a multiple of 8, at most 128; scale finite and > 0; pointers, and the byte sizes of the strides, multiples of 16; the token stride
+ * D: a multiple of 8, at most 128; scale finite, also times log2 e, and > 0; pointers, and the byte sizes of the strides, multiples of 16; the token stride
  * of k and v below 16 MiB; 65 token strides plus one group of head strides of q (and of dout) below 2 GiB.
  * Softmax statistics and sums are fp32; with bf16 tensors the probabilities (and score gradients) are rounded to bf16 before the
  * products that take them, the results once at the end.  Summation orders are fixed: results are reproducible. */

@@ -200,3 +200,16 @@ def test_what_is_not_seen_does_not_reach_a_row_of_huge_scores(form, bad, size, d
     got = (out,) + torch.autograd.grad(out, x, do.cuda())
     for name, g, keep in zip(("out", "dq", "dk", "dv"), got, (~hit, ~hit, far, far)):
         R.check(f"{name}, {bad} in a value", g[:, keep], ref[name][0][:, keep], ref[name][1][:, keep])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("scale", [1.2e-38, 1e-39, 3e-42, 1.5e-45])
+@pytest.mark.parametrize("form", [(2, 13, 13, 2, 2, 64, 5, 2, 1), (1, 1, 3000, 2, 2, 64, None, 0, 0), (80, 150, 150, 4, 2, 64, 20, 2, 3), (1, 900, 900, 8, 1, 32, 400, 0, 3)])
+def test_the_smallest_scales(form, scale, dtype):
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    q, k, v, do = (_normal(B, T, H, D, seed=n) for n, (T, H) in enumerate(((Tq, Hq), (Tk, Hkv), (Tk, Hkv), (Tq, Hq))))
+    # Products of up to 1e38.  A scale below 2^-126 holds fewer bits: scale log2 e is off by half a step of 2^-149, which at these scores (3e37 scale, times 5
+    # at most) is below 2^-23 and so part of what the bound gives exponentials (2^-20).
+    q, k, v, do = (q * 2e18).to(dtype), (k * 2e18).to(dtype), v.to(dtype), do.to(dtype)
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    _compare(R.attention(q, k, v, R.seen(B, Tq, Tk, left, right, sinks), scale=scale, dout=do), q, k, v, do, (left, right, sinks), scale=scale)

@@ -151,3 +151,17 @@ def test_shared_bytes_are_told_from_bytes_between_each_other():
         assert A._touch(*views) == bool(held[0] & held[1])
         found[bool(held[0] & held[1])] += 1
     assert min(found) > 50
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38, float("inf"), 1e39])
+def test_scales_that_leave_32_bits_are_refused(scale):
+    """Exponents are formed as 2^(s scale log2 e)."""
+    import ctypes as C
+
+    from test_sequence_cpu import P, _attn_desc
+
+    from trajectorydiffusion_amd import _lib
+    lib = _lib.lib()
+    for d, f in ((_attn_desc(scale=scale), lib.tdx_window_attention), (_attn_desc(scale=scale, ws=16 * P, ws_bytes=1 << 40), lib.tdx_window_attention_bwd)):
+        assert f(C.byref(d), None) == 1 and b"scale" in lib.tdx_last_error()
+    assert lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(scale=2.3e38))) > 0

@@ -578,6 +578,7 @@ __device__ __forceinline__ int seen_class(const WaArgs& a, const Seq& s, int j0,
 // m is the running maximum of the raw scores that the exponents are taken against.  It follows the true maximum only when that is more
 // than 8 powers of two above it: the terms stay below 2^8, nothing is lost in fp32 (nor in bf16, whose exponent is as wide), and the
 // accumulators are rescaled in the first tiles of a row only.
+__device__ __forceinline__ float softmax_slack(float c) { return fminf(8.0f / c, 3.4e38f); }   // (a number: a row without a maximum, m = -inf, is below every score)
 // Takes the maximum t of new scores into m (rescaling l and o); returns m c, what the exponents are taken against
 template <int ND>
 __device__ __forceinline__ float softmax_follow(float t, float& m, float& l, f32x16 (&o)[ND], float c, float slack) {
@@ -813,7 +814,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = -INFINITY, l = 0.f;
-  const float c = a.scale * kLog2e, slack = 8.0f / c;
+  const float c = a.scale * kLog2e, slack = softmax_slack(c);
   if (r0 < rend) {
     Frags16<N, DP> qf;
     load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
@@ -955,7 +956,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = -INFINITY, l = 0.f;
-  const float c = a.scale * kLog2e, slack = 8.0f / c;
+  const float c = a.scale * kLog2e, slack = softmax_slack(c);
   if (r0 < rend) {
     Frags16<Planes<T>::N, DP> qf;
     load_frags16<T, DP>(qf, (const T*)a.q + b * a.q_bs + (long)i * a.q_ts + (long)(hk * a.G + g) * a.q_hs, row_ok, a.D, lane);
@@ -1958,7 +1959,7 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
                 d->B, d->Tq, d->Tk, d->Hq, d->Hkv);
   TDX_CHECK_ARG(d->Tq < (1 << 28) && d->Tk < (1 << 28) && (int64_t)d->Tq * (d->Hq / d->Hkv) < (1 << 30), "%s: Tq=%d Tk=%d are too long", fn, d->Tq, d->Tk);
   TDX_CHECK_ARG(d->D >= 8 && d->D <= 128 && d->D % 8 == 0, "%s: D=%d (a multiple of 8, at most 128)", fn, d->D);
-  TDX_CHECK_ARG(std::isfinite(d->scale) && d->scale > 0.f, "%s: scale=%g (finite, > 0)", fn, (double)d->scale);
+  TDX_CHECK_ARG(std::isfinite(d->scale) && d->scale > 0.f && std::isfinite(d->scale * kLog2e), "%s: scale=%g (finite, also times log2 e, > 0)", fn, (double)d->scale);
   TDX_CHECK_ARG(d->sinks >= 0, "%s: sinks=%d", fn, d->sinks);
   const int es = d->dtype == TDX_F32 ? 4 : 2;
   a = WaArgs{};
