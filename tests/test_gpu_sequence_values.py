@@ -213,3 +213,48 @@ def test_the_smallest_scales(form, scale, dtype):
     q, k, v, do = (q * 2e18).to(dtype), (k * 2e18).to(dtype), v.to(dtype), do.to(dtype)
     scale = float(torch.tensor(scale, dtype=torch.float32))
     _compare(R.attention(q, k, v, R.seen(B, Tq, Tk, left, right, sinks), scale=scale, dout=do), q, k, v, do, (left, right, sinks), scale=scale)
+
+
+# ---- values next to the largest --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("form", [(2, 13, 13, 2, 2, 64, None, None, 0), (1, 1, 3000, 2, 2, 64, None, 0, 0), (1, 70, 70, 4, 2, 64, 5, 0, 3), (80, 150, 150, 4, 2, 64, 20, 2, 3),
+                                  (40, 140, 140, 8, 4, 128, 50, 0, 40), (300, 130, 130, 1, 1, 32, 33, 20, 5)])
+def test_averages_of_values_next_to_the_largest(form, dtype):
+    """A weighted mean of numbers is a number, also where the sum of them all is none."""
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    A = _att()
+    q, k, v = (_normal(B, T, H, D, seed=n, dtype=dtype) for n, (T, H) in enumerate(((Tq, Hq), (Tk, Hkv), (Tk, Hkv))))
+    most = 3.4e38 if dtype == torch.float32 else 3.0e38
+    for v in (torch.full_like(v, most), (v.float().sign() * most).to(dtype), (v.float() * 1e37).to(dtype)):
+        ref = R.attention(q, k, v, R.seen(B, Tq, Tk, left, right, sinks))
+        R.check("out", A.window_attention(q.cuda(), k.cuda(), v.cuda(), left, right, sinks), *ref["out"])
+
+
+@pytest.mark.parametrize("form", [(2, 13, 13, 2, 2, 64), (80, 150, 150, 4, 4, 64), (40, 140, 140, 8, 8, 128), (300, 130, 130, 1, 1, 32), (1, 900, 900, 1, 1, 64)])
+def test_fp32_numbers_between_the_largest_of_bf16_and_of_fp32(form):
+    """In every operand in turn, its partner small: each row sees one key, so dv is dout."""
+    B, Tq, Tk, Hq, Hkv, D = form
+    parts = [_normal(B, T, H, D, seed=n) for n, (T, H) in enumerate(((Tq, Hq), (Tk, Hkv), (Tk, Hkv), (Tq, Hq)))]
+    small = lambda t: t * 2.0 ** -100                                                       # noqa: E731
+    big = lambda t: torch.where(t > 0, 3.4e38, -3.395e38) * torch.where(t.abs() < 1, 1.0, 0.5)   # noqa: E731
+    ok = R.seen(B, Tq, Tk, 0, 0, 0)
+    for forms in ((big, small, None, None), (small, big, None, None), (None, None, big, small), (None, None, small, big)):
+        q, k, v, do = (t if f is None else f(t) for f, t in zip(forms, parts))
+        scale = 2.0 ** -30 if forms[0] else D ** -0.5
+        _compare(R.attention(q, k, v, ok, scale=scale, dout=do), q, k, v, do, (0, 0, 0), scale=scale)
+
+
+@pytest.mark.parametrize("form", [(2, 13, 13, 2, 2, 64, 5, 2, 1), (80, 150, 150, 4, 2, 64, 20, 2, 3), (40, 140, 140, 8, 4, 128, 50, 0, 40)])
+def test_fp32_numbers_next_to_the_smallest(form):
+    """Around 2^-118 the second and third bf16 plane of a number have exponents below bf16's normal numbers, whose step is 2^-133: half of it is lost of each
+    number.  As q (k 2^118 times as large) that is 2^-16 sum |k| scale of a score, below 2^-13 here, so 2^-12 of a probability, once more for their sum."""
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    q, k, v = (_normal(B, T, H, D, seed=n) for n, (T, H) in enumerate(((Tq, Hq), (Tk, Hkv), (Tk, Hkv))))
+    ok = R.seen(B, Tq, Tk, left, right, sinks)
+    A = _att()
+    tiny = 2.0 ** -118
+    assert float(k.abs().sum(-1).max()) * D ** -0.5 < 8 * 1.6
+    for f, more in (((tiny, 1 / tiny, 1), 2.0 ** -11 * float(v.abs().max())), ((1 / tiny, tiny, 1), 2.0 ** -11 * float(v.abs().max())), ((1, 1, tiny), 2.0 ** -133)):
+        x = [t * n for t, n in zip((q, k, v), f)]
+        want, bound = R.attention(*x, ok)["out"]
+        R.check(f"out {f}", A.window_attention(*(t.cuda() for t in x), left, right, sinks), want, bound + more)

@@ -306,16 +306,22 @@ __device__ __forceinline__ void rows16(f32x16& acc, const LaneOff<DP>& off, cons
     pin();
   }
 }
-// x as N bf16 planes; an infinity (or what rounds to one) is the first plane alone
+// x as N bf16 planes.  The first is bf16's largest number where fp32's are larger still, so that every number is the sum of its planes; an infinity
+// has one that is NaN, and so have its products
 template <int N>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[N]) {
-  u32x4 w = Elem<__bf16>::pack(x);
-  p[0] = __builtin_bit_cast(bf16x8, w);
-  if constexpr (N == 3) {
+  if constexpr (N == 1) {
+    p[0] = __builtin_bit_cast(bf16x8, Elem<__bf16>::pack(x));
+  } else {
+    constexpr float most = 0x1.fep127f;
     float h[8], r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __builtin_amdgcn_fmed3f(x[i], -most, most);
+    u32x4 w = Elem<__bf16>::pack(r);
+    p[0] = __builtin_bit_cast(bf16x8, w);
     Elem<__bf16>::unpack(w, h);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = x[i] - h[i], r[i] = __builtin_fabsf(r[i]) < INFINITY ? r[i] : 0.f;
+    for (int i = 0; i < 8; ++i) r[i] = x[i] - h[i];
     w = Elem<__bf16>::pack(r);
     p[1] = __builtin_bit_cast(bf16x8, w);
     Elem<__bf16>::unpack(w, h);
@@ -669,9 +675,10 @@ __device__ __forceinline__ void store_out(const WaArgs& a, int b, int i, long hq
 // What is computed from `lane` from here on is computed here, not kept in registers from where the kernel's loops computed it
 __device__ __forceinline__ void fresh(int& lane) { asm volatile("" : "+v"(lane)); }
 
-// A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN.  A row whose sum of exponentials is
-// a number but whose result is not is therefore taken again, over the keys it sees alone: one wave, 32 keys at a time, their scores' maximum and sum first,
-// so that the probabilities sum to 1 whatever the scores; then its lanes split the channels.
+// A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN; and sums of exponentials (up to 2^8 each) times values next
+// to the largest are infinite where their mean is not.  A row whose sum of exponentials is a number but whose result is not, or is infinite, is therefore taken
+// again, over the keys it sees alone: one wave, 32 keys at a time, a running mean (whose weights sum to 1 whatever the scores, so that it never leaves the range
+// of its values), the lanes split the channels.
 template <typename T>
 __device__ __forceinline__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int r, int lane) {
   fresh(lane);
@@ -687,30 +694,26 @@ __device__ __forceinline__ void row_again(const WaArgs& a, const Seq& s, int b, 
   const int d0 = lane, d1 = lane + 64;
   const bool on0 = d0 < a.D, on1 = d1 < a.D;
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int pass = 0; pass < 2; ++pass)
-    for (int it = 0; it < t.na + t.nb; ++it) {
-      const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
-      const bool seen = j <= hi && (j >= lo || j < a.sinks);
-      const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
-      if (pass == 0) {
-        const float top = fmaxf(wave_max(seen ? sc : -INFINITY), m);
-        if (top == -INFINITY) continue;
-        l = l * __builtin_amdgcn_exp2f((m - top) * c) + 0.5f * wave_sum(seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f);   // (both halves hold the keys)
-        m = top;
-        continue;
-      }
-      const float w = seen ? __builtin_amdgcn_exp2f((sc - m) * c) : 0.f;
-      const uint32_t mask = (uint32_t)__ballot(seen);
+  for (int it = 0; it < t.na + t.nb; ++it) {
+    const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
+    const bool seen = j <= hi && (j >= lo || j < a.sinks);
+    const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
+    const float top = fmaxf(wave_max(seen ? sc : -INFINITY), m);
+    if (top == -INFINITY) continue;
+    float w = seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f;
+    const float was = l * __builtin_amdgcn_exp2f((m - top) * c);
+    l = was + 0.5f * wave_sum(w);                                          // (both lane halves hold the keys)
+    m = top, w /= l, o0 *= was / l, o1 *= was / l;
+    const uint32_t mask = (uint32_t)__ballot(seen);
 #pragma unroll 4
-      for (int n = 0; n < 32; ++n) {
-        const T* vr = v + (long)(j0 + n) * a.v_ts;
-        const bool in = mask >> n & 1;
-        const float wn = __shfl(w, n, 64), v0 = in && on0 ? Elem<T>::ld(vr + d0) : 0.f, v1 = in && on1 ? Elem<T>::ld(vr + d1) : 0.f;
-        o0 = fmaf(wn, v0, o0);
-        o1 = fmaf(wn, v1, o1);
-      }
+    for (int n = 0; n < 32; ++n) {
+      const T* vr = v + (long)(j0 + n) * a.v_ts;
+      const bool in = mask >> n & 1;
+      const float wn = __shfl(w, n, 64), v0 = in && on0 ? Elem<T>::ld(vr + d0) : 0.f, v1 = in && on1 ? Elem<T>::ld(vr + d1) : 0.f;
+      o0 = fmaf(wn, v0, o0);
+      o1 = fmaf(wn, v1, o1);
     }
-  o0 /= l, o1 /= l;
+  }
   if (on0) o[d0] = (T)o0;
   if (on1) o[d1] = (T)o1;
   if constexpr (sizeof(T) == 2) {
@@ -894,7 +897,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
-          bad |= v[x] != v[x];
+          bad |= !(__builtin_fabsf(v[x]) < INFINITY);
         }
         if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
       }
@@ -1029,7 +1032,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
-            bad |= v[x] != v[x];
+            bad |= !(__builtin_fabsf(v[x]) < INFINITY);
           }
           if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
         }
@@ -1096,7 +1099,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         v[x] = inv != 0.f ? oo[x] * inv : (ll != ll ? ll : 0.f);
-        bad |= v[x] != v[x];
+        bad |= !(__builtin_fabsf(v[x]) < INFINITY);
       }
       if (d < a.D) store_out<T>(a, b, ii, hk * a.G + gg, d, v);
       if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? mm * a.scale + __logf(ll) : -INFINITY;
@@ -1174,7 +1177,7 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     v[x] = inv != 0.f ? O[x] * inv : (L != L ? L : 0.f);
-    bad |= v[x] != v[x];
+    bad |= !(__builtin_fabsf(v[x]) < INFINITY);
   }
   if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store_out<T>(a, b, i, hk * a.G + g, 4 * threadIdx.x, v);
   if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L) : -INFINITY;
