@@ -258,3 +258,21 @@ def test_fp32_numbers_next_to_the_smallest(form):
         x = [t * n for t, n in zip((q, k, v), f)]
         want, bound = R.attention(*x, ok)["out"]
         R.check(f"out {f}", A.window_attention(*(t.cuda() for t in x), left, right, sinks), want, bound + more)
+
+
+# ---- a value that is not a number in a long causal sequence -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_one_channel_of_one_value_spoils_one_channel_of_its_rows(bad, dtype):
+    A = _att()
+    B, T, H, D = 2, 1500, 8, 64
+    q, k, v = (_normal(B, T, H, D, dtype=dtype, seed=n) for n in range(3))
+    ref = R.attention(q, k, v, R.seen(B, T, T, None, 0, 0))["out"]
+    v[:, 700, :, 5] = bad
+    out = A.window_attention(q.cuda(), k.cuda(), v.cuda(), None, 0).cpu()
+    keep = torch.ones(T, D, dtype=torch.bool)
+    keep[700:, 5] = False
+    for b in range(B):
+        for h in range(H):
+            R.check("out", out[b, :, h][keep], ref[0][b, :, h][keep], ref[1][b, :, h][keep])
+            assert not torch.isfinite(out[b, 700:, h, 5]).any()

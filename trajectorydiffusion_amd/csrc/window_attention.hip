@@ -675,6 +675,14 @@ __device__ __forceinline__ void store_out(const WaArgs& a, int b, int i, long hq
 // What is computed from `lane` from here on is computed here, not kept in registers from where the kernel's loops computed it
 __device__ __forceinline__ void fresh(int& lane) { asm volatile("" : "+v"(lane)); }
 
+// Whether a channel that this wave has stored is no number (the again-functions' channels to take: the others are right, and a channel that is NaN over what is
+// seen stays so, which ends the walk)
+template <typename T>
+__device__ __forceinline__ bool no_number(const T* at, bool on) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  return on && !(__builtin_fabsf(Elem<T>::ld(at)) < INFINITY);
+}
+
 // A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN; and sums of exponentials (up to 2^8 each) times values next
 // to the largest are infinite where their mean is not.  A row whose sum of exponentials is a number but whose result is not, or is infinite, is therefore taken
 // again, over the keys it sees alone: one wave, 32 keys at a time, a running mean (whose weights sum to 1 whatever the scores, so that it never leaves the range
@@ -692,7 +700,7 @@ __device__ __forceinline__ void row_again(const WaArgs& a, const Seq& s, int b, 
   const float c = a.scale * kLog2e;
   const Tiles t = tiles_of(a, s, p, p, 32);
   const int d0 = lane, d1 = lane + 64;
-  const bool on0 = d0 < a.D, on1 = d1 < a.D;
+  const bool on0 = no_number<T>(o + min(d0, a.D - 1), d0 < a.D), on1 = no_number<T>(o + min(d1, a.D - 1), d1 < a.D);
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int it = 0; it < t.na + t.nb; ++it) {
     const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
@@ -713,6 +721,7 @@ __device__ __forceinline__ void row_again(const WaArgs& a, const Seq& s, int b, 
       o0 = fmaf(wn, v0, o0);
       o1 = fmaf(wn, v1, o1);
     }
+    if (__all((!on0 || o0 != o0) && (!on1 || o1 != o1))) break;
   }
   if (on0) o[d0] = (T)o0;
   if (on1) o[d1] = (T)o1;
@@ -1242,8 +1251,7 @@ __device__ __forceinline__ void rows_max_sum(const WaArgs& a, const Seq& s, cons
   l = half_sum(l);
 }
 
-// The gradient of one query row, over the keys it sees alone (see row_again), 32 at a time: their scores' maximum and sum first, so that the probabilities sum
-// to 1 whatever the scores
+// The gradient of one query row, over the keys it sees alone (see row_again), 32 at a time, with weights that sum to 1 whatever the scores
 template <typename T>
 __device__ __forceinline__ void dq_again(const WaArgs& a, const Seq& s, int b, int hk, int r, float delta, int lane) {
   fresh(lane);
@@ -1258,32 +1266,30 @@ __device__ __forceinline__ void dq_again(const WaArgs& a, const Seq& s, int b, i
   const float c = a.scale * kLog2e;
   const Tiles t = tiles_of(a, s, p, p, 32);
   const int d0 = lane, d1 = lane + 64;
-  const bool on0 = d0 < a.D, on1 = d1 < a.D;
+  const bool on0 = no_number<T>(dq + min(d0, a.D - 1), d0 < a.D), on1 = no_number<T>(dq + min(d1, a.D - 1), d1 < a.D);
   float m = -INFINITY, l = 0.f, r0 = 0.f, r1 = 0.f;
-  for (int pass = 0; pass < 2; ++pass)
-    for (int it = 0; it < t.na + t.nb; ++it) {
-      const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
-      const bool seen = j <= hi && (j >= lo || j < a.sinks);
-      const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
-      if (pass == 0) {
-        const float top = fmaxf(wave_max(seen ? sc : -INFINITY), m);
-        if (top == -INFINITY) continue;
-        l = l * __builtin_amdgcn_exp2f((m - top) * c) + 0.5f * wave_sum(seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f);   // (both halves hold the keys)
-        m = top;
-        continue;
-      }
-      const float dp = row_times<T>(dO, v + (long)j * a.v_ts, j < s.kl, a.D, lane);
-      const float ds = seen && l != 0.f ? __builtin_amdgcn_exp2f((sc - m) * c) / l * (dp - delta) : 0.f;
-      const uint32_t mask = (uint32_t)__ballot(seen);
+  for (int it = 0; it < t.na + t.nb; ++it) {
+    const int j0 = tile_start(t, it, 32), j = j0 + (lane & 31);
+    const bool seen = j <= hi && (j >= lo || j < a.sinks);
+    const float sc = row_times<T, true>(q, k + (long)j * a.k_ts, j < s.kl, a.D, lane);
+    const float top = fmaxf(wave_max(seen ? sc : -INFINITY), m);
+    if (top == -INFINITY) continue;
+    const float dp = row_times<T>(dO, v + (long)j * a.v_ts, j < s.kl, a.D, lane);
+    float ds = seen ? __builtin_amdgcn_exp2f((sc - top) * c) : 0.f;
+    const float was = l * __builtin_amdgcn_exp2f((m - top) * c);
+    l = was + 0.5f * wave_sum(ds);                                         // (both lane halves hold the keys)
+    m = top, ds = seen ? ds / l * (dp - delta) : 0.f, r0 *= was / l, r1 *= was / l;
+    const uint32_t mask = (uint32_t)__ballot(seen);
 #pragma unroll 4
-      for (int n = 0; n < 32; ++n) {
-        const T* kr = k + (long)(j0 + n) * a.k_ts;
-        const bool in = mask >> n & 1;
-        const float w = __shfl(ds, n, 64), k0 = in && on0 ? Elem<T>::ld(kr + d0) : 0.f, k1 = in && on1 ? Elem<T>::ld(kr + d1) : 0.f;
-        r0 = fmaf(w, k0, r0);
-        r1 = fmaf(w, k1, r1);
-      }
+    for (int n = 0; n < 32; ++n) {
+      const T* kr = k + (long)(j0 + n) * a.k_ts;
+      const bool in = mask >> n & 1;
+      const float w = __shfl(ds, n, 64), k0 = in && on0 ? Elem<T>::ld(kr + d0) : 0.f, k1 = in && on1 ? Elem<T>::ld(kr + d1) : 0.f;
+      r0 = fmaf(w, k0, r0);
+      r1 = fmaf(w, k1, r1);
     }
+    if (__all((!on0 || r0 != r0) && (!on1 || r1 != r1))) break;
+  }
   if (on0) dq[d0] = (T)(r0 * a.scale);
   if (on1) dq[d1] = (T)(r1 * a.scale);
 }
@@ -1556,7 +1562,11 @@ __device__ __forceinline__ void dkv_again(const WaArgs& a, const Seq& s, int b, 
   const T* k = (const T*)a.k + b * a.k_bs + j * a.k_ts + hk * a.k_hs;
   const T* v = (const T*)a.v + b * a.v_bs + j * a.v_ts + hk * a.v_hs;
   const int d0 = lane, d1 = lane + 64;
-  const bool on0 = d0 < a.D, on1 = d1 < a.D;
+  T* dk = (T*)a.dk + b * a.dk_bs + j * a.dk_ts + hk * a.dk_hs;
+  T* dv = (T*)a.dv + b * a.dv_bs + j * a.dv_ts + hk * a.dv_hs;
+  const int e0 = min(d0, a.D - 1), e1 = min(d1, a.D - 1);
+  const bool k0 = want_dk && no_number<T>(dk + e0, d0 < a.D), k1 = want_dk && no_number<T>(dk + e1, d1 < a.D);
+  const bool v0 = want_dv && no_number<T>(dv + e0, d0 < a.D), v1 = want_dv && no_number<T>(dv + e1, d1 < a.D);
   const float c = a.scale * kLog2e;
   const int ilo = max(0, j - a.right - s.shift), ihi = j < a.sinks ? s.ql - 1 : min(s.ql - 1, j + a.left - s.shift);
   const int rlo = ilo * a.G, rhi = (ihi + 1) * a.G;
@@ -1578,19 +1588,17 @@ __device__ __forceinline__ void dkv_again(const WaArgs& a, const Seq& s, int b, 
       const T* q = (const T*)a.q + b * a.q_bs + at * a.q_ts + hn * a.q_hs;
       const T* dO = (const T*)a.dout + b * a.do_bs + at * a.do_ts + hn * a.do_hs;
       const float pn = __shfl(p, n, 64), dn = __shfl(ds, n, 64);
-      dv0 = fmaf(pn, on0 ? Elem<T>::ld(dO + d0) : 0.f, dv0);
-      dv1 = fmaf(pn, on1 ? Elem<T>::ld(dO + d1) : 0.f, dv1);
-      dk0 = fmaf(dn, on0 ? Elem<T>::ld(q + d0) : 0.f, dk0);
-      dk1 = fmaf(dn, on1 ? Elem<T>::ld(q + d1) : 0.f, dk1);
+      dv0 = fmaf(pn, v0 ? Elem<T>::ld(dO + d0) : 0.f, dv0);
+      dv1 = fmaf(pn, v1 ? Elem<T>::ld(dO + d1) : 0.f, dv1);
+      dk0 = fmaf(dn, k0 ? Elem<T>::ld(q + d0) : 0.f, dk0);
+      dk1 = fmaf(dn, k1 ? Elem<T>::ld(q + d1) : 0.f, dk1);
     }
-    if (__all((!on0 || (dk0 != dk0 && dv0 != dv0)) && (!on1 || (dk1 != dk1 && dv1 != dv1)))) break;   // it is what it is
+    if (__all((!k0 || dk0 != dk0) && (!k1 || dk1 != dk1) && (!v0 || dv0 != dv0) && (!v1 || dv1 != dv1))) break;
   }
-  T* dk = (T*)a.dk + b * a.dk_bs + j * a.dk_ts + hk * a.dk_hs;
-  T* dv = (T*)a.dv + b * a.dv_bs + j * a.dv_ts + hk * a.dv_hs;
-  if (on0 && want_dk) dk[d0] = (T)(dk0 * a.scale);
-  if (on1 && want_dk) dk[d1] = (T)(dk1 * a.scale);
-  if (on0 && want_dv) dv[d0] = (T)dv0;
-  if (on1 && want_dv) dv[d1] = (T)dv1;
+  if (k0) dk[d0] = (T)(dk0 * a.scale);
+  if (k1) dk[d1] = (T)(dk1 * a.scale);
+  if (v0) dv[d0] = (T)dv0;
+  if (v1) dv[d1] = (T)dv1;
 }
 
 // What the dK / dV kernel walks over the rows with: RS rows a stage (q, dout and their statistics), two stages for bf16
