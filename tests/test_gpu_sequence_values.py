@@ -276,3 +276,31 @@ def test_one_channel_of_one_value_spoils_one_channel_of_its_rows(bad, dtype):
         for h in range(H):
             R.check("out", out[b, :, h][keep], ref[0][b, :, h][keep], ref[1][b, :, h][keep])
             assert not torch.isfinite(out[b, 700:, h, 5]).any()
+
+
+# ---- offsets beyond 32 bits in the backward pass --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+def test_gradients_at_offsets_beyond_32_bits(dtype):
+    """Batches 2^31 elements and more apart, and tokens whose indexes times their stride pass 2^31 elements; results are those of packed tensors."""
+    A = _att()
+    B, T, H, D, es = 2, 300, 2, 32, 2 if dtype == torch.bfloat16 else 4
+    x = [_normal(B, T, H, D, dtype=dtype, seed=n).cuda() for n in range(4)]
+    far_token = (1 << 24) // es - 64                           # just below 16 MiB
+    ts = far_token - far_token % 8
+    assert es == 4 or T * ts > 1 << 31
+    room = torch.empty(max((1 << 31) + 64 + T * H * D, (T * ts if es == 2 else 0) + 1024), dtype=dtype, device="cuda")
+
+    def run(q, k, v, do):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        out = A.window_attention(q, k, v, 40, 9, 5)
+        return (out.detach(),) + torch.autograd.grad(out, (q, k, v), do)
+    want = run(*x)
+    strides = {"batches": ((1 << 31) + 64, H * D, D)}
+    if es == 2:
+        strides["tokens"] = (512, ts, D)
+    for name, st in strides.items():
+        for n in range(4):                                      # one operand at a time
+            far = room.as_strided((B, T, H, D), st + (1,))
+            far.copy_(x[n])
+            got = run(*(far if m == n else t for m, t in enumerate(x)))
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (name, n)
