@@ -15,6 +15,7 @@
 #include "tdx_common.h"
 
 #include <algorithm>
+#include <bit>
 #include <cmath>
 #include <type_traits>
 
@@ -39,7 +40,7 @@ struct WaArgs {
   long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;
   int B, Tq, Tk, Hkv, G, D;
   int left, right, sinks;
-  float scale;
+  float scale, down, up;              // exponentials are taken 2^down smaller, up = 2^down (see softmax_exp)
   const int *q_lens, *k_lens;
   int ntiles, nsplit;                 // row (backward: or key) tiles of a (batch, key head); key (backward: row) splits
   float* ws;
@@ -607,6 +608,8 @@ __device__ __forceinline__ float softmax_max(const float (&s)[16], float& m, flo
   for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
   return softmax_follow<ND>(half_max(t), m, l, o, c, slack);
 }
+// Every exponent is also lowered by a.down = 8 + log2 Tk, so that a row's exponentials sum to at most 1 before they are normalised too, and their sum with values
+// next to the largest stays a number; at the other end values lose what lies below 2^(down - 149).
 // exp2(s c - mc) in one fused step is exact enough while the rounding of mc = m c is small; beyond 2^22 the scores are moved by m first
 template <int NS>
 __device__ __forceinline__ void softmax_huge(float (&s)[NS][16], float m, float& mc) {
@@ -683,10 +686,9 @@ __device__ __forceinline__ bool no_number(const T* at, bool on) {
   return on && !(__builtin_fabsf(Elem<T>::ld(at)) < INFINITY);
 }
 
-// A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN; and sums of exponentials (up to 2^8 each) times values next
-// to the largest are infinite where their mean is not.  A row whose sum of exponentials is a number but whose result is not, or is infinite, is therefore taken
-// again, over the keys it sees alone: one wave, 32 keys at a time, a running mean (whose weights sum to 1 whatever the scores, so that it never leaves the range
-// of its values), the lanes split the channels.
+// A product over a tile also adds 0 times what stands at unseen keys, and 0 times an infinity is NaN.  A row whose sum of exponentials is
+// a number but whose result is not is therefore taken again, over the keys it sees alone: one wave, 32 keys at a time, a running mean (its weights sum to 1 whatever
+// the scores), the lanes split the channels.
 template <typename T>
 __device__ __forceinline__ void row_again(const WaArgs& a, const Seq& s, int b, int hk, int r, int lane) {
   fresh(lane);
@@ -866,6 +868,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
           for (int e = 0; e < 16; ++e) t = fmaxf(t, sc[n][e]);
         float mc = softmax_follow<ND>(half_max(t), m, l, o, c, slack);
         softmax_huge<2>(sc, m, mc);
+        mc += a.down;
         softmax_exp<0, 16>(sc[0], l, mc, c);
         pack16<N>(pb, sc[0]);
         // the exponentials of the second half stand between the products of the first with V
@@ -886,6 +889,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
         if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
         float mc = softmax_max<ND>(sc[0], m, l, o, c, slack);
         softmax_huge<1>(sc, m, mc);
+        mc += a.down;
         softmax_exp<0, 16>(sc[0], l, mc, c);
         pack16<N>(pb, sc[0]);
         cols16<N, DP, S0 + W::TILE, W::PLANE>(o, off, pb);
@@ -906,11 +910,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
-          bad |= !(__builtin_fabsf(v[x]) < INFINITY);
+          bad |= v[x] != v[x];
         }
         if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
       }
-    if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l) : -INFINITY;
+    if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l * a.up) : -INFINITY;
   }
   uint64_t again = __ballot(bad && row_ok && l == l);
   again = (again | (again >> 32)) & 0xffffffffull;
@@ -1020,6 +1024,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
         if (cls == 1) mask_scores(sc[0], a, s, j0, p, lane);
         float mc = softmax_max<G::ND>(sc[0], m, l, o, c, slack);
         softmax_huge<1>(sc, m, mc);
+        mc += a.down;
         softmax_exp<0, 16>(sc[0], l, mc, c);
         cols_times<DP>(o, vt, 0, sc[0], lane, T());
       }
@@ -1041,11 +1046,11 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             v[x] = inv != 0.f ? o[d][4 * e + x] * inv : (l != l ? l : 0.f);
-            bad |= !(__builtin_fabsf(v[x]) < INFINITY);
+            bad |= v[x] != v[x];
           }
           if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
         }
-      if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l) : -INFINITY;
+      if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l * a.up) : -INFINITY;
     }
     uint64_t again = __ballot(bad && row_ok && l == l);
     again = (again | (again >> 32)) & 0xffffffffull;
@@ -1108,10 +1113,10 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         v[x] = inv != 0.f ? oo[x] * inv : (ll != ll ? ll : 0.f);
-        bad |= !(__builtin_fabsf(v[x]) < INFINITY);
+        bad |= v[x] != v[x];
       }
       if (d < a.D) store_out<T>(a, b, ii, hk * a.G + gg, d, v);
-      if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? mm * a.scale + __logf(ll) : -INFINITY;
+      if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? mm * a.scale + __logf(ll * a.up) : -INFINITY;
     }
     uint64_t again = __ballot(bad && ok && ll == ll);
     while (again) {                                                              // D4 (8 .. 32) lanes hold a row
@@ -1186,10 +1191,10 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     v[x] = inv != 0.f ? O[x] * inv : (L != L ? L : 0.f);
-    bad |= !(__builtin_fabsf(v[x]) < INFINITY);
+    bad |= v[x] != v[x];
   }
   if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store_out<T>(a, b, i, hk * a.G + g, 4 * threadIdx.x, v);
-  if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L) : -INFINITY;
+  if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L * a.up) : -INFINITY;
   if (__ballot(bad && ok && L == L)) row_again<T>(a, s, b, hk, rr, threadIdx.x);
 #endif
 }
@@ -1979,6 +1984,7 @@ int translate(const tdx_window_attn_desc* d, WaArgs& a, const char* fn) {
   a.v_bs = d->v_bs, a.v_ts = d->v_ts, a.v_hs = d->v_hs, a.o_bs = d->out_bs, a.o_ts = d->out_ts, a.o_hs = d->out_hs;
   a.B = d->B, a.Tq = d->Tq, a.Tk = d->Tk, a.Hkv = d->Hkv, a.G = d->Hq / d->Hkv, a.D = d->D, a.scale = d->scale;
   a.q_lens = d->q_lens, a.k_lens = d->k_lens;
+  a.down = (float)(8 + std::bit_width((uint32_t)d->Tk)), a.up = std::ldexp(1.f, (int)a.down);
   a.out_lo = d->dtype == TDX_BF16 ? (__bf16*)d->out_lo : nullptr;
   TDX_CHECK_ARG(((uintptr_t)a.out_lo & 15) == 0, "%s: misaligned out_lo", fn);
   // a limit beyond every length is none; sinks that hold every key too
