@@ -302,7 +302,7 @@ class _Form:
     __slots__ = ("desc", "ws", "lse_shape", "bwd", "bwd_key", "bwd_ws")
 
 
-def _form(q, k, v, left, right, sinks, scale, q_lens, k_lens) -> _Form:
+def _form(q, k, v, left, right, sinks, scale) -> _Form:
     key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), v.stride(), left, right, sinks, scale)
     known = _known("attention")
     f = known.get(key)
@@ -324,7 +324,7 @@ def _forward(q, k, v, left, right, sinks, scale, q_lens, k_lens, want_lse, out_l
     out = q.new_empty(q.shape)
     if out.numel() == 0:
         return out, q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32) if want_lse else None
-    f = _form(q, k, v, left, right, sinks, scale, q_lens, k_lens)
+    f = _form(q, k, v, left, right, sinks, scale)
     lse = q.new_empty(f.lse_shape, dtype=torch.float32) if want_lse else None
     d = f.desc
     d.q, d.k, d.v, d.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
@@ -362,7 +362,7 @@ class _WindowAttention(torch.autograd.Function):
         if dq.numel() == 0 or dk.numel() == 0:
             return (dq.zero_(), dk.zero_(), dv.zero_()) + none
         dout = _fits(dout, 1 << 31)
-        f = _form(q, k, v, *ctx.args, q_lens, k_lens)
+        f = _form(q, k, v, *ctx.args)
         lib = _lib.lib()
         key = dout.stride()
         if f.bwd_key != key:

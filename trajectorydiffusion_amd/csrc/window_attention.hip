@@ -459,7 +459,6 @@ struct Stager<__bf16, DP, ROWS> {
       dma16n<PER>(lds + wave * 1024, v, srd);
     }
   }
-  __device__ __forceinline__ void put(uint32_t, uint32_t) const {}
 };
 template <int DP, int ROWS>
 struct Stager<float, DP, ROWS> {
@@ -1121,7 +1120,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
     uint64_t again = __ballot(bad && ok && ll == ll);
     while (again) {                                                              // D4 (8 .. 32) lanes hold a row
       const int f = __builtin_ctzll(again), row_lane = f - f % D4;
-      again &= ~(((D4 == 64 ? 0ull : (1ull << D4)) - 1) << row_lane);
+      again &= ~(((1ull << D4) - 1) << row_lane);
       row_again<T>(a, s, b, hk, __builtin_amdgcn_readlane(rr, f), lane);
     }
   }
@@ -1523,7 +1522,6 @@ struct PackedStager<__bf16, DP, ROWS, NW> {
       }
     }
   }
-  __device__ __forceinline__ void put(uint32_t) const {}
 };
 template <int DP, int ROWS, int NW>
 struct PackedStager<float, DP, ROWS, NW> {
