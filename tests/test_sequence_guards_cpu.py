@@ -165,3 +165,16 @@ def test_scales_that_leave_32_bits_are_refused(scale):
     for d, f in ((_attn_desc(scale=scale), lib.tdx_window_attention), (_attn_desc(scale=scale, ws=16 * P, ws_bytes=1 << 40), lib.tdx_window_attention_bwd)):
         assert f(C.byref(d), None) == 1 and b"scale" in lib.tdx_last_error()
     assert lib.tdx_window_attention_bwd_ws_bytes(C.byref(_attn_desc(scale=2.3e38))) > 0
+
+
+def test_a_block_pickled_before_there_were_windows_attends_as_it_did():
+    import io
+
+    from trajectorydiffusion_amd import AttnBlock
+    old = AttnBlock(64, 32)
+    del old.__dict__["window_spec"]                       # as such a pickle holds it
+    held = io.BytesIO()
+    torch.save(old, held)
+    held.seek(0)
+    assert torch.load(held, weights_only=False).window_spec is None
+    assert AttnBlock(64, 32, window=5).window_spec.window == 5

@@ -142,6 +142,8 @@ class AttnBlock(_HipBlock):
     up to w away, and the first `sinks` of all; heads splits the channels (at most 128 a head); rotary = base turns q and k by the token's
     index.  The parameters are the same."""
 
+    window_spec: Optional[engine.WindowSpec] = None       # (blocks pickled whole before there were windows have none)
+
     def __init__(self, in_c: int, norm_groups: int, *, heads: int = 1, window: Optional[int] = None, sinks: int = 0,
                  rotary: Optional[float] = None) -> None:
         super().__init__()
