@@ -91,8 +91,9 @@ def test_tracing_is_refused(launches, name):
     assert not launches
     leaf = x.clone().requires_grad_()
     y = f(leaf)
-    with pytest.raises(A.TdxError, match=f"{name}: cannot be traced"):
-        make_fx(lambda g: torch.autograd.grad(y, leaf, g))(torch.ones_like(y))
+    for ahead in (False, True):
+        with pytest.raises(A.TdxError, match=f"{name}: cannot be traced"):
+            make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True), pre_dispatch=ahead)(torch.ones_like(y))
     assert len(launches) == 1
 
 
@@ -102,7 +103,7 @@ def test_modes_that_only_watch_are_no_trace(launches):
 
     from trajectorydiffusion_amd import attention as A
     x, pos = torch.randn(1, 4, 2, 16), torch.zeros(1, 4, 1)
-    with FlopCounterMode(display=False):
+    with FlopCounterMode(display=False), torch.device("cpu"):
         for f in _both(A, pos).values():
             f(x)
     assert launches == ["tdx_rotary_axes", "tdx_window_attention"]

@@ -59,14 +59,14 @@ def _launch(fn, name: str, d, index: int) -> None:
         _lib.check(rc, name)
 
 
-# What a call asks before anything else: is a trace being recorded?  (proxies by dispatch mode, ahead of dispatch, or torch.jit)
-_modes, _modes_ahead, _jit = torch._C._len_torch_dispatch_stack, torch._ops._len_torch_dispatch_stack_pre_dispatch, torch._C._get_tracing_state
+# What a call asks before anything else: may a trace be recorded?  (Proxies come with a dispatch mode, ahead of dispatch with a function mode.)
+_modes, _function_modes, _jit = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack, torch._C._is_tracing
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
 def _refuse_traces(fn: str) -> None:
     """Raises under a trace, which holds torch's operators and not the launch: its result would be memory that nothing wrote."""
-    if _jit() is not None or torch._C._get_dispatch_mode(_PROXY) is not None or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None:
+    if _jit() or torch._C._get_dispatch_mode(_PROXY) is not None or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None:
         raise TdxError(f"{fn}: cannot be traced; call it outside of the traced function")
 
 
@@ -128,7 +128,8 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dout):
         if torch.is_grad_enabled():
             raise TdxError("rotary_axes: second derivatives are not provided")
-        _refuse_traces("rotary_axes")
+        if _modes() or _function_modes() or _jit():
+            _refuse_traces("rotary_axes")
         pos, = ctx.saved_tensors
         sections, bases, layout, inverse = ctx.args
         if dout.stride(3) != 1 and dout.shape[3] != 1:
@@ -222,7 +223,7 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
     out       write here (x itself: in place; no other overlap with x, none with pos); not differentiable
     Differentiable in x (backward only).  Returns a contiguous tensor of x's type."""
     fn = "rotary_axes"
-    if _modes() or _modes_ahead() or _jit() is not None:
+    if _modes() or _function_modes() or _jit():
         _refuse_traces(fn)
     if forward_ad._current_level >= 0:
         _refuse_tangents(fn, x, pos, out)
@@ -353,7 +354,8 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if torch.is_grad_enabled():
             raise TdxError("window_attention: second derivatives are not provided")
-        _refuse_traces("window_attention")
+        if _modes() or _function_modes() or _jit():
+            _refuse_traces("window_attention")
         none = (None,) * 6
         if dout is None:
             return (None, None, None) + none
@@ -439,7 +441,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     those behind q_len, get zeros (lse -inf) and pass no gradient; gradients of keys behind k_len are zero.  Whatever stands at keys a
     query does not see, NaN and infinities too, does not reach it.  Strided tensors are taken as they lie when their channels are
     contiguous and their strides multiples of 16 bytes, else copied.  Differentiable in q, k, v (backward only); results are reproducible."""
-    if _modes() or _modes_ahead() or _jit() is not None:
+    if _modes() or _function_modes() or _jit():
         _refuse_traces("window_attention")
     if forward_ad._current_level >= 0:
         _refuse_tangents("window_attention", q, k, v)
