@@ -59,8 +59,10 @@ def _launch(fn, name: str, d, index: int) -> None:
         _lib.check(rc, name)
 
 
-# What a call asks before anything else: may a trace be recorded?  (Proxies come with a dispatch mode, ahead of dispatch with a function mode.)
+# What a call asks before anything else: may a trace be recorded?  Proxies come with a dispatch mode, ahead of dispatch with a stack of their own and, in the
+# forward pass, a function mode (whose stack is counted in a third of the time).
 _modes, _function_modes, _jit = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack, torch._C._is_tracing
+_modes_ahead = torch._ops._len_torch_dispatch_stack_pre_dispatch
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
@@ -128,7 +130,7 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dout):
         if torch.is_grad_enabled():
             raise TdxError("rotary_axes: second derivatives are not provided")
-        if _modes() or _function_modes() or _jit():
+        if _modes() or _modes_ahead() or _jit():
             _refuse_traces("rotary_axes")
         pos, = ctx.saved_tensors
         sections, bases, layout, inverse = ctx.args
@@ -354,7 +356,7 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if torch.is_grad_enabled():
             raise TdxError("window_attention: second derivatives are not provided")
-        if _modes() or _function_modes() or _jit():
+        if _modes() or _modes_ahead() or _jit():
             _refuse_traces("window_attention")
         none = (None,) * 6
         if dout is None:
