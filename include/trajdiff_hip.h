@@ -449,7 +449,7 @@ int tdx_rotary_axes(const tdx_rotary_desc* host_desc, void* stream);
  *   j < k_len,  j <= p + right,  and (j >= p - left or j < sinks)
  * (left / right < 0: no limit on that side; right = 0 is causal).  Query head h reads key head h / (Hq / Hkv).
  *   out = softmax over the seen keys of (scale q k^T) times v,   lse = log sum exp of the same scores (natural logarithm, fp32),
- * rows that see nothing (rows i >= q_len among them) get out = 0 and lse = -inf.  q_lens / k_lens: device int32 (B), or NULL = Tq / Tk;
+ * rows that see nothing (rows i >= q_len among them) get out = 0 and lse = -inf (below 32 bits, the lse of others is their lowest number).  q_lens / k_lens: device int32 (B), or NULL = Tq / Tk;
  * values are clamped to [0, Tq] / [0, Tk].  What is stored at keys that a row does not see (infinities and NaN too) does not reach it.
  * D: a multiple of 8, at most 128; scale finite, also times log2 e, and > 0; pointers, and the byte sizes of the strides, multiples of 16; the token stride
  * of k and v below 16 MiB; 65 token strides plus one group of head strides of q (and of dout) below 2 GiB.

@@ -304,3 +304,20 @@ def test_gradients_at_offsets_beyond_32_bits(dtype):
             far.copy_(x[n])
             got = run(*(far if m == n else t for m, t in enumerate(x)))
             assert all(torch.equal(a, b) for a, b in zip(got, want)), (name, n)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("form", [(2, 13, 13, 2, 2, 8, 2, 1, 0), (1, 1, 3000, 2, 2, 8, None, 0, 0), (1, 300, 300, 8, 1, 8, 100, 30, 16), (300, 130, 130, 1, 1, 8, 33, 20, 5)])
+def test_rows_whose_scaled_scores_all_lie_below_32_bits(form, dtype):
+    """Their log-sum is none that 32 bits hold, but they see keys: all alike here, so each gets an equal share.  Sums of products are -2.4e38, times a scale of 2."""
+    B, Tq, Tk, Hq, Hkv, D, left, right, sinks = form
+    A = _att()
+    q, k = (torch.full((B, T, H, D), x).to(dtype) for T, H, x in ((Tq, Hq, 3e18), (Tk, Hkv, -1e19)))
+    v, do = (_normal(B, T, H, D, seed=n, dtype=dtype) for n, (T, H) in enumerate(((Tk, Hkv), (Tq, Hq))))
+    zero = torch.zeros_like(q)
+    ref = R.attention(zero, k * 0, v, R.seen(B, Tq, Tk, left, right, sinks), dout=do)      # equal scores
+    x = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out, lse = A.window_attention(*x, left, right, sinks, scale=2.0, return_lse=True)
+    R.check("out", out, *ref["out"])
+    assert (lse < -3.4e38).all() and torch.isfinite(lse).all()
+    R.check("dv", torch.autograd.grad(out, x, do.cuda())[2], *ref["dv"])

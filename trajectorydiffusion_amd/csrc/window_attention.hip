@@ -632,6 +632,11 @@ __device__ __forceinline__ void softmax_exp(float (&s)[16], float& l, float off,
   }
   l += sum;
 }
+// log-sum-exp of a row that sees keys.  Below 32 bits it is their lowest number, -inf is for rows that see none.
+__device__ __forceinline__ float log_sum(const WaArgs& a, float m, float l) {
+  const float x = m * a.scale + __logf(l * a.up);
+  return x < -3.4028235e38f ? -3.4028235e38f : x;
+}
 // scores of keys a row does not see become -inf (element i: key j0 + 8 (i / 4) + 4 h + i % 4)
 __device__ __forceinline__ void mask_scores(float (&s)[16], const WaArgs& a, const Seq& q, int j0, int p, int lane) {
   asm volatile("");   // (a branch, not a select over all tiles)
@@ -913,7 +918,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
         }
         if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
       }
-    if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l * a.up) : -INFINITY;
+    if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? log_sum(a, m, l) : -INFINITY;
   }
   uint64_t again = __ballot(bad && row_ok && l == l);
   again = (again | (again >> 32)) & 0xffffffffull;
@@ -1049,7 +1054,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
           }
           if (32 * d + 8 * e + h4 < a.D) store_out<T>(a, b, i, hk * a.G + g, 32 * d + 8 * e + h4, v);
         }
-      if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? m * a.scale + __logf(l * a.up) : -INFINITY;
+      if (a.lse && lane < 32) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = row_ok && l != 0.f ? log_sum(a, m, l) : -INFINITY;
     }
     uint64_t again = __ballot(bad && row_ok && l == l);
     again = (again | (again >> 32)) & 0xffffffffull;
@@ -1115,7 +1120,7 @@ __global__ __launch_bounds__(256) void window_attn_few_kernel(const WaArgs a) {
         bad |= v[x] != v[x];
       }
       if (d < a.D) store_out<T>(a, b, ii, hk * a.G + gg, d, v);
-      if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? mm * a.scale + __logf(ll * a.up) : -INFINITY;
+      if (a.lse && d == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + gg) * a.Tq + ii] = ok && ll != 0.f ? log_sum(a, mm, ll) : -INFINITY;
     }
     uint64_t again = __ballot(bad && ok && ll == ll);
     while (again) {                                                              // D4 (8 .. 32) lanes hold a row
@@ -1193,7 +1198,7 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
     bad |= v[x] != v[x];
   }
   if ((int)threadIdx.x < D4 && 4 * (int)threadIdx.x < a.D) store_out<T>(a, b, i, hk * a.G + g, 4 * threadIdx.x, v);
-  if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? M * a.scale + __logf(L * a.up) : -INFINITY;
+  if (a.lse && threadIdx.x == 0) a.lse[((long)b * a.Hkv * a.G + hk * a.G + g) * a.Tq + i] = ok && L != 0.f ? log_sum(a, M, L) : -INFINITY;
   if (__ballot(bad && ok && L == L)) row_again<T>(a, s, b, hk, rr, threadIdx.x);
 #endif
 }
