@@ -15,7 +15,8 @@ Single tokens over a cache (B, capacity, Hkv, D) that holds k_lens[b] keys, the 
     out = window_attention(q, k_cache, v_cache, left=4095, right=0, sinks=4, k_lens=k_lens)    # q (B, 1, Hq, D)
 
 Everything runs on torch's current stream of the tensors' device; results are allocated by torch.  No CPU fallback: CPU tensors raise
-TdxError, like shapes, types and limits the kernels do not take.
+TdxError, like shapes, types and limits the kernels do not take, and like a trace (make_fx, torch.export, torch.jit), which would hold the
+empty result and not the launch.
 """
 from __future__ import annotations
 

@@ -331,7 +331,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[N]) {
     p[2] = __builtin_bit_cast(bf16x8, Elem<__bf16>::pack(r));
   }
 }
-// the right operand of cols16: 32 rows' numbers as rows16 left them (element i of a lane is tile row 8 (i / 4) + 4 h + i % 4)
+// the right operand of cols16: 32 rows' numbers as rows16 left them (element i of a lane is tile row 8 (i / 4) + 4 h + i % 4).  bf16 tensors: probabilities and
+// score gradients are rounded to 16 bits here, which the instruction takes on both sides.  Each is off by 2^-9 at most, independently, so a result is off by 1.35
+// to 1.45 times what rounding it once at the end leaves (measured against 64 bits: 0.0023 and 0.0017 of its size); a second plane would double the products with V.
 template <int N>
 __device__ __forceinline__ void pack16(bf16x8 (&b)[2][N], const float (&p)[16]) {
 #pragma unroll
@@ -757,7 +759,7 @@ __device__ __forceinline__ Item xcd_item(int block, int nbh, int per) {
 }
 
 // What the many-row kernels walk over the key tiles with: BN keys a tile, bf16 in two stages of direct loads, fp32 in one stage of planes and
-// one of numbers as they arrive (forward at 128 channels: 128 us with the numbers held in registers, 88 so; 64 keys a tile would leave a compute unit one workgroup)
+// one of numbers as they arrive (forward at 128 channels: 128 us with the numbers held in registers, 84 so; 64 keys a tile would leave a compute unit one workgroup)
 template <typename T, int DP>
 struct Walk {
   static constexpr int N = Planes<T>::N, BN = N == 1 ? 64 : 32, NSTAGE = N == 1 ? 2 : 1;
@@ -808,9 +810,9 @@ __device__ __forceinline__ void walk_keys(const WaArgs& a, const Seq& s, const T
 // ---- forward, many rows: 4 waves x 32 rows ----------------------------------------------------------------------------------------------
 // Bound by the SIMDs, which share their issue between matrix and vector work (a score costs as many cycles of exponential, mask, sum and rounding
 // as of products at 64 channels, half at 128): what helps is waves enough to have both at hand, so registers are held to 2 waves a SIMD at 128
-// channels, 3 or 4 below.  Measured: bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 91 us, 660 TFLOP/s of what is seen (the
-// matrix units are busy 35 % of the time, the vector units 41 %); 16384 tokens, 8 heads of 64 channels, window 1025: 64 us, 540 TFLOP/s; fp32, 8 x
-// 1250 tokens and fewer, 8 heads of 64, window 257: 64 us, 80 TFLOP/s (480 of bf16 products).
+// channels, 3 or 4 below.  Measured, in a row of calls (alone, under the profiler): bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 83 us (94 to
+// 100), 720 TFLOP/s of what is seen (the matrix units are busy 35 % of the time, the vector units 41 %); 16384 tokens, 8 heads of 64 channels, window 1025:
+// 56 us (63 to 67), 610 TFLOP/s; fp32, 8 x 1250 tokens and fewer, 8 heads of 64, window 257: 55 us (63), 93 TFLOP/s (560 of bf16 products).
 template <typename T, int DP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ? 2 : sizeof(T) == 4 ? (DP == 64 ? 3 : 4) : 4))) void window_attn_kernel(const WaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -933,10 +935,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 ?
 // ---- forward, few rows: one 32-row tile per workgroup, its waves (and the splits) share the keys -------------------------------------
 // Single tokens over a cache are bound by the reads of K and V: every wave streams its own key tiles through LDS of its own, so a compute
 // unit has up to 128 KB of direct loads in flight and no wave waits for another before the end.  bf16 has two stages a wave, fp32 one, whose halves
-// are reloaded in turn, which leaves room for four waves at 128 channels too (8 x 4 heads over 8192 keys, window 4096: 75 -> 42 us).  Where a row tile sees two key
+// are reloaded in turn, which leaves room for four waves at 128 channels too (8 x 4 heads over 8192 keys, window 4096: 75 -> 41 us).  Where a row tile sees two key
 // tiles at most (short tracks) a workgroup is one wave and keeps its result in registers: more workgroups fit a compute unit, and there is
 // nothing to join (64 x 8 heads x 13 tokens of 128 channels, fp32: 14 us, latency; 29 with two waves that join).  fp32 splits a tile into
-// planes as it reads it for the scores, which so have the bits that the backward pass sees again; the product with V takes the fp32 matrix instructions: it is
+// planes as it reads it for the scores, which so have the bits that the backward pass sees again (instead of fp32 instructions: 16 x 4 heads of 64 over 4096 keys 33 -> 31 us, 13 tokens of 128
+// 13.1 -> 13.7); the product with V takes the fp32 matrix instructions: it is
 // not what binds it, and a tile that is read once need not be split first.
 // Measured: 64 streams of up to 8192 cached keys, 4 heads of 128 channels in bf16, window 4096: 98 us, 5.3 TB/s (a copy reaches 5.2); one stream of
 // 32768, window 16384: 13 to 15 us and 4 to join, 2.4 TB/s.
@@ -1210,12 +1213,13 @@ __global__ __launch_bounds__(256) void window_attn_join_kernel(const WaArgs a) {
 // the scores' own sums are off (fp32: 3e-5 of P) or a fraction of P's rounding (bf16: 5e-4).  Beyond, P would neither sum to 1 nor stay finite (one key that a row
 // sees alone: P = 1.02 at a score of 1e5, 9 at 1e7): dQ's waves take the maximum m and the sum l of such rows again from the scores as they see them, and
 // P = 2^((s - m) c - log2 l) then.  The forward kernels, dQ and dK / dV have the same bits of s: all add the same products in the same order.  The way there costs
-// rows that do not need it up to 3 % (dK / dV 41.4 -> 42.8 us at 8192 tokens, 8 heads of 64 channels, window 257, bf16; 229 -> 230 at the next line's size).
+// rows that do not need it up to 3 % (dK / dV, bf16: 40.7 -> 42.0 us at 8192 tokens, 8 heads of 64 channels, window 257; 227 -> 234 at dQ's size below), a row
+// that does one more walk over its keys, straight from memory.
 // Two kernels take S and dP again, each in the orientation that leaves its sums in one wave's registers, so nothing is added by atomics
 // and the order of every sum is fixed: dQ walks the keys of 128 rows (like the forward pass), dK / dV walk the rows that see 32 keys a
 // wave.  The sinks are seen by every later row: their rows beyond the window are cut into shares that run as workgroups of their own.
 // dQ, bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 118 us, 766 TFLOP/s; fp32, 16 x 625 tokens and fewer, 8 heads of 128,
-// window 129: 159 us, where one wave has a SIMD to itself (434 registers: the planes of Q and dO alone are 192) and nothing covers its vector work.
+// window 129: 155 us, where one wave has a SIMD to itself (422 registers: the planes of Q and dO alone are 192) and nothing covers its vector work.
 
 template <typename T>
 constexpr float kBuilt = sizeof(T) == 4 ? 128.f : 2048.f;
@@ -1617,7 +1621,7 @@ struct RowWalk {
   // At 128 channels two waves share 32 keys, one for dV and one for dK: each has one accumulator, so two waves fit a SIMD where one with both
   // had it alone, for a quarter more matrix instructions (both take S).  bf16, 2 x 4096 tokens, 16 / 4 heads, window 1024: 241 -> 223 us.
   // fp32 holds its V planes in LDS, 24 KB a wave: 16 x 625 tokens and fewer, 8 heads, window 129: 298 -> 235 us.  At 64 channels too, 12 KB a wave,
-  // where 57 spilled registers become 7: 2048 tokens, 8 / 1 heads, causal: 122 -> 82 us.
+  // where 57 registers were spilled and none is now: 2048 tokens, 8 / 1 heads, causal: 122 -> 82 us.
   static constexpr bool TWO = DP == 128, VLDS = DP >= 64 && N == 3;
   static constexpr int NW = TWO ? 8 : 4;
   // fp32: the dV wave, which has registers and time left, stages for its pair (the dK wave spilled what it held for it:
@@ -1722,7 +1726,7 @@ __device__ __forceinline__ void dkv_step(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP 
 // stage, and every wave leaves its fp32 sums.  Sinks among the 128 keys leave theirs as the first shares.  Where the keys are too few to fill the chip
 // (grouped heads, small batches), the rows of 128 keys are cut into nrow shares too.
 // Bound by the LDS reads of its tiles (each of the four products reads one) and the waits at its barriers, at two waves a SIMD: matrix units busy
-// 38 % of the time, LDS 25 %.  bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 230 us, 524 TFLOP/s of what is seen; 8192 tokens, 8
+// 38 % of the time, LDS 25 %.  bf16, 2 x 4096 tokens, 16 / 4 heads of 128 channels, window 1024: 234 us, 515 TFLOP/s of what is seen; 8192 tokens, 8
 // heads of 64, window 257: 42 us, 420 TFLOP/s.
 template <typename T, int DP, int OCC>
 __global__ __launch_bounds__((RowWalk<T, DP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void window_attn_dkv_kernel(const WaArgs a) {
