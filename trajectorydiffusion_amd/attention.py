@@ -108,13 +108,18 @@ def _rotary_desc(x, pos, sections, bases, layout, inverse, out) -> RotaryDesc:
     return d
 
 
-def _rotary_launch(x, pos, sections, bases, layout, inverse, out) -> None:
+def _rotary_launch(x, pos, sections, bases, layout, inverse, out, given=False) -> None:
+    """given: out is the caller's, and may lie over pos"""
     key = (x.shape, x.stride(), x.dtype, pos.shape, pos.stride(), sections, bases, layout, inverse, None if out.is_contiguous() else out.stride())
     known = _known("rotary")
     d = known.get(key)
     if d is None:
         d = known[key] = _rotary_desc(x, pos, sections, bases, layout, inverse, out)
-    d.x, d.out, d.pos = x.data_ptr(), out.data_ptr(), pos.data_ptr()
+        d.out_bytes, d.pos_bytes = _bytes(out), _bytes(pos)
+    at, pos_at = out.data_ptr(), pos.data_ptr()
+    if given and at < pos_at + d.pos_bytes and pos_at < at + d.out_bytes and _touch(out, pos):
+        raise TdxError("rotary_axes: out overlaps pos")
+    d.x, d.out, d.pos = x.data_ptr(), at, pos_at
     _launch(_lib.lib().tdx_rotary_axes, "tdx_rotary_axes", d, x.get_device())
 
 
@@ -162,18 +167,14 @@ def _rotary_args(x, pos, sections, base, layout) -> Tuple:
     return sections, bases, _LAYOUTS[layout]
 
 
-def _span(t: torch.Tensor) -> Tuple[int, int]:
-    """First byte of t's elements and the one behind the last."""
-    at = t.data_ptr()
-    return at, at + (sum((n - 1) * st for st, n in zip(t.stride(), t.shape)) + 1) * t.element_size()
+def _bytes(t: torch.Tensor) -> int:
+    """From t's first element to behind its last."""
+    return (sum((n - 1) * st for st, n in zip(t.stride(), t.shape)) + 1) * t.element_size()
 
 
 def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the memory between the first and the last element of each has bytes in common."""
-    if not a.numel() or not b.numel():
-        return False
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < b.data_ptr() + _bytes(b) and b.data_ptr() < a.data_ptr() + _bytes(a)
 
 
 def _reached(far: int, dims: Sequence[Tuple[int, int, int]]) -> bool:
@@ -196,10 +197,10 @@ def _reached(far: int, dims: Sequence[Tuple[int, int, int]]) -> bool:
 
 
 def _touch(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the two share a byte."""
+    """Whether the two, which have elements, share a byte."""
     ea, eb = a.element_size(), b.element_size()
     dims = [(st * ea, 0, n - 1) for st, n in zip(a.stride(), a.shape)] + [(st * eb, 1 - n, 0) for st, n in zip(b.stride(), b.shape)]
-    return _meet(a, b) and _reached(b.data_ptr() - a.data_ptr(), dims + [(1, 1 - eb, ea - 1)])
+    return _reached(b.data_ptr() - a.data_ptr(), dims + [(1, 1 - eb, ea - 1)])
 
 
 def _clash(x: torch.Tensor, out: torch.Tensor) -> bool:
@@ -260,10 +261,8 @@ def rotary_axes(x: torch.Tensor, pos: torch.Tensor, sections: Sequence[int], bas
             raise TdxError(f"{fn}: out must not repeat its own memory")
         if out is not x and _clash(x, out):
             raise TdxError(f"{fn}: out overlaps x other than in place")
-        if _touch(out, pos):
-            raise TdxError(f"{fn}: out overlaps pos")
         if x.numel():
-            _rotary_launch(x, pos, sections, bases, code, bool(inverse), out)
+            _rotary_launch(x, pos, sections, bases, code, bool(inverse), out, given=True)
             torch.autograd.graph.increment_version(out)   # the launch writes behind autograd's back
         return out
     if x.requires_grad and torch.is_grad_enabled():
