@@ -453,7 +453,7 @@ int tdx_rotary_axes(const tdx_rotary_desc* host_desc, void* stream);
  * values are clamped to [0, Tq] / [0, Tk].  What is stored at keys that a row does not see (infinities and NaN too) does not reach it.
  * D: a multiple of 8, at most 128; scale finite, also times log2 e, and > 0; pointers, and the byte sizes of the strides, multiples of 16; the token stride
  * of k and v below 16 MiB; 65 token strides plus one group of head strides of q (and of dout) below 2 GiB.
- * All finite numbers are taken as they are (fp32 down to a step of 2^-133); an infinity that a row sees in k (or has in q) makes its result NaN in fp32.
+ * All finite numbers are taken as they are (fp32 down to a step of 2^-133, v of 2^(log2 Tk - 140)); an infinity that a row sees in k (or has in q) makes its result NaN in fp32.
  * Softmax statistics and sums are fp32; with bf16 tensors the probabilities (and score gradients) are rounded to bf16 before the
  * products that take them, the results once at the end.  Summation orders are fixed: results are reproducible. */
 typedef struct {
